@@ -40,7 +40,12 @@ typedef enum WsvdStatus {
   WSVD_ERR_TOO_LARGE = 8         /* size beyond a documented fixed limit */
 } WsvdStatus;
 
-typedef enum WsvdDtype { WSVD_I8 = 0, WSVD_F16 = 1, WSVD_F32 = 2 /* quant-append input only */ } WsvdDtype;
+typedef enum WsvdDtype {
+  WSVD_I8 = 0,
+  WSVD_F16 = 1,
+  WSVD_F32 = 2,  /* quant-append input only */
+  WSVD_BF16 = 3  /* wsvd_kv_rope_append, wsvd_paged_decode and wsvd_adapter_add only */
+} WsvdDtype;
 typedef enum WsvdRopeLayout { WSVD_ROPE_HALF = 0, WSVD_ROPE_INTERLEAVED = 1 } WsvdRopeLayout;
 
 /* Which stage-1 kernel to run.  AUTO picks the tcgen05 kernel when the shape allows. */
@@ -119,8 +124,11 @@ int wsvd_rope_table_init(void* table, size_t table_bytes, int32_t positions, int
  * Device-side status of the kernels: 0, or the highest code recorded since the last reset:
  * 1-3 a bounded wait of the tensor-core kernel timed out (1 copy issuer, 2 MMA issuer,
  * 3 epilogue), 4 its shared-memory base was misaligned, 5 wsvd_latent_quant_append_i8 met
- * a position outside [0, max_len) and skipped that row, 6 the group barrier of
- * wsvd_latent_decode_gather gave up waiting for a peer.  SYNCHRONISES the device; meant
+ * a position outside [0, max_len) and skipped that row (wsvd_kv_rope_append too; wsvd_paged_decode met a
+ * length beyond the page table's width and left the rest out), 6 the group barrier of
+ * wsvd_latent_decode_gather gave up waiting for a peer, 7 wsvd_kv_rope_append or wsvd_paged_decode met a
+ * token slot outside the cache or a request outside the page table and left it out, or wsvd_adapter_add an adapter
+ * that does not exist.  SYNCHRONISES the device; meant
  * for tests and diagnostics, and for a serving loop to poll at a point where it synchronises
  * anyway.  wsvd_kernel_status_reset clears it.  A tensor-core work item whose wait timed out
  * writes NaN instead of its result, so the affected output rows are NaN, not plausible numbers.
@@ -248,6 +256,106 @@ typedef struct WsvdQuantAppendParams {
   int32_t x_dtype;          /* WSVD_F16 or WSVD_F32 */
 } WsvdQuantAppendParams;
 int wsvd_latent_quant_append_i8(const WsvdQuantAppendParams* p, void* stream);
+
+/*
+ * The dense counterpart of the cache producer, for prompts, chunks of them and single tokens: rotate new keys
+ * (and, beside them, queries) to their positions and store keys and values in the token slots of the page table.
+ *
+ *   k, v [rows, Hkv, D], q [rows, Hq, D] (optional), f16 or bf16: rows packed by sequence, cu_new [batch + 1] int32 the
+ *   first row of each (NULL: one row per sequence, rows == batch).  Row i of sequence b has position
+ *   pos = b_seq_len[b] + i (b_seq_len: lengths BEFORE the append) and goes to token slot
+ *   req_to_token[b_req_idx[b]][pos]; its rotation angles are (pos + pos_offset[b]) * inv_freq[j], j < rot_dim / 2, the
+ *   exact product of the integer and the f32 frequency.  The first rot_dim dims of q and k are rotated, the others and v
+ *   go through.  WSVD_ROPE_HALF pairs (j, j + rot_dim / 2), WSVD_ROPE_INTERLEAVED (2 j, 2 j + 1).
+ *   cache_k, cache_v [T, Hkv, D]: the rows' dtype, or int8 with f16 scales [T, Hkv] per (slot, head): the quantiser of
+ *   wsvd_latent_quant_append_i8 on the rotated f32 row.
+ *   q_out [rows, Hq, D] receives the rotated queries; it may be q itself (same strides).
+ *
+ * Rows behind cu_new[batch] are padding: nothing of them is stored (q_out: left as it was, or zeroed with clear_tail).  A row
+ * whose position is outside [0, max_len) is skipped (status 5), one whose request or slot does not exist too
+ * (status 7); its query is rotated all the same.  Two rows that name one slot leave either's values, head by head.
+ * head_dim <= 256 and even, rot_dim even and <= head_dim.  No counterpart in the reference, whose dense caches are made
+ * by its test script (efficiency/test_timing_layer.py).
+ */
+typedef struct WsvdKvRopeAppendParams {
+  const void* k;            int64_t k_stride_n, k_stride_h;
+  const void* v;            int64_t v_stride_n, v_stride_h;
+  const void* q;            int64_t q_stride_n, q_stride_h;     /* optional */
+  void* q_out;              int64_t qo_stride_n, qo_stride_h;
+  void* cache_k;            int64_t ck_stride_t, ck_stride_h;
+  void* cache_v;            int64_t cv_stride_t, cv_stride_h;
+  void* k_scale;            int64_t ks_stride_t, ks_stride_h;   /* int8 caches only */
+  void* v_scale;            int64_t vs_stride_t, vs_stride_h;
+  const float* inv_freq;    /* [rot_dim / 2] */
+  const int32_t* req_to_token; int64_t rtt_stride;
+  const int32_t* b_req_idx;
+  const int32_t* b_seq_len;
+  const int32_t* cu_new;      /* optional */
+  const int32_t* pos_offset;  /* optional [batch] */
+  int64_t n_token_slots;      /* T */
+  int32_t rows, batch, n_q_heads, n_kv_heads, head_dim, rot_dim;
+  int32_t max_len, n_req;     /* columns and rows of req_to_token */
+  int32_t dtype, cache_dtype; /* WsvdDtype: F16 or BF16; the same or I8 */
+  int32_t rope_layout;        /* WsvdRopeLayout */
+  int32_t clear_tail;
+} WsvdKvRopeAppendParams;
+int wsvd_kv_rope_append(const WsvdKvRopeAppendParams* p, void* stream);
+
+/*
+ * Attention of one new token per sequence over a paged cache [T, Hkv, D], K stored rotated, as wsvd_kv_rope_append
+ * leaves it:  out = sum_s softmax_s(sm_scale q . k_s) v_s over the positions max(0, len - window) <= s < len
+ * (window 0: all), q and out [B, Hq, D] f16 or bf16; the caches have q's dtype, or are int8 with f16 scales [T, Hkv].
+ * The query heads of a KV head share its loads.  lse (optional, f32 [B, Hq] contiguous): log of the sum of
+ * exp(sm_scale q . k_s).  A sequence without positions gives zeros and -inf.
+ * What is stored in slots that no position of the call names is never read.  A page-table entry outside [0, T) is left out
+ * as if it were masked, a request outside the table leaves its sequence empty (status 7); a length beyond max_len is
+ * clamped to it (status 5).
+ * wsvd_dense_decode_f16 is the reference's dense baseline (f16, each query head for itself); this is the serving form.
+ */
+typedef struct WsvdPagedDecodeParams {
+  const void* q;            int64_t q_stride_b, q_stride_h;
+  const void* k;            int64_t k_stride_t, k_stride_h;
+  const void* v;            int64_t v_stride_t, v_stride_h;
+  const void* k_scale;      int64_t ks_stride_t, ks_stride_h;   /* int8 caches only */
+  const void* v_scale;      int64_t vs_stride_t, vs_stride_h;
+  const int32_t* req_to_token; int64_t rtt_stride;
+  const int32_t* b_req_idx;
+  const int32_t* b_seq_len;
+  void* out;                int64_t out_stride_b, out_stride_h;
+  float* lse;               /* optional */
+  int64_t n_token_slots;    /* T */
+  int32_t batch, n_q_heads, n_kv_heads, head_dim;
+  int32_t max_len, n_req;   /* columns and rows of req_to_token */
+  int32_t dtype, cache_dtype;
+  int32_t window;           /* 0: none */
+  float sm_scale;           /* 0 = 1/sqrt(head_dim) */
+} WsvdPagedDecodeParams;
+size_t wsvd_paged_decode_workspace_bytes(const WsvdPagedDecodeParams* p);
+int wsvd_paged_decode(const WsvdPagedDecodeParams* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Low-rank adapters of many requests beside a shared projection:
+ *   out[n] = y[n] + scale[i] (x[n] A_i) B_i,   i = adapter[request of row n]  (-1: out[n] = y[n])
+ * y, out [rows, n_out], x [rows, n_in], A [n_adapters, n_in, rank], B [n_adapters, rank, n_out], all f16 or all bf16,
+ * innermost stride 1; adapter [batch] int32; scale (optional) f32 [n_adapters].  Rows are packed by request, cu_new as
+ * above (NULL: one row per request).  x A is summed in f32.  out may be y (same stride), and must not overlap x.
+ * Rows behind cu_new[batch] are padding: left as they were, or copied from y with copy_tail.  An adapter outside [-1, n_adapters) adds nothing (status 7).  rank <= 256.
+ */
+typedef struct WsvdAdapterAddParams {
+  const void* y;            int64_t y_stride;
+  const void* x;            int64_t x_stride;
+  const void* a;            int64_t a_stride_i, a_stride_k;
+  const void* b;            int64_t b_stride_i, b_stride_r;
+  void* out;                int64_t out_stride;
+  const int32_t* adapter;
+  const float* scale;       /* optional */
+  const int32_t* cu_new;    /* optional */
+  int32_t rows, batch, n_in, n_out, rank, n_adapters;
+  int32_t dtype;
+  int32_t copy_tail;
+} WsvdAdapterAddParams;
+size_t wsvd_adapter_add_workspace_bytes(const WsvdAdapterAddParams* p);
+int wsvd_adapter_add(const WsvdAdapterAddParams* p, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Element-wise pieces of the decode step around the attention op, one kernel each (in the

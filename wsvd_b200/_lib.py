@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes
 import os
 import shutil
+import struct
 import subprocess
 import threading
 
@@ -19,7 +20,7 @@ LIB_PATH = os.path.join(_PKG, "libwsvd_b200.so")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC", "-shared", "--threads", "0",
 ]
 
 _lock = threading.Lock()
@@ -140,6 +141,78 @@ class QuantAppendParams(ctypes.Structure):
     ]
 
 
+class KvRopeAppendParams(ctypes.Structure):
+    """ctypes mirror of WsvdKvRopeAppendParams."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("k_stride_n", ctypes.c_int64), ("k_stride_h", ctypes.c_int64),
+        ("v", ctypes.c_void_p), ("v_stride_n", ctypes.c_int64), ("v_stride_h", ctypes.c_int64),
+        ("q", ctypes.c_void_p), ("q_stride_n", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p), ("qo_stride_n", ctypes.c_int64), ("qo_stride_h", ctypes.c_int64),
+        ("cache_k", ctypes.c_void_p), ("ck_stride_t", ctypes.c_int64), ("ck_stride_h", ctypes.c_int64),
+        ("cache_v", ctypes.c_void_p), ("cv_stride_t", ctypes.c_int64), ("cv_stride_h", ctypes.c_int64),
+        ("k_scale", ctypes.c_void_p), ("ks_stride_t", ctypes.c_int64), ("ks_stride_h", ctypes.c_int64),
+        ("v_scale", ctypes.c_void_p), ("vs_stride_t", ctypes.c_int64), ("vs_stride_h", ctypes.c_int64),
+        ("inv_freq", ctypes.c_void_p),
+        ("req_to_token", ctypes.c_void_p), ("rtt_stride", ctypes.c_int64),
+        ("b_req_idx", ctypes.c_void_p), ("b_seq_len", ctypes.c_void_p),
+        ("cu_new", ctypes.c_void_p), ("pos_offset", ctypes.c_void_p),
+        ("n_token_slots", ctypes.c_int64),
+        ("rows", ctypes.c_int32), ("batch", ctypes.c_int32), ("n_q_heads", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("rot_dim", ctypes.c_int32),
+        ("max_len", ctypes.c_int32), ("n_req", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("cache_dtype", ctypes.c_int32), ("rope_layout", ctypes.c_int32),
+        ("clear_tail", ctypes.c_int32),
+    ]
+
+
+class PagedDecodeParams(ctypes.Structure):
+    """ctypes mirror of WsvdPagedDecodeParams."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("q_stride_b", ctypes.c_int64), ("q_stride_h", ctypes.c_int64),
+        ("k", ctypes.c_void_p), ("k_stride_t", ctypes.c_int64), ("k_stride_h", ctypes.c_int64),
+        ("v", ctypes.c_void_p), ("v_stride_t", ctypes.c_int64), ("v_stride_h", ctypes.c_int64),
+        ("k_scale", ctypes.c_void_p), ("ks_stride_t", ctypes.c_int64), ("ks_stride_h", ctypes.c_int64),
+        ("v_scale", ctypes.c_void_p), ("vs_stride_t", ctypes.c_int64), ("vs_stride_h", ctypes.c_int64),
+        ("req_to_token", ctypes.c_void_p), ("rtt_stride", ctypes.c_int64),
+        ("b_req_idx", ctypes.c_void_p), ("b_seq_len", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("out_stride_b", ctypes.c_int64), ("out_stride_h", ctypes.c_int64),
+        ("lse", ctypes.c_void_p),
+        ("n_token_slots", ctypes.c_int64),
+        ("batch", ctypes.c_int32), ("n_q_heads", ctypes.c_int32), ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("max_len", ctypes.c_int32), ("n_req", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("cache_dtype", ctypes.c_int32), ("window", ctypes.c_int32),
+        ("sm_scale", ctypes.c_float),
+    ]
+
+
+class AdapterAddParams(ctypes.Structure):
+    """ctypes mirror of WsvdAdapterAddParams."""
+
+    _fields_ = [
+        ("y", ctypes.c_void_p), ("y_stride", ctypes.c_int64),
+        ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+        ("a", ctypes.c_void_p), ("a_stride_i", ctypes.c_int64), ("a_stride_k", ctypes.c_int64),
+        ("b", ctypes.c_void_p), ("b_stride_i", ctypes.c_int64), ("b_stride_r", ctypes.c_int64),
+        ("out", ctypes.c_void_p), ("out_stride", ctypes.c_int64),
+        ("adapter", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("cu_new", ctypes.c_void_p),
+        ("rows", ctypes.c_int32), ("batch", ctypes.c_int32), ("n_in", ctypes.c_int32), ("n_out", ctypes.c_int32),
+        ("rank", ctypes.c_int32), ("n_adapters", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("copy_tail", ctypes.c_int32),
+    ]
+
+
+def packer(cls):
+    """A function of a structure's fields, in order, that gives the structure's bytes (pointers as whole numbers, 0 for
+    none): a tenth of the time that filling the ctypes structure takes, which is most of a small call's."""
+    code = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f"}
+    s = struct.Struct("@" + "".join(code[t] for _, t in cls._fields_))
+    assert s.size <= ctypes.sizeof(cls) < s.size + 8  # C pads the end to the widest field, struct does not
+    s = struct.Struct(s.format + f"{ctypes.sizeof(cls) - s.size}x")
+    return s.pack
+
+
 MAX_PEERS = 8
 PEER_HANDLE_BYTES = 64
 
@@ -184,6 +257,12 @@ SYMBOLS = {
     "wsvd_peer_import": (ctypes.c_int, [ctypes.c_char_p, ctypes.POINTER(ctypes.c_void_p)]),
     "wsvd_peer_release": (ctypes.c_int, [ctypes.c_void_p]),
     "wsvd_latent_quant_append_i8": (ctypes.c_int, [ctypes.POINTER(QuantAppendParams), ctypes.c_void_p]),
+    # (c_void_p: the bytes of a packed structure, or byref of one)
+    "wsvd_kv_rope_append": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "wsvd_paged_decode_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "wsvd_paged_decode": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    "wsvd_adapter_add_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p]),
+    "wsvd_adapter_add": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "wsvd_rms_norm_f16": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32, ctypes.c_int32,
                                          ctypes.c_float, ctypes.c_void_p]),
     "wsvd_add_rms_norm_f16": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,

@@ -4,6 +4,7 @@
 #include <string.h>
 
 #include "common.cuh"
+#include "dense_ops.cuh"
 
 namespace {
 
@@ -305,7 +306,7 @@ const char* wsvd_status_string(int status) {
     case WSVD_ERR_BAD_SHAPE: return "unsupported head_dim / rank / head count / length";
     case WSVD_ERR_BAD_DTYPE: return "unknown dtype or layout code, or int8 data without its scales";
     case WSVD_ERR_BAD_STRIDE: return "stride or alignment precondition violated";
-    case WSVD_ERR_WORKSPACE_TOO_SMALL: return "workspace smaller than wsvd_latent_decode_workspace_bytes()";
+    case WSVD_ERR_WORKSPACE_TOO_SMALL: return "workspace smaller than the entry point's ..._workspace_bytes()";
     case WSVD_ERR_CUDA: return "a CUDA runtime call failed (see wsvd_last_cuda_error)";
     case WSVD_ERR_UNSUPPORTED: return "no kernel in this build for the requested combination";
     case WSVD_ERR_TOO_LARGE: return "size beyond a fixed limit of this entry point";
@@ -365,12 +366,17 @@ int wsvd_rope_table_init(void* table, size_t table_bytes, int32_t positions, int
 
 int wsvd_kernel_status(uint32_t* status) {
   if (!status) return WSVD_ERR_NULL_POINTER;
-  unsigned int v = 0, w = 0, x = 0;
+  unsigned int v = 0, w = 0, x = 0, dense[3] = {0, 0, 0};
   cudaError_t e = wsvd::read_tc_status(&v);
   if (e == cudaSuccess) e = wsvd::read_append_status(&w);
   if (e == cudaSuccess) e = wsvd::read_peer_status(&x);
+  if (e == cudaSuccess) e = wsvd::read_kv_append_status(&dense[0]);
+  if (e == cudaSuccess) e = wsvd::read_paged_decode_status(&dense[1]);
+  if (e == cudaSuccess) e = wsvd::read_adapter_status(&dense[2]);
   *status = v > w ? v : w;
   if (x > *status) *status = x;
+  for (unsigned int d : dense)
+    if (d > *status) *status = d;
   return e == cudaSuccess ? WSVD_OK : cuda_fail(e);
 }
 
@@ -378,6 +384,9 @@ int wsvd_kernel_status_reset(void) {
   cudaError_t e = wsvd::reset_tc_status();
   if (e == cudaSuccess) e = wsvd::reset_append_status();
   if (e == cudaSuccess) e = wsvd::reset_peer_status();
+  if (e == cudaSuccess) e = wsvd::reset_kv_append_status();
+  if (e == cudaSuccess) e = wsvd::reset_paged_decode_status();
+  if (e == cudaSuccess) e = wsvd::reset_adapter_status();
   return e == cudaSuccess ? WSVD_OK : cuda_fail(e);
 }
 

@@ -451,6 +451,293 @@ def latent_quant_append(x_k, x_v, infer_state, cache_latent_k, cache_latent_k_sc
         check(_lib.lib().wsvd_latent_quant_append_i8(ctypes.byref(p), _stream(stream)), "wsvd_latent_quant_append_i8")
 
 
+# ---- the dense attention block of a step: adapters beside a projection, rotate-and-append, attention over the paged cache
+
+BF16 = 3
+_CODE = {torch.float16: F16, torch.bfloat16: BF16, torch.int8: I8}
+_HALVES = (torch.float16, torch.bfloat16)
+_pack_append = _lib.packer(_lib.KvRopeAppendParams)
+_pack_paged = _lib.packer(_lib.PagedDecodeParams)
+_pack_adapter = _lib.packer(_lib.AdapterAddParams)
+
+
+def _tensor(name, t, dtypes, ndim, inner_contiguous=True):
+    """As `_cuda_tensor`, the device left to `_on_one_gpu`."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected one of {dtypes}")
+    if t.dim() != ndim:
+        raise ValueError(f"{name} must have {ndim} dims, got {tuple(t.shape)}")
+    if inner_contiguous and t.stride(-1) != 1 and t.shape[-1] > 1 and t.numel() != 0:
+        raise ValueError(f"{name}: innermost dimension must be contiguous")
+
+
+def _on_one_gpu(tensors):
+    """The index of the GPU that all of `tensors` (name, tensor or None) are on."""
+    index = tensors[0][1].get_device()
+    for name, t in tensors:
+        if t is not None and t.get_device() != index or index < 0:
+            if t is not None and not t.is_cuda:
+                raise ValueError(f"{name} must be a CUDA tensor (no CPU path exists)")
+            raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
+    return index
+
+
+def _no_gradient(op, *tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{op} has no backward: call it under torch.no_grad() or on detached tensors")
+
+
+def _new(alloc_tensor_func, shape, dtype, device, stream):
+    """A buffer of the op's own.  On a stream of the caller's its memory must not go back to the current stream's pool while
+    that one still works on it."""
+    t = alloc_tensor_func(shape, dtype=dtype, device=device)
+    if stream is not None:
+        t.record_stream(stream)
+    return t
+
+
+def _metadata(infer_state, B):
+    """(b_seq_len, b_req_idx, page table) of a batch of B sequences."""
+    lens, idx, table = infer_state.b_seq_len, infer_state.b_req_idx, infer_state.req_manager.req_to_token_indexs
+    _tensor("b_seq_len", lens, (torch.int32,), 1)
+    _tensor("b_req_idx", idx, (torch.int32,), 1)
+    _tensor("req_to_token_indexs", table, (torch.int32,), 2)
+    if lens.shape[0] != B or idx.shape[0] != B:
+        raise ValueError("batch metadata must have one entry per sequence")
+    return lens, idx, table
+
+
+def _dense_cache(cache_k, cache_v, k_scale, v_scale, dtype, Hkv, D):
+    """Checks of a dense cache [T, Hkv, D] (and scales [T, Hkv] of an int8 one)."""
+    _tensor("cache_k", cache_k, (dtype, torch.int8), 3)
+    _tensor("cache_v", cache_v, (cache_k.dtype,), 3)
+    if cache_k.shape[1:] != (Hkv, D) or cache_v.shape != cache_k.shape:
+        raise ValueError(f"cache_k and cache_v must be [T, {Hkv}, {D}], got {tuple(cache_k.shape)} and {tuple(cache_v.shape)}")
+    if cache_k.dtype == torch.int8:
+        if k_scale is None or v_scale is None:
+            raise TypeError("int8 caches need their scales")
+        for name, t in (("cache_k's scale", k_scale), ("cache_v's scale", v_scale)):
+            _tensor(name, t, (torch.float16,), 2, inner_contiguous=False)
+            if t.shape != cache_k.shape[:2]:
+                raise ValueError(f"{name} must be [T, Hkv] = {tuple(cache_k.shape[:2])}, got {tuple(t.shape)}")
+    elif k_scale is not None or v_scale is not None:
+        raise TypeError("only int8 caches have scales")
+
+
+def kv_rope_append(k, v, infer_state, cache_k, cache_v, inv_freq, *, cache_k_scale=None, cache_v_scale=None, q=None,
+                   q_out=None, cu_new=None, pos_offset=None, rope_layout="half", stream=None):
+    """Store new keys and values in the paged cache (in place), the keys rotated to their positions on the way; with `q`,
+    return the queries rotated beside them.  For prompts, chunks of them and single tokens.
+
+    k, v [N, Hkv, D], q [N, Hq, D] (f16 or bf16, any stride between rows and heads: column slices of one joined
+    projection will do) are rows packed by sequence; `cu_new` [B + 1] int32 has each sequence's first row, None means
+    one row per sequence.  Row i of sequence b goes to position ``b_seq_len[b] + i`` in token slot
+    ``req_to_token_indexs[b_req_idx[b], position]``: ``infer_state.b_seq_len`` holds the lengths before the append, the caller
+    adds the new rows afterwards.  The first ``2 * len(inv_freq)`` dims are rotated by ``(position + pos_offset[b]) *
+    inv_freq`` (`rope_layout` as in `latent_decode`), the others and v go through.
+    cache_k, cache_v [T, Hkv, D] in the rows' dtype, or int8 with f16 scales [T, Hkv] (the quantiser of
+    `latent_quant_append`, on the rotated f32 row).  `q_out` may be q.
+
+    Rows behind cu_new[B] are padding: nothing of them is stored, a `q_out` of the caller's keeps its rows, the op's own has
+    zeros there.  A row without a place in the table or the cache is skipped and reported by `kernel_status`.
+    The reference's dense caches are made by its test script (efficiency/test_timing_layer.py)."""
+    _tensor("k", k, _HALVES, 3)
+    dtype = k.dtype
+    _tensor("v", v, (dtype,), 3)
+    N, Hkv, D = k.shape
+    if v.shape != k.shape:
+        raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
+    _tensor("inv_freq", inv_freq, (torch.float32,), 1)
+    rot = 2 * inv_freq.shape[0]
+    if D % 2 or D > 256 or rot > D:
+        raise ValueError(f"head_dim must be even and at most 256, with at most head_dim / 2 frequencies: {D}, {rot // 2}")
+    _dense_cache(cache_k, cache_v, cache_k_scale, cache_v_scale, dtype, Hkv, D)
+    if cu_new is None:
+        B = N
+    else:
+        _tensor("cu_new", cu_new, (torch.int32,), 1)
+        B = cu_new.shape[0] - 1
+        if B < 0:
+            raise ValueError("cu_new must have batch + 1 entries")
+    lens, idx, table = _metadata(infer_state, B)
+    if pos_offset is not None:
+        _tensor("pos_offset", pos_offset, (torch.int32,), 1)
+        if pos_offset.shape[0] != B:
+            raise ValueError("pos_offset must have batch entries")
+    if rope_layout not in ROPE:
+        raise ValueError(f"rope_layout must be one of {list(ROPE)}")
+    own = False
+    Hq = 0
+    if q is not None:
+        _tensor("q", q, (dtype,), 3)
+        Hq = q.shape[1]
+        if q.shape[0] != N or q.shape[2] != D:
+            raise ValueError(f"q must be [{N}, Hq, {D}], got {tuple(q.shape)}")
+        if q_out is not None:
+            _tensor("q_out", q_out, (dtype,), 3)
+            if q_out.shape != q.shape:
+                raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
+            if q_out.data_ptr() == q.data_ptr() and q_out.stride() != q.stride():
+                raise ValueError("q_out may be q itself, not another view of its storage")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    _no_gradient("kv_rope_append", k, v, q, q_out, cache_k, cache_v)
+    index = _on_one_gpu((("k", k), ("v", v), ("q", q), ("q_out", q_out), ("cache_k", cache_k), ("cache_v", cache_v),
+                         ("cache_k_scale", cache_k_scale), ("cache_v_scale", cache_v_scale), ("inv_freq", inv_freq),
+                         ("b_seq_len", lens), ("b_req_idx", idx), ("req_to_token_indexs", table), ("cu_new", cu_new),
+                         ("pos_offset", pos_offset)))
+    if q is not None and q_out is None:
+        own = True
+        q_out = _new(torch.empty, (N, Hq, D), dtype, q.device, stream)
+    i8 = cache_k.dtype == torch.int8
+    args = _pack_append(
+        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+        *((0, 0, 0, 0, 0, 0) if q is None else
+          (q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1))),
+        cache_k.data_ptr(), cache_k.stride(0), cache_k.stride(1), cache_v.data_ptr(), cache_v.stride(0), cache_v.stride(1),
+        *((cache_k_scale.data_ptr(), *cache_k_scale.stride(), cache_v_scale.data_ptr(), *cache_v_scale.stride()) if i8 else
+          (0, 0, 0, 0, 0, 0)),
+        inv_freq.data_ptr(), table.data_ptr(), table.stride(0), idx.data_ptr(), lens.data_ptr(),
+        0 if cu_new is None else cu_new.data_ptr(), 0 if pos_offset is None else pos_offset.data_ptr(), cache_k.shape[0],
+        N, B, Hq, Hkv, D, rot, table.shape[1], table.shape[0], _CODE[dtype], I8 if i8 else _CODE[dtype], ROPE[rope_layout], own)
+    with _on_device(k.device):
+        check(_lib.lib().wsvd_kv_rope_append(args, _stream(stream)), "wsvd_kv_rope_append")
+    return q_out
+
+
+def paged_decode(q, infer_state, cache_k, cache_v, k_scale=None, v_scale=None, *, out=None, return_lse=False, window=0,
+                 sm_scale=0.0, workspace: Optional[torch.Tensor] = None, alloc_tensor_func: Callable = torch.empty,
+                 stream=None):
+    """Attention of one new token per sequence over a paged cache: q [B, Hq, D] (f16 or bf16), caches [T, Hkv, D] in q's
+    dtype or int8 with f16 scales [T, Hkv], as `kv_rope_append` fills them -> [B, Hq, D]; with `return_lse` also the log of
+    the sum of exponentials [B, Hq] f32.
+
+    Sequence b attends to the positions ``max(0, b_seq_len[b] - window) <= s < b_seq_len[b]`` (window 0: all), position s in
+    token slot ``req_to_token_indexs[b_req_idx[b], s]``.  Query heads that share a KV head share its loads.  A
+    sequence without positions gives zeros and -inf.  A page-table entry outside the cache is left out and
+    reported by `kernel_status`, a length is clamped to the table's width.  `sm_scale` 0 means 1/sqrt(D).
+    `workspace`: an optional CUDA byte/float buffer of `paged_decode_workspace_bytes` bytes; calls that may
+    run at the same time need one each.  (`dense_decode` is the reference's f16 baseline.)"""
+    _tensor("q", q, _HALVES, 3)
+    B, Hq, D = q.shape
+    dtype = q.dtype
+    _tensor("cache_k", cache_k, (dtype, torch.int8), 3)
+    Hkv = cache_k.shape[1]
+    if D < 1 or D > 256:
+        raise ValueError(f"head_dim {D} not in [1, 256]")
+    _dense_cache(cache_k, cache_v, k_scale, v_scale, dtype, Hkv, D)
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"q heads ({Hq}) must be a multiple of KV heads ({Hkv})")
+    lens, idx, table = _metadata(infer_state, B)
+    if out is not None:
+        _tensor("out", out, (dtype,), 3)
+        if out.shape != q.shape:
+            raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    window = int(window)
+    if window < 0:
+        raise ValueError("window must not be negative")
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    _no_gradient("paged_decode", q, cache_k, cache_v, out)
+    _on_one_gpu((("q", q), ("cache_k", cache_k), ("cache_v", cache_v), ("k_scale", k_scale), ("v_scale", v_scale),
+                 ("b_seq_len", lens), ("b_req_idx", idx), ("req_to_token_indexs", table), ("out", out),
+                 ("workspace", workspace)))
+    device = q.device
+    if out is None:
+        out = _new(alloc_tensor_func, (B, Hq, D), dtype, device, stream)
+    lse = _new(alloc_tensor_func, (B, Hq), torch.float32, device, stream) if return_lse else None
+    i8 = cache_k.dtype == torch.int8
+    args = _pack_paged(
+        q.data_ptr(), q.stride(0), q.stride(1), cache_k.data_ptr(), cache_k.stride(0), cache_k.stride(1),
+        cache_v.data_ptr(), cache_v.stride(0), cache_v.stride(1),
+        *((k_scale.data_ptr(), *k_scale.stride(), v_scale.data_ptr(), *v_scale.stride()) if i8 else (0, 0, 0, 0, 0, 0)),
+        table.data_ptr(), table.stride(0), idx.data_ptr(), lens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
+        0 if lse is None else lse.data_ptr(), cache_k.shape[0], B, Hq, Hkv, D, table.shape[1], table.shape[0], _CODE[dtype],
+        I8 if i8 else _CODE[dtype], min(window, 2 ** 31 - 1), float(sm_scale))
+    lib = _lib.lib()
+    with _on_device(device):
+        if workspace is None:
+            need = lib.wsvd_paged_decode_workspace_bytes(args)
+            workspace = _new(alloc_tensor_func, ((need + 3) // 4,), torch.float32, device, stream)
+        check(lib.wsvd_paged_decode(args, workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream)),
+              "wsvd_paged_decode")
+    return (out, lse) if return_lse else out
+
+
+def adapter_add(y, x, a, b, adapter, *, scale=None, cu_new=None, out=None, workspace: Optional[torch.Tensor] = None,
+                alloc_tensor_func: Callable = torch.empty, stream=None):
+    """Low-rank adapters of many requests beside a shared projection: ``out[n] = y[n] + scale[i] * (x[n] @ a[i]) @ b[i]``
+    with ``i = adapter[request of row n]`` (-1: ``out[n] = y[n]``).
+
+    x [N, n_in], y [N, n_out] (the projection's result), a [n_adapters, n_in, rank], b [n_adapters, rank, n_out], all f16 or all
+    bf16 (rows at any stride: y and out may be column slices); adapter [B] int32; scale [n_adapters] f32, None means
+    1.  Rows are packed by request, `cu_new` [B + 1] int32 as in `kv_rope_append` (None: one row per request).  Returns
+    out; `out=y` adds in place.  x a is summed in f32.  Rows behind cu_new[B] are padding: a caller's `out` keeps its rows,
+    the op's own has y's there.  An adapter that does not exist adds nothing and is reported by `kernel_status`."""
+    _tensor("x", x, _HALVES, 2)
+    dtype = x.dtype
+    one = (dtype,)
+    _tensor("y", y, one, 2)
+    _tensor("a", a, one, 3)
+    _tensor("b", b, one, 3)
+    _tensor("adapter", adapter, (torch.int32,), 1)
+    N, n_in = x.shape
+    n_out = y.shape[1]
+    count, _, rank = a.shape
+    if y.shape[0] != N:
+        raise ValueError(f"x and y must have the same rows, got {N} and {y.shape[0]}")
+    if a.shape[1] != n_in or b.shape != (count, rank, n_out):
+        raise ValueError(f"a must be [n_adapters, {n_in}, rank] and b [n_adapters, rank, {n_out}], got {tuple(a.shape)} and "
+                         f"{tuple(b.shape)}")
+    if not 1 <= rank <= 256:
+        raise ValueError(f"rank {rank} not in [1, 256]")
+    if n_in < 1 or n_out < 1:
+        raise ValueError("x and y must have columns")
+    B = adapter.shape[0]
+    if scale is not None:
+        _tensor("scale", scale, (torch.float32,), 1)
+        if scale.shape[0] != count:
+            raise ValueError(f"scale must have n_adapters = {count} entries")
+    if cu_new is None:
+        if B != N:
+            raise ValueError("adapter must have one entry per row where there is no cu_new")
+    else:
+        _tensor("cu_new", cu_new, (torch.int32,), 1)
+        if cu_new.shape[0] != B + 1:
+            raise ValueError("cu_new must have batch + 1 entries")
+    if out is not None:
+        _tensor("out", out, one, 2)
+        if out.shape != y.shape:
+            raise ValueError(f"out must be {tuple(y.shape)}, got {tuple(out.shape)}")
+        if out.data_ptr() == y.data_ptr() and out.stride() != y.stride():
+            raise ValueError("out may be y itself, not another view of its storage")
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    _no_gradient("adapter_add", y, x, a, b, out)
+    _on_one_gpu((("x", x), ("y", y), ("a", a), ("b", b), ("adapter", adapter), ("scale", scale), ("cu_new", cu_new),
+                 ("out", out), ("workspace", workspace)))
+    device = x.device
+    own = out is None
+    if own:
+        out = _new(alloc_tensor_func, (N, n_out), dtype, device, stream)
+    args = _pack_adapter(
+        y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), a.data_ptr(), a.stride(0), a.stride(1), b.data_ptr(), b.stride(0),
+        b.stride(1), out.data_ptr(), out.stride(0), adapter.data_ptr(), 0 if scale is None else scale.data_ptr(),
+        0 if cu_new is None else cu_new.data_ptr(), N, B, n_in, n_out, rank, count, _CODE[dtype], own)
+    lib = _lib.lib()
+    with _on_device(device):
+        if workspace is None:
+            need = lib.wsvd_adapter_add_workspace_bytes(args)
+            workspace = _new(alloc_tensor_func, ((need + 3) // 4,), torch.float32, device, stream)
+        check(lib.wsvd_adapter_add(args, workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream)),
+              "wsvd_adapter_add")
+    return out
+
+
 # ---- element-wise pieces of the decode step (one kernel each), launched on the device of their tensors
 
 def _one_device(x, **others):
