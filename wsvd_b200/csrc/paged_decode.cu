@@ -2,6 +2,8 @@
 //
 //   out = sum_s w_s v_s / sum_s w_s,  w_s = exp(c q . k_s - max),  max(0, len - window) <= s < len
 //   lse = max + log(sum_s w_s);  no positions: out = 0, lse = -inf
+#include <type_traits>
+
 #include "dense_ops.cuh"
 
 namespace wsvd {
@@ -103,6 +105,740 @@ __global__ void __launch_bounds__(kAnyWarps * 32) paged_decode_any_kernel(const 
     p.lse[(int64_t)b * p.n_q_heads + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
+// ---- the tensor-core kernel: head_dim 64, 96, 128 and 256, rows of whole 16-byte pieces
+//
+// Memory bound: 2 D values of cache per token and KV head, once for all its query heads.  The scores of a warp's 16 tokens
+// are one product S^T = K Q^T with the tokens as rows (m16n8k16: a row of 8 query heads costs nothing more than one head), and
+// O^T += V^T P^T has the dims as rows, so that a query head's statistics, weights and sums sit in the same lanes and the
+// accumulators are half of what 16 padded heads would take.  P^T is S^T's fragment turned by movmatrix.
+//
+// Every warp has a ring of its own in shared memory, filled with 16-byte asynchronous copies of its tokens' rows (zeros for
+// rows that are masked: what they hold must not reach a product), waits for nothing but its own copies, and goes on from one
+// sequence and head to the next without draining the ring.  The tiles of the batch are dealt out in equal shares to the CTAs
+// (common.cuh), so that ragged batches load every SM alike; what several CTAs hold of one (sequence, head) they leave
+// as partial sums, which paged_merge_kernel joins in a fixed order.
+//
+// Weights go into the product as two 16-bit terms (17 bits of bf16, 22 of f16): the one rounding that is left is the
+// result's.  int8 rows become f16 exactly (a byte under the exponent of 1024); their queries are scaled by a power of two to
+// [1, 2) at the largest, which is exact, so that bf16 ones of any size fit f16; the running maximum is that of score times v
+// scale, so that the weights with the v scale in them stay at or below one.
+
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kMaxShares = 1024;  // upper bound of the grid, for the workspace
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {  // zeros where it is not on
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ uint32_t turned(uint32_t v) {  // an 8 x 8 fragment of 16-bit values, transposed
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+  return r;
+}
+template <typename M>
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (sizeof(M) == 2 && std::is_same<M, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <typename M>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename M>
+__device__ __forceinline__ float2 unpack2(uint32_t v);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+// bytes of u (signed values + 128) at two places -> f16 pair: 0x64 on top of a byte is 1024 + byte
+template <uint32_t kPlaces>
+__device__ __forceinline__ uint32_t bytes_to_f16(uint32_t u) {
+  const uint32_t v = __byte_perm(u, 0x64646464u, kPlaces);
+  const uint32_t k1152 = 0x64806480u;
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&k1152));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T_, bool I8_, int D_, int NT_>
+struct Cfg {
+  using T = T_;                                                         // q and out
+  using M = typename std::conditional<I8_, __half, T_>::type;           // the products' operands
+  static constexpr bool I8 = I8_;
+  static constexpr int D = D_, NT = NT_, HEADS = 8 * NT_;               // query heads of an item, at most
+  static constexpr int ROW = D * (I8 ? 1 : 2), PIECES = ROW / 16;       // bytes and 16-byte pieces of a cached row
+  static constexpr int PITCH = (PIECES | 1) * 16;                       // an odd number of pieces: conflict-free ldmatrix
+  static constexpr int TOK = ROW >= 128 ? 16 : 32, SUBS = TOK / 16;     // tokens of a warp's step
+  static constexpr int STAGES = ROW >= 512 ? 2 : 3;
+  static constexpr int TILE = kWarps * TOK;
+  static constexpr int STAGE_BYTES = 2 * TOK * PITCH;                   // K rows, then V rows
+  static constexpr int O_LD = D + 4;
+};
+
+// What the ring holds besides rows: which tokens count, and where a sequence and head begin and end.
+struct Step {
+  int64_t item_first;  // the item's first tile in the batch's order
+  uint32_t mask;       // its tokens that count
+  int32_t flags;       // 1: first step of a run in this CTA, 2: last one
+  int32_t b, it, tiles;
+};
+
+// Partial sums of a run: [slot][head of the item][D] f32, (maximum, sum) beside them, and per item the first slot and how many.
+struct Partials {
+  float* o;
+  float2* ml;
+  int2* items;
+};
+
+template <typename C>
+__global__ void __launch_bounds__(kThreads)
+paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Partials part, int group, int hpi, int chunks) {
+  using T = typename C::T;
+  using M = typename C::M;
+  constexpr int D = C::D, NT = C::NT, S = C::STAGES, TOK = C::TOK;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ Step ring[kWarps][S];
+  __shared__ int32_t ring_slot[C::I8 ? kWarps : 1][C::I8 ? S : 1][TOK];
+  __shared__ float2 sm_scale[C::I8 ? kWarps : 1][TOK];
+  __shared__ float2 sm_ml[kWarps][C::HEADS];
+  __shared__ int64_t sm_scan[kWarps + 1];
+  __shared__ int64_t sm_before;
+  __shared__ int sm_b;
+  float* sm_o = reinterpret_cast<float*>(smem + kWarps * S * C::STAGE_BYTES);  // [2][hpi][O_LD]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c4 = lane & 3;
+  const int n_it = p.n_kv_heads * chunks;  // items (KV head, chunk of its query heads) of a sequence
+
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+
+  auto tiles_of = [&](int b) {
+    int n = min(p.b_seq_len[b], p.max_len);
+    const int req = p.b_req_idx[b];
+    if (n <= 0 || req < 0 || req >= p.n_req) return 0;
+    if (p.window > 0) n = min(n, p.window);
+    return (n + C::TILE - 1) / C::TILE;
+  };
+
+  // ---- this CTA's share [lo, hi) of the tiles in the order (sequence, item, tile)
+  const int per = (p.batch + kThreads - 1) / kThreads, b0 = min(p.batch, (int)threadIdx.x * per), b1 = min(p.batch, b0 + per);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += tiles_of(b);
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sm_scan[warp] = incl;
+  __syncthreads();
+  int64_t total = 0, before = incl - mine;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sm_scan[w];
+    total += sm_scan[w];
+  }
+  total *= n_it;
+  before *= n_it;
+  const int shares = (int)min((int64_t)gridDim.x, total);
+  const bool busy = (int)blockIdx.x < shares;
+  const int64_t lo = busy ? share_begin(blockIdx.x, total, shares) : 0, hi = busy ? share_begin(blockIdx.x + 1, total, shares) : 0;
+  if (busy && lo >= before && lo < before + mine * n_it) {
+    int b = b0;
+    int64_t at = before;
+    for (;; ++b) {
+      const int64_t n = (int64_t)tiles_of(b) * n_it;
+      if (lo < at + n) break;
+      at += n;
+    }
+    sm_b = b;
+    sm_before = at;
+  }
+  __syncthreads();
+
+  if (busy) {
+    // ---- the cursor: the step whose rows are requested next
+    int left = (int)(hi - lo);  // tiles not yet requested
+    int cb = sm_b, cit, ct, cnt = tiles_of(sm_b), first, end;
+    {
+      const int64_t in = lo - sm_before;
+      cit = (int)(in / cnt);
+      ct = (int)(in - (int64_t)cit * cnt);
+    }
+    int64_t seq_first = sm_before;
+    const int32_t* page;
+    auto enter = [&]() {  // sequence cb
+      const Span sp = span_of(p, cb);
+      first = sp.first;
+      end = sp.end;
+      page = sp.page;
+    };
+    enter();
+    bool fresh = true;  // the run begins with this step
+    int slot = -1;
+    auto fetch_slots = [&]() {  // of the cursor's step: lane i has token i's
+      const int s = first + ct * C::TILE + warp * TOK + lane;
+      slot = -1;
+      if (lane < TOK && s < end) slot = page[s];
+    };
+    const int64_t n_slots = p.n_token_slots;
+    const int k_row = (int)(p.k_stride_t * (C::I8 ? 1 : 2)), v_row = (int)(p.v_stride_t * (C::I8 ? 1 : 2));
+    const uint32_t my_ring = smem_addr(smem) + warp * S * C::STAGE_BYTES;
+    fetch_slots();
+
+    auto request = [&](int stage) {
+      if (left > 0) {
+        const int s = first + ct * C::TILE + warp * TOK + lane;
+        const bool want = lane < TOK && s < end, ok = want && slot >= 0 && (int64_t)slot < n_slots;
+        if (want && !ok) atomicMax(&g_status, kOutsideStorage);
+        const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+        const int from = ok ? slot : -1;
+        const int hk = cit / chunks;
+        const char* kb = reinterpret_cast<const char*>(p.k) + (int64_t)hk * p.k_stride_h * (C::I8 ? 1 : 2);
+        const char* vb = reinterpret_cast<const char*>(p.v) + (int64_t)hk * p.v_stride_h * (C::I8 ? 1 : 2);
+        const uint32_t dst = my_ring + stage * C::STAGE_BYTES;
+#pragma unroll
+        for (int i = 0; i < TOK * C::PIECES / 32; ++i) {
+          const int piece = lane + 32 * i, row = piece / C::PIECES, col = piece - row * C::PIECES;
+          const int t = __shfl_sync(0xffffffffu, from, row);
+          const bool on = t >= 0;
+          const char* ks = kb + (on ? (int64_t)t * k_row + col * 16 : 0);
+          const char* vs = vb + (on ? (int64_t)t * v_row + col * 16 : 0);
+          copy16(dst + row * C::PITCH + col * 16, ks, on);
+          copy16(dst + TOK * C::PITCH + row * C::PITCH + col * 16, vs, on);
+        }
+        if constexpr (C::I8)
+          if (lane < TOK) ring_slot[warp][stage][lane] = from;
+        const bool last = ct + 1 == cnt || left == 1;
+        if (lane == 0) ring[warp][stage] = Step{seq_first + (int64_t)cit * cnt, mask, (fresh ? 1 : 0) | (last ? 2 : 0), cb, cit, cnt};
+        fresh = last;
+        --left;
+        if (++ct == cnt) {
+          ct = 0;
+          if (++cit == n_it) {
+            cit = 0;
+            if (left > 0) {
+              seq_first += (int64_t)cnt * n_it;
+              do { cnt = tiles_of(++cb); } while (cnt == 0);
+              enter();
+            }
+          }
+        }
+        if (left > 0) fetch_slots();
+      }
+      copies_commit();
+    };
+
+    for (int i = 0; i < S - 1; ++i) request(i);
+
+    // int8: the scales of a step are two-byte loads a step ahead of their use, a token a lane
+    __half next_sk, next_sv;
+    auto fetch_scales = [&](int stage) {
+      next_sk = next_sv = __float2half_rn(0.f);
+      const int t = lane < TOK ? ring_slot[warp][stage][lane] : -1;
+      if (t < 0) return;
+      const int64_t hk = ring[warp][stage].it / chunks;
+      next_sk = reinterpret_cast<const __half*>(p.k_scale)[(int64_t)t * p.ks_stride_t + hk * p.ks_stride_h];
+      next_sv = reinterpret_cast<const __half*>(p.v_scale)[(int64_t)t * p.vs_stride_t + hk * p.vs_stride_h];
+    };
+    if constexpr (C::I8) {
+      __syncwarp();
+      fetch_scales(0);
+    }
+
+    const float c = (p.sm_scale != 0.f ? p.sm_scale : rsqrtf((float)D)) * kLog2e;
+    uint32_t q[NT][D / 16][2];
+    float cq[NT][2], m[NT][2], l[NT][2], acc[D / 16][NT][4];
+    const int steps = (int)(hi - lo);
+    int stage = 0;
+    for (int step = 0; step < steps; ++step) {
+      request(stage == 0 ? S - 1 : stage - 1);
+      if constexpr (C::I8)
+        if (lane < TOK) sm_scale[warp][lane] = make_float2(__half2float(next_sk), __half2float(next_sv));
+      copies_wait<S - 1>();
+      __syncwarp();
+      const Step now = ring[warp][stage];
+      if constexpr (C::I8)
+        if (step + 1 < steps) fetch_scales(stage + 1 == S ? 0 : stage + 1);
+      const int hk = now.it / chunks, h0 = hk * group + (now.it - hk * chunks) * hpi;
+      const int heads = min(hpi, group - (now.it - hk * chunks) * hpi);
+      if (now.flags & 1) {
+        // queries as B operand: lane (head g, dims 2 c4, 2 c4 + 1 and + 8 of every 16; bytes: dims 4 c4 .. 4 c4 + 3)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const bool on = 8 * j + g < heads;
+          const T* qr = reinterpret_cast<const T*>(p.q) + (int64_t)now.b * p.q_stride_b + (int64_t)(h0 + (on ? 8 * j + g : 0)) * p.q_stride_h;
+          float amax = 0.f;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int d = 16 * k + (C::I8 ? 4 * c4 + 2 * e : 2 * c4 + 8 * e);
+              q[j][k][e] = on ? *reinterpret_cast<const uint32_t*>(qr + d) : 0u;
+              if constexpr (C::I8) {
+                const float2 f = unpack2<T>(q[j][k][e]);
+                amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+              }
+            }
+          }
+          cq[j][0] = cq[j][1] = c;
+          if constexpr (C::I8) {
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+            int e = 0;
+            if (amax > 0.f && amax < INFINITY) e = max(-126, ilogbf(amax));
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+              for (int t = 0; t < 2; ++t) {
+                const float2 f = unpack2<T>(q[j][k][t]);
+                q[j][k][t] = pack2<M>(scalbnf(f.x, -e), scalbnf(f.y, -e));
+              }
+            // the factor of head 8 j + g; this lane's columns are heads 2 c4 and 2 c4 + 1
+            const float f = scalbnf(c, e);
+            cq[j][0] = __shfl_sync(0xffffffffu, f, 8 * c4);
+            cq[j][1] = __shfl_sync(0xffffffffu, f, 8 * c4 + 4);
+          }
+          m[j][0] = m[j][1] = -FLT_MAX;
+          l[j][0] = l[j][1] = 0.f;
+#pragma unroll
+          for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[t][j][i] = 0.f;
+        }
+      }
+
+      // ---- scores: rows tokens, columns heads
+      const uint32_t kst = my_ring + stage * C::STAGE_BYTES, vst = kst + TOK * C::PITCH;
+      float z[C::SUBS][NT][4];
+#pragma unroll
+      for (int u = 0; u < C::SUBS; ++u) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) z[u][j][i] = 0.f;
+        const uint32_t base = kst + (16 * u + (lane & 15)) * C::PITCH + (lane >> 4) * 16;
+        if constexpr (!C::I8) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            uint32_t a[4];
+            ldmatrix4(a, base + k * 32);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) mma<M>(z[u][j], a[0], a[1], a[2], a[3], q[j][k][0], q[j][k][1]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < D / 16; k += 2) {
+            uint32_t r[4];
+            ldmatrix4(r, base + k * 16);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t x = r[2 * e] ^ 0x80808080u, y = r[2 * e + 1] ^ 0x80808080u;
+              const uint32_t a0 = bytes_to_f16<0x4140>(x), a2 = bytes_to_f16<0x4342>(x), a1 = bytes_to_f16<0x4140>(y),
+                             a3 = bytes_to_f16<0x4342>(y);
+#pragma unroll
+              for (int j = 0; j < NT; ++j) mma<M>(z[u][j], a0, a1, a2, a3, q[j][k + e][0], q[j][k + e][1]);
+            }
+          }
+        }
+      }
+
+      // ---- weights
+      float sv[C::SUBS][2];
+      float top[NT][2];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) top[j][0] = m[j][0], top[j][1] = m[j][1];
+#pragma unroll
+      for (int u = 0; u < C::SUBS; ++u)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int tok = 16 * u + g + 8 * e;
+          const bool on = (now.mask >> tok) & 1;
+          float sk = 1.f, lsv = 0.f;
+          sv[u][e] = 1.f;
+          if constexpr (C::I8) {
+            const float2 s = sm_scale[warp][tok];
+            sk = s.x;
+            sv[u][e] = s.y;
+            lsv = __log2f(fmaxf(fabsf(sv[u][e]), 5.9604644775390625e-8f));
+          }
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float& v = z[u][j][2 * e + i];
+              v = on ? v * (C::I8 ? cq[j][i] * sk : c) : -INFINITY;
+              top[j][i] = fmaxf(top[j][i], C::I8 ? v + lsv : v);
+            }
+        }
+      bool moved = false;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int o = 4; o <= 16; o <<= 1) top[j][i] = fmaxf(top[j][i], __shfl_xor_sync(0xffffffffu, top[j][i], o));
+          moved |= top[j][i] != m[j][i];
+        }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const float keep = ex2(m[j][i] - top[j][i]);
+            m[j][i] = top[j][i];
+            l[j][i] *= keep;
+#pragma unroll
+            for (int t = 0; t < D / 16; ++t) {
+              acc[t][j][i] *= keep;
+              acc[t][j][2 + i] *= keep;
+            }
+          }
+      }
+#pragma unroll
+      for (int u = 0; u < C::SUBS; ++u) {
+        uint32_t hi_b[NT][2], lo_b[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float w[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              w[i] = ex2(z[u][j][2 * e + i] - m[j][i]);
+              l[j][i] += w[i];
+              if (C::I8) w[i] *= sv[u][e];
+            }
+            const uint32_t h = pack2<M>(w[0], w[1]);
+            const float2 f = unpack2<M>(h);
+            hi_b[j][e] = turned(h);
+            lo_b[j][e] = turned(pack2<M>(w[0] - f.x, w[1] - f.y));
+          }
+        // ---- values: rows dims, columns heads
+        if constexpr (!C::I8) {
+          const uint32_t base = vst + (16 * u + (lane & 7) + 8 * (lane >> 4)) * C::PITCH + ((lane >> 3) & 1) * 16;
+#pragma unroll
+          for (int t = 0; t < D / 16; ++t) {
+            uint32_t a[4];
+            ldmatrix4_trans(a, base + t * 32);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              mma<M>(acc[t][j], a[0], a[1], a[2], a[3], hi_b[j][0], hi_b[j][1]);
+              mma<M>(acc[t][j], a[0], a[1], a[2], a[3], lo_b[j][0], lo_b[j][1]);
+            }
+          }
+        } else {
+          // a transposed pair of bytes is two dims of one token: row g of the product is dim 2 g, row g + 8 dim 2 g + 1
+          const uint32_t base = vst + (16 * u + (lane & 7) + 8 * ((lane >> 3) & 1)) * C::PITCH + (lane >> 4) * 16;
+#pragma unroll
+          for (int t = 0; t < D / 16; t += 2) {
+            uint32_t r[4];
+            ldmatrix4_trans(r, base + t * 16);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t x = r[2 * e] ^ 0x80808080u, y = r[2 * e + 1] ^ 0x80808080u;
+              const uint32_t a0 = bytes_to_f16<0x4240>(x), a1 = bytes_to_f16<0x4341>(x), a2 = bytes_to_f16<0x4240>(y),
+                             a3 = bytes_to_f16<0x4341>(y);
+#pragma unroll
+              for (int j = 0; j < NT; ++j) {
+                mma<M>(acc[t + e][j], a0, a1, a2, a3, hi_b[j][0], hi_b[j][1]);
+                mma<M>(acc[t + e][j], a0, a1, a2, a3, lo_b[j][0], lo_b[j][1]);
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();  // the stage may be filled again
+
+      if (now.flags & 2) {
+        // ---- the end of a run: the warps' sums joined (warps 0 and 1 write, 2 and 3 add), then the result or a partial
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int o = 4; o <= 16; o <<= 1) l[j][i] += __shfl_xor_sync(0xffffffffu, l[j][i], o);
+            if (g == 0) sm_ml[warp][8 * j + 2 * c4 + i] = make_float2(m[j][i], l[j][i]);
+          }
+        __syncthreads();
+#pragma unroll
+        for (int pass = 0; pass < 2; ++pass) {
+          if ((warp >> 1) == pass) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int h = 8 * j + 2 * c4 + i;
+                if (h >= heads) continue;
+                float all = sm_ml[0][h].x;
+#pragma unroll
+                for (int w = 1; w < kWarps; ++w) all = fmaxf(all, sm_ml[w][h].x);
+                const float f = ex2(m[j][i] - all);
+                float* o = sm_o + ((warp & 1) * hpi + h) * C::O_LD;
+#pragma unroll
+                for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const int d = 16 * t + (C::I8 ? 2 * g + e : g + 8 * e);
+                    const float v = acc[t][j][2 * e + i] * f;
+                    if (pass == 0) o[d] = v;
+                    else o[d] += v;
+                  }
+              }
+          }
+          __syncthreads();
+        }
+        const int c0 = share_owner(now.item_first, total, shares), c1 = share_owner(now.item_first + now.tiles - 1, total, shares);
+        const int64_t item = (int64_t)now.b * n_it + now.it;
+        const int64_t at = (item + blockIdx.x) * hpi;  // (items and CTAs only grow: no two runs have the same sum)
+        if (c0 == (int)blockIdx.x && threadIdx.x == 0) part.items[item] = make_int2((int)(item + c0), c1 - c0 + 1);
+        T* out = reinterpret_cast<T*>(p.out) + (int64_t)now.b * p.out_stride_b + (int64_t)h0 * p.out_stride_h;
+        for (int i = threadIdx.x; i < heads * D; i += kThreads) {
+          const int h = i / D, d = i - h * D;
+          const float o = sm_o[h * C::O_LD + d] + sm_o[(hpi + h) * C::O_LD + d];
+          float all = sm_ml[0][h].x, sum = 0.f;
+#pragma unroll
+          for (int w = 1; w < kWarps; ++w) all = fmaxf(all, sm_ml[w][h].x);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) sum += sm_ml[w][h].y * ex2(sm_ml[w][h].x - all);
+          if (c0 == c1) {
+            out[(int64_t)h * p.out_stride_h + d] = narrow<T>(sum == 0.f ? 0.f : o / sum);
+            if (d == 0 && p.lse != nullptr)
+              p.lse[(int64_t)now.b * p.n_q_heads + h0 + h] = sum == 0.f ? -INFINITY : (all + log2f(sum)) * kLn2;
+          } else {
+            part.o[(at + h) * D + d] = o;
+            if (d == 0) part.ml[at + h] = make_float2(all, sum);
+          }
+        }
+        __syncthreads();
+      }
+      stage = stage + 1 == S ? 0 : stage + 1;
+    }
+  }
+
+  // ---- sequences without positions
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    if (tiles_of(b) > 0) continue;
+    if (threadIdx.x == 0) span_of(p, b);  // (records why)
+    for (int i = threadIdx.x; i < p.n_q_heads * D; i += kThreads) {
+      const int h = i / D, d = i - h * D;
+      reinterpret_cast<T*>(p.out)[(int64_t)b * p.out_stride_b + (int64_t)h * p.out_stride_h + d] = narrow<T>(0.f);
+      if (d == 0 && p.lse != nullptr) p.lse[(int64_t)b * p.n_q_heads + h] = -INFINITY;
+    }
+  }
+}
+
+// Joins the partial sums of one (sequence, query head): a warp takes every eighth of them, a lane D / 32 dims, four partials'
+// loads in flight; the warps' sums meet in shared memory.  Always the same order.
+constexpr int kMergeWarps = 8;
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeWarps * 32)
+paged_merge_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Partials part, int group, int hpi, int chunks) {
+  constexpr int E = D / 32;
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int req = p.b_req_idx[b];
+  if (p.b_seq_len[b] <= 0 || p.max_len <= 0 || req < 0 || req >= p.n_req) return;
+  const int hk = h / group, in = h - hk * group;
+  const int2 info = part.items[(int64_t)b * p.n_kv_heads * chunks + hk * chunks + in / hpi];
+  if (info.y <= 1) return;
+  const int64_t first = (int64_t)info.x * hpi + in % hpi;
+  float m = -FLT_MAX, l = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int i0 = warp; i0 < info.y; i0 += 4 * kMergeWarps) {
+    float2 ml[4];
+    float v[4][E];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = i0 + i * kMergeWarps;
+      const bool on = k < info.y;
+      const int64_t at = first + (int64_t)(on ? k : 0) * hpi;
+      ml[i] = on ? part.ml[at] : make_float2(-FLT_MAX, 0.f);
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[i][e] = on ? part.o[at * D + lane + 32 * e] : 0.f;
+    }
+    float top = m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = fmaxf(top, ml[i].x);
+    const float keep = ex2(m - top);
+    l *= keep;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= keep;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float f = ex2(ml[i].x - top);
+      l = fmaf(ml[i].y, f, l);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(v[i][e], f, o[e]);
+    }
+    m = top;
+  }
+  __shared__ float sm_o[kMergeWarps][D];
+  __shared__ float2 sm_ml[kMergeWarps];
+  if (lane == 0) sm_ml[warp] = make_float2(m, l);
+#pragma unroll
+  for (int e = 0; e < E; ++e) sm_o[warp][lane + 32 * e] = o[e];
+  __syncthreads();
+  float top = sm_ml[0].x, sum = 0.f;
+#pragma unroll
+  for (int w = 1; w < kMergeWarps; ++w) top = fmaxf(top, sm_ml[w].x);
+  const int d = threadIdx.x;
+  float r = 0.f;
+#pragma unroll
+  for (int w = 0; w < kMergeWarps; ++w) {
+    const float f = ex2(sm_ml[w].x - top);
+    sum = fmaf(sm_ml[w].y, f, sum);
+    if (d < D) r = fmaf(sm_o[w][d], f, r);
+  }
+  if (d < D)
+    reinterpret_cast<T*>(p.out)[(int64_t)b * p.out_stride_b + (int64_t)h * p.out_stride_h + d] = narrow<T>(sum == 0.f ? 0.f : r / sum);
+  if (d == 0 && p.lse != nullptr) p.lse[(int64_t)b * p.n_q_heads + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+}
+
+// ---- host side
+
+// How the query heads of a KV head are cut into items: all of them, or chunks of 16.
+struct Items {
+  int group, hpi, chunks, nt;
+};
+Items items_of(const WsvdPagedDecodeParams& p) {
+  const int group = p.n_q_heads / p.n_kv_heads;
+  const int chunks = (group + 15) / 16, hpi = (group + chunks - 1) / chunks;
+  return {group, hpi, chunks, hpi <= 8 ? 1 : 2};
+}
+size_t pad256(size_t b) { return (b + 255) & ~(size_t)255; }
+struct Room {
+  size_t o, ml, items, total;
+};
+Room room_of(const WsvdPagedDecodeParams& p) {
+  const Items it = items_of(p);
+  const size_t items = (size_t)p.batch * p.n_kv_heads * it.chunks, rows = (items + kMaxShares) * it.hpi;
+  Room r;
+  r.o = 0;
+  r.ml = r.o + pad256(rows * p.head_dim * sizeof(float));
+  r.items = r.ml + pad256(rows * sizeof(float2));
+  r.total = r.items + pad256(items * sizeof(int2));
+  return r;
+}
+// Whether the tensor-core kernel takes the call; the rest (other head dimensions, rows off 16 bytes) runs on the kernel for
+// any shape, at about a tenth of its speed.
+bool fits_tensor_cores(const WsvdPagedDecodeParams& p) {
+  const int es = p.cache_dtype == WSVD_I8 ? 1 : 2, unit = 16 / es;
+  if (p.head_dim != 64 && p.head_dim != 96 && p.head_dim != 128 && p.head_dim != 256) return false;
+  if (((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v)) & 15) != 0) return false;
+  if (p.k_stride_t % unit || p.k_stride_h % unit || p.v_stride_t % unit || p.v_stride_h % unit) return false;
+  // token strides in bytes are multiplied as 32-bit values
+  if (p.k_stride_t < 0 || p.v_stride_t < 0 || p.k_stride_t * es > INT32_MAX || p.v_stride_t * es > INT32_MAX) return false;
+  return (reinterpret_cast<uintptr_t>(p.q) & 3) == 0 && p.q_stride_b % 2 == 0 && p.q_stride_h % 2 == 0;
+}
+
+int sm_count(int device) {
+  static int counts[64];
+  if (device < 0 || device >= 64) return 148;
+  if (counts[device] == 0) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) n = 148;
+    counts[device] = n;
+  }
+  return counts[device];
+}
+
+template <typename K, typename... Args>
+cudaError_t launch(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  // the kernel's set-up may overlap the end of the kernel in front of it: both wait (griddepcontrol.wait) before they
+  // read or write anything
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <typename C>
+cudaError_t launch_fast(const WsvdPagedDecodeParams& p, const Items& it, const Partials& part, cudaStream_t s) {
+  constexpr size_t kRing = (size_t)kWarps * C::STAGES * C::STAGE_BYTES;
+  const size_t smem = kRing + 2 * (size_t)it.hpi * C::O_LD * sizeof(float);
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  static bool ready[64];
+  if (device >= 64 || !ready[device]) {
+    e = cudaFuncSetAttribute(paged_decode_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)(kRing + 2 * C::HEADS * C::O_LD * sizeof(float)));
+    if (e != cudaSuccess) return e;
+    if (device < 64) ready[device] = true;
+  }
+  // CTAs per SM: what shared memory holds (1 KB of it is the system's, about 1.5 KB the kernel's own variables)
+  const int fit = (int)((228 * 1024) / (smem + 2560)), per_sm = fit < 1 ? 1 : fit > 3 ? 3 : fit;
+  const int reach = p.window > 0 && p.window < p.max_len ? p.window : p.max_len;
+  const int64_t most = (int64_t)p.batch * p.n_kv_heads * it.chunks * ((reach + C::TILE - 1) / C::TILE);
+  int64_t grid = (int64_t)sm_count(device) * per_sm;
+  if (grid > kMaxShares) grid = kMaxShares;
+  if (grid > most) grid = most;
+  if (grid < 1) grid = 1;
+  e = launch(paged_decode_kernel<C>, dim3((unsigned)grid), kThreads, smem, s, p, part, it.group, it.hpi, it.chunks);
+  if (e != cudaSuccess || grid == 1 || reach <= C::TILE) return e;  // (one tile an item: no partials)
+  return launch(paged_merge_kernel<typename C::T, C::D>, dim3(p.n_q_heads, p.batch), kMergeWarps * 32, 0, s, p, part, it.group,
+                it.hpi, it.chunks);
+}
+
+template <typename T, bool I8, int NT>
+cudaError_t launch_dims(const WsvdPagedDecodeParams& p, const Items& it, const Partials& part, cudaStream_t s) {
+  switch (p.head_dim) {
+    case 64: return launch_fast<Cfg<T, I8, 64, NT>>(p, it, part, s);
+    case 96: return launch_fast<Cfg<T, I8, 96, NT>>(p, it, part, s);
+    case 128: return launch_fast<Cfg<T, I8, 128, NT>>(p, it, part, s);
+    default: return launch_fast<Cfg<T, I8, 256, NT>>(p, it, part, s);
+  }
+}
+template <typename T, bool I8>
+cudaError_t launch_tensor_cores(const WsvdPagedDecodeParams& p, void* workspace, cudaStream_t s) {
+  const Items it = items_of(p);
+  const Room r = room_of(p);
+  char* w = reinterpret_cast<char*>(workspace);
+  const Partials part{reinterpret_cast<float*>(w + r.o), reinterpret_cast<float2*>(w + r.ml), reinterpret_cast<int2*>(w + r.items)};
+  return it.nt == 1 ? launch_dims<T, I8, 1>(p, it, part, s) : launch_dims<T, I8, 2>(p, it, part, s);
+}
+
 template <typename T, typename C>
 void launch_any(const WsvdPagedDecodeParams& p, cudaStream_t s) {
   paged_decode_any_kernel<T, C><<<dim3(p.n_q_heads, p.batch), kAnyWarps * 32, 0, s>>>(p);
@@ -121,8 +857,8 @@ cudaError_t reset_paged_decode_status() {
 extern "C" {
 
 size_t wsvd_paged_decode_workspace_bytes(const WsvdPagedDecodeParams* p) {
-  (void)p;
-  return 0;
+  if (!p || p->batch <= 0 || p->n_q_heads <= 0 || p->n_kv_heads <= 0 || p->n_q_heads % p->n_kv_heads || p->head_dim <= 0) return 0;
+  return wsvd::fits_tensor_cores(*p) ? wsvd::room_of(*p).total : 0;
 }
 
 int wsvd_paged_decode(const WsvdPagedDecodeParams* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -143,12 +879,18 @@ int wsvd_paged_decode(const WsvdPagedDecodeParams* p, void* workspace, size_t wo
   if (workspace_bytes < need) return WSVD_ERR_WORKSPACE_TOO_SMALL;
   if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return WSVD_ERR_BAD_STRIDE;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (p->dtype == WSVD_F16) {
-    i8 ? wsvd::launch_any<__half, int8_t>(*p, s) : wsvd::launch_any<__half, __half>(*p, s);
+  cudaError_t e;
+  if (need > 0) {
+    if (p->dtype == WSVD_F16)
+      e = i8 ? wsvd::launch_tensor_cores<__half, true>(*p, workspace, s) : wsvd::launch_tensor_cores<__half, false>(*p, workspace, s);
+    else
+      e = i8 ? wsvd::launch_tensor_cores<__nv_bfloat16, true>(*p, workspace, s)
+             : wsvd::launch_tensor_cores<__nv_bfloat16, false>(*p, workspace, s);
   } else {
-    i8 ? wsvd::launch_any<__nv_bfloat16, int8_t>(*p, s) : wsvd::launch_any<__nv_bfloat16, __nv_bfloat16>(*p, s);
+    if (p->dtype == WSVD_F16) i8 ? wsvd::launch_any<__half, int8_t>(*p, s) : wsvd::launch_any<__half, __half>(*p, s);
+    else i8 ? wsvd::launch_any<__nv_bfloat16, int8_t>(*p, s) : wsvd::launch_any<__nv_bfloat16, __nv_bfloat16>(*p, s);
+    e = cudaGetLastError();
   }
-  const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? WSVD_OK : wsvd::record_cuda_error(e);
 }
 
