@@ -44,4 +44,21 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int batch, int n) 
   return lo;
 }
 
+// Launch of a kernel that waits (griddepcontrol.wait) before it reads or writes anything: its blocks may be set up
+// while the kernel in front of it in the stream still ends.
+template <typename K, typename... Args>
+cudaError_t launch_overlapped(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 }  // namespace wsvd

@@ -127,10 +127,230 @@ __global__ void __launch_bounds__(128) kv_append_any_kernel(const __grid_constan
   }
 }
 
+// ---- the same for head_dim and rot_dim in whole 16s and rows of whole 16-byte vectors
+//
+// Bound by memory: every value is read and written once.  A thread's unit is two 8-value vectors of a row that turn into one
+// another (half: dims 8 j .. and rot / 2 + 8 j ..; interleaved and what is not rotated: 16 dims in a row), so that nothing but
+// the angles passes through shared memory; unit j of any head turns by the angles 8 j .. 8 j + 7 of its row.  A block takes a
+// run of units of consecutive rows; the angles of those rows (f64 reduction, sine and cosine: ~100 instructions) are
+// computed once for all heads.  What a row's place is (up to four dependent loads) and the angles are worked out while the
+// block's vectors are on their way.
+constexpr int kVecThreads = 256;
+// from here on four units a thread (a block's set-up is paid for more data), below it one (more SMs at work)
+constexpr int64_t kManyUnits = 148 * 4 * kVecThreads * 4;
+
+struct Divisor {  // n / d for n < 2^31
+  uint32_t d, m, s;
+  __host__ static Divisor of(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    return {d, (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(m, n) + n) >> s; }
+};
+
+template <typename T>
+struct Pair;
+template <>
+struct Pair<__half> {
+  static __device__ __forceinline__ float2 open(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+  static __device__ __forceinline__ uint32_t close(float x, float y) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct Pair<__nv_bfloat16> {
+  static __device__ __forceinline__ float2 open(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v)); }
+  static __device__ __forceinline__ uint32_t close(float x, float y) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void open8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = Pair<T>::open(w[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 close8(const float (&f)[8]) {
+  return make_uint4(Pair<T>::close(f[0], f[1]), Pair<T>::close(f[2], f[3]), Pair<T>::close(f[4], f[5]), Pair<T>::close(f[6], f[7]));
+}
+__device__ __forceinline__ uint2 bytes8(const float (&f)[8], float s) {
+  uint32_t w[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    w[i] = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      w[i] |= ((uint32_t)(int)fminf(fmaxf(rintf(f[4 * i + e] / s), -128.f), 127.f) & 255u) << (8 * e);
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// lanes: log2 of the lanes of a head (D / 16 rounded up to a power of two); per_row: units of a row; U: units of a thread
+template <typename T, bool I8, int U>
+__global__ void __launch_bounds__(kVecThreads)
+kv_append_vec_kernel(const __grid_constant__ WsvdKvRopeAppendParams p, const int lanes, const Divisor per_row, const int most_rows) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int half = p.rot_dim / 2, groups = p.rot_dim / 16;  // angles of a row, units that turn
+  int64_t* row_slot = reinterpret_cast<int64_t*>(smem);     // -1: not stored, -2: padding
+  int64_t* row_place = row_slot + most_rows;
+  float2* turn = reinterpret_cast<float2*>(row_place + most_rows);  // [row][8][groups]: neighbouring units, neighbouring words
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  const uint32_t total = (uint32_t)p.rows * per_row.d, first = blockIdx.x * (uint32_t)(kVecThreads * U);
+  const int row0 = per_row.div(first);
+  const int rows = (int)per_row.div(min(total, first + kVecThreads * U) - 1) - row0 + 1;
+  const int units = p.head_dim / 16;
+  const bool half_layout = p.rope_layout == WSVD_ROPE_HALF;
+
+  // where a unit's two vectors start in its row
+  auto second = [&](int j, bool turns) { return turns && half_layout ? half + 8 * j : 16 * j + 8; };
+  auto start = [&](int j, bool turns) { return turns && half_layout ? 8 * j : 16 * j; };
+
+  uint4 va[U], vb[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t idx = first + u * kVecThreads + threadIdx.x;
+    if (idx >= total) continue;
+    const int row = per_row.div(idx), in = idx - row * per_row.d, head = in >> lanes, j = in & ((1 << lanes) - 1);
+    if (j >= units) continue;
+    const int hk = head - p.n_q_heads, hv = hk - p.n_kv_heads;
+    const T* src = hk < 0   ? reinterpret_cast<const T*>(p.q) + (int64_t)row * p.q_stride_n + (int64_t)head * p.q_stride_h
+                   : hv < 0 ? reinterpret_cast<const T*>(p.k) + (int64_t)row * p.k_stride_n + (int64_t)hk * p.k_stride_h
+                            : reinterpret_cast<const T*>(p.v) + (int64_t)row * p.v_stride_n + (int64_t)hv * p.v_stride_h;
+    const bool turns = hv < 0 && j < groups;
+    va[u] = *reinterpret_cast<const uint4*>(src + start(j, turns));
+    vb[u] = *reinterpret_cast<const uint4*>(src + second(j, turns));
+  }
+  for (int r = threadIdx.x; r < rows; r += kVecThreads) {
+    const RowPlace at = place_of(p, row0 + r);
+    row_slot[r] = at.row ? at.slot : -2;
+    row_place[r] = at.place;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows * half; i += kVecThreads) {
+    const int r = i / half, a = i - r * half;
+    float sn, cs;
+    rotation(row_place[r], p.inv_freq[a], &sn, &cs);
+    turn[r * half + (a & 7) * groups + (a >> 3)] = make_float2(cs, sn);
+  }
+  __syncthreads();
+
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t idx = first + u * kVecThreads + threadIdx.x;
+    const bool in_range = idx < total;
+    const int row = in_range ? per_row.div(idx) : row0, in = in_range ? idx - row * per_row.d : 0;
+    const int head = in >> lanes, j = in & ((1 << lanes) - 1);
+    const bool active = in_range && j < units;
+    const int hk = head - p.n_q_heads, hv = hk - p.n_kv_heads;
+    const bool turns = active && hv < 0 && j < groups;
+    const int64_t slot = row_slot[row - row0];
+    float a[8], b[8];
+    if (active) {
+      open8<T>(va[u], a);
+      open8<T>(vb[u], b);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) a[e] = b[e] = 0.f;
+    }
+    if (turns) {
+      const float2* t = turn + (row - row0) * half + j;
+      if (half_layout) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float2 w = t[e * groups];
+          const float x = a[e], y = b[e];
+          a[e] = x * w.x - y * w.y;
+          b[e] = y * w.x + x * w.y;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float2 w = t[e * groups];
+          float* v = e < 4 ? a + 2 * e : b + 2 * (e - 4);
+          const float x = v[0], y = v[1];
+          v[0] = x * w.x - y * w.y;
+          v[1] = y * w.x + x * w.y;
+        }
+      }
+    }
+    const int d0 = start(j, turns), d1 = second(j, turns);
+    if (hk < 0) {
+      if (active && (slot != -2 || p.clear_tail)) {
+        T* dst = reinterpret_cast<T*>(p.q_out) + (int64_t)row * p.qo_stride_n + (int64_t)head * p.qo_stride_h;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(dst + d0) = slot == -2 ? zero : close8<T>(a);
+        *reinterpret_cast<uint4*>(dst + d1) = slot == -2 ? zero : close8<T>(b);
+      }
+    } else if (!I8 && active && slot >= 0) {
+      T* dst = hv < 0 ? reinterpret_cast<T*>(p.cache_k) + slot * p.ck_stride_t + (int64_t)hk * p.ck_stride_h
+                      : reinterpret_cast<T*>(p.cache_v) + slot * p.cv_stride_t + (int64_t)hv * p.cv_stride_h;
+      *reinterpret_cast<uint4*>(dst + d0) = close8<T>(a);
+      *reinterpret_cast<uint4*>(dst + d1) = close8<T>(b);
+    }
+    if constexpr (I8) {
+      // the lanes of a head are neighbours in a warp (all lanes take part, also those without a unit)
+      float amax = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fmaxf(fabsf(a[e]), fabsf(b[e])));
+      for (int o = 1; o < (1 << lanes); o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (hk >= 0 && active && slot >= 0) {
+        const __half scale = __float2half_rn(amax == 0.f ? 1.f : fminf(fmaxf(amax / 127.f, 5.9604644775390625e-8f), 65504.f));
+        const float sc = __half2float(scale);
+        int8_t* dst = hv < 0 ? reinterpret_cast<int8_t*>(p.cache_k) + slot * p.ck_stride_t + (int64_t)hk * p.ck_stride_h
+                             : reinterpret_cast<int8_t*>(p.cache_v) + slot * p.cv_stride_t + (int64_t)hv * p.cv_stride_h;
+        *reinterpret_cast<uint2*>(dst + d0) = bytes8(a, sc);
+        *reinterpret_cast<uint2*>(dst + d1) = bytes8(b, sc);
+        if (j == 0) {
+          if (hv < 0) reinterpret_cast<__half*>(p.k_scale)[slot * p.ks_stride_t + (int64_t)hk * p.ks_stride_h] = scale;
+          else reinterpret_cast<__half*>(p.v_scale)[slot * p.vs_stride_t + (int64_t)hv * p.vs_stride_h] = scale;
+        }
+      }
+    }
+  }
+}
+
+bool whole_vectors(const WsvdKvRopeAppendParams& p) {
+  const bool i8 = p.cache_dtype == WSVD_I8;
+  if (p.head_dim % 16 || p.rot_dim % 16) return false;
+  const uintptr_t in = reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) |
+                       (p.n_q_heads > 0 ? reinterpret_cast<uintptr_t>(p.q) | reinterpret_cast<uintptr_t>(p.q_out) : 0);
+  const uintptr_t held = reinterpret_cast<uintptr_t>(p.cache_k) | reinterpret_cast<uintptr_t>(p.cache_v);
+  int64_t strides = p.k_stride_n | p.k_stride_h | p.v_stride_n | p.v_stride_h | p.ck_stride_t | p.ck_stride_h | p.cv_stride_t |
+                    p.cv_stride_h;
+  if (p.n_q_heads > 0) strides |= p.q_stride_n | p.q_stride_h | p.qo_stride_n | p.qo_stride_h;
+  return (in & 15) == 0 && (held & (i8 ? 7 : 15)) == 0 && strides % 8 == 0;
+}
+
+template <typename T, bool I8, int U>
+cudaError_t launch_vec(const WsvdKvRopeAppendParams& p, int lanes, int per_row, cudaStream_t s) {
+  const int64_t total = (int64_t)p.rows * per_row;
+  const int most_rows = (kVecThreads * U - 1) / per_row + 2;
+  const size_t smem = (size_t)most_rows * (2 * sizeof(int64_t) + p.rot_dim / 2 * sizeof(float2));
+  return launch_overlapped(kv_append_vec_kernel<T, I8, U>, dim3((unsigned)((total + kVecThreads * U - 1) / (kVecThreads * U))),
+                           kVecThreads, smem, s, p, lanes, Divisor::of(per_row), most_rows);
+}
+
 template <typename T, bool I8>
-void launch_any(const WsvdKvRopeAppendParams& p, cudaStream_t s) {
+cudaError_t launch_append(const WsvdKvRopeAppendParams& p, cudaStream_t s) {
+  int lanes = 0;
+  while (16 << lanes < p.head_dim) ++lanes;
+  const int64_t heads = p.n_q_heads + 2 * (int64_t)p.n_kv_heads, per_row = heads << lanes, total = p.rows * per_row;
+  if (whole_vectors(p) && total < (1ll << 31) - 4096) {
+    return total >= kManyUnits ? launch_vec<T, I8, 4>(p, lanes, (int)per_row, s) : launch_vec<T, I8, 1>(p, lanes, (int)per_row, s);
+  }
   const int64_t items = (int64_t)p.rows * (p.n_q_heads + 2 * p.n_kv_heads);
   kv_append_any_kernel<T, I8><<<(unsigned)((items + 3) / 4), 128, 0, s>>>(p);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -163,11 +383,8 @@ extern "C" int wsvd_kv_rope_append(const WsvdKvRopeAppendParams* p, void* stream
   if (i8 && (!p->k_scale || !p->v_scale)) return WSVD_ERR_BAD_DTYPE;
   if ((int64_t)p->rows * ((int64_t)p->n_q_heads + 2 * (int64_t)p->n_kv_heads) > (int64_t)1 << 32) return WSVD_ERR_TOO_LARGE;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (p->dtype == WSVD_F16) {
-    i8 ? wsvd::launch_any<__half, true>(*p, s) : wsvd::launch_any<__half, false>(*p, s);
-  } else {
-    i8 ? wsvd::launch_any<__nv_bfloat16, true>(*p, s) : wsvd::launch_any<__nv_bfloat16, false>(*p, s);
-  }
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = p->dtype == WSVD_F16 ? (i8 ? wsvd::launch_append<__half, true>(*p, s) : wsvd::launch_append<__half, false>(*p, s))
+                        : i8                 ? wsvd::launch_append<__nv_bfloat16, true>(*p, s)
+                                             : wsvd::launch_append<__nv_bfloat16, false>(*p, s);
   return e == cudaSuccess ? WSVD_OK : wsvd::record_cuda_error(e);
 }

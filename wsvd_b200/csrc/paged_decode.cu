@@ -776,23 +776,6 @@ int sm_count(int device) {
   return counts[device];
 }
 
-template <typename K, typename... Args>
-cudaError_t launch(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  // the kernel's set-up may overlap the end of the kernel in front of it: both wait (griddepcontrol.wait) before they
-  // read or write anything
-  cudaLaunchAttribute attr = {};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <typename C>
 cudaError_t launch_fast(const WsvdPagedDecodeParams& p, const Items& it, const Partials& part, cudaStream_t s) {
   constexpr size_t kRing = (size_t)kWarps * C::STAGES * C::STAGE_BYTES;
@@ -815,9 +798,9 @@ cudaError_t launch_fast(const WsvdPagedDecodeParams& p, const Items& it, const P
   if (grid > kMaxShares) grid = kMaxShares;
   if (grid > most) grid = most;
   if (grid < 1) grid = 1;
-  e = launch(paged_decode_kernel<C>, dim3((unsigned)grid), kThreads, smem, s, p, part, it.group, it.hpi, it.chunks);
+  e = launch_overlapped(paged_decode_kernel<C>, dim3((unsigned)grid), kThreads, smem, s, p, part, it.group, it.hpi, it.chunks);
   if (e != cudaSuccess || grid == 1 || reach <= C::TILE) return e;  // (one tile an item: no partials)
-  return launch(paged_merge_kernel<typename C::T, C::D>, dim3(p.n_q_heads, p.batch), kMergeWarps * 32, 0, s, p, part, it.group,
+  return launch_overlapped(paged_merge_kernel<typename C::T, C::D>, dim3(p.n_q_heads, p.batch), kMergeWarps * 32, 0, s, p, part, it.group,
                 it.hpi, it.chunks);
 }
 
