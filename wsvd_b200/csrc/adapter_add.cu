@@ -3,6 +3,8 @@
 //   out[n] = y[n] + scale[i] (x[n] A_i) B_i,   i = adapter[request of row n]
 //
 // Two kernels: h = x A in f32 (shrink) and out = y + scale h B (expand).
+#include <type_traits>
+
 #include "dense_ops.cuh"
 
 namespace wsvd {
@@ -50,10 +52,617 @@ __global__ void __launch_bounds__(256) expand_any_kernel(const __grid_constant__
   reinterpret_cast<T*>(p.out)[(int64_t)n * p.out_stride + c] = narrow<T>(y + s);
 }
 
+// ---- one row per request (a decode step): products on the CUDA cores, weights read once per four rows that share them
+//
+// Bound by the adapters' bytes.  Every row of the batch has its blocks; those of a row that is the first, fifth, ... of its
+// adapter in the batch do the work for it and the next three, so that an adapter comes from memory once and from L2 once
+// per four rows, whatever the order of the requests.  The input's length is cut into slices over the blocks; the slices'
+// sums are added in a fixed order by the expanding blocks, which have asked for their weights before (they are launched
+// while the shrinking ones still run).
+constexpr int kStepRows = 4, kStepThreads = 128, kStepCols = 8 * kStepThreads, kMaxSlices = 64, kMaxSlice = 2048;
+
+// The rows (at most four) that the blocks of row n work for: rows[0] = n; 0 where another row's blocks do, or there is no
+// adapter.  The first warp looks the batch over; all threads get the answer.
+struct Rows {
+  int count, adapter;
+  int row[kStepRows];
+};
+__device__ __forceinline__ void rows_of(const WsvdAdapterAddParams& p, int n, Rows* sm) {
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x, mine = adapter_of(p, n);
+    int before = 0, count = 0, row[kStepRows] = {n, n, n, n};
+    if (mine >= 0) {
+      count = 1;
+      for (int j0 = 0; j0 < p.batch && count < kStepRows; j0 += 128) {
+        int a[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = j0 + 32 * i + lane;
+          a[i] = j < p.batch ? p.adapter[j] : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int j = j0 + 32 * i;
+          unsigned same = __ballot_sync(0xffffffffu, a[i] == mine);
+          const unsigned up_to = n >= j + 31 ? 0xffffffffu : n < j ? 0u : (2u << (n - j)) - 1u;  // rows up to n
+          before += __popc(same & up_to);
+          same &= ~up_to;
+          while (same != 0 && count < kStepRows) {
+            row[count++] = j + __ffs(same) - 1;
+            same &= same - 1;
+          }
+        }
+      }
+      if ((before - 1) % kStepRows != 0) count = 0;  // (`before` counts row n itself)
+    }
+    if (lane == 0) {
+      sm->count = count;
+      sm->adapter = mine;
+#pragma unroll
+      for (int i = 0; i < kStepRows; ++i) sm->row[i] = row[i];
+    }
+  }
+  __syncthreads();
+}
+
 template <typename T>
-void launch_any(const WsvdAdapterAddParams& p, float* h, cudaStream_t s) {
+__device__ __forceinline__ float2 two(uint32_t v);
+template <>
+__device__ __forceinline__ float2 two<__half>(uint32_t v) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+template <>
+__device__ __forceinline__ float2 two<__nv_bfloat16>(uint32_t v) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
+template <typename T>
+__device__ __forceinline__ uint32_t both(float x, float y);
+template <>
+__device__ __forceinline__ uint32_t both<__half>(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t both<__nv_bfloat16>(float x, float y) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// h[slice][row][r]: the sum over the slice's inputs.  A thread has four neighbouring ranks and every `lanes`-th input.
+template <typename T, int R>
+__device__ __forceinline__ void step_products(const T* a, int64_t stride, int k0, int k1, int lanes, int kl, const float* xs, float (&acc)[kStepRows][4]) {
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+#pragma unroll 8
+  for (int k = k0 + kl; k < k1; k += lanes) {
+    const uint2 w = __ldg(reinterpret_cast<const uint2*>(a + (int64_t)k * stride));
+    const float2 lo = two<T>(w.x), hi = two<T>(w.y);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const float x = xs[(k - k0) * R + i];
+      acc[i][0] = fmaf(x, lo.x, acc[i][0]);
+      acc[i][1] = fmaf(x, lo.y, acc[i][1]);
+      acc[i][2] = fmaf(x, hi.x, acc[i][2]);
+      acc[i][3] = fmaf(x, hi.y, acc[i][3]);
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kStepThreads)
+shrink_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, float* h, const int slice) {
+  extern __shared__ __align__(16) float xs[];  // [inputs of the slice][rows], then [lanes][rows][rank]
+  __shared__ Rows rows;
+  before_this();
+  let_next_in();
+  rows_of(p, blockIdx.x, &rows);
+  const int count = rows.count, quads = p.rank / 4, lanes = kStepThreads / quads;
+  if (count == 0) return;
+  const int R = count == 1 ? 1 : count == 2 ? 2 : 4;
+  const int k0 = blockIdx.y * slice, k1 = min(p.n_in, k0 + slice), kl = threadIdx.x / quads, quad = threadIdx.x - kl * quads;
+  for (int i = 0; i < R; ++i) {
+    const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)rows.row[i] * p.x_stride;  // (a row that is not there: row n again)
+    for (int k = k0 + threadIdx.x; k < k1; k += kStepThreads) xs[(k - k0) * R + i] = wide(x[k]);
+  }
+  __syncthreads();
+  float acc[kStepRows][4];
+  const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)rows.adapter * p.a_stride_i + 4 * quad;
+  if (kl < lanes) {
+    if (R == 1) step_products<T, 1>(a, p.a_stride_k, k0, k1, lanes, kl, xs, acc);
+    else if (R == 2) step_products<T, 2>(a, p.a_stride_k, k0, k1, lanes, kl, xs, acc);
+    else step_products<T, 4>(a, p.a_stride_k, k0, k1, lanes, kl, xs, acc);
+  }
+  __syncthreads();
+  if (kl < lanes) {
+#pragma unroll
+    for (int i = 0; i < kStepRows; ++i)
+      if (i < R)
+        *reinterpret_cast<float4*>(xs + (kl * R + i) * p.rank + 4 * quad) = make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < count * p.rank; j += kStepThreads) {
+    const int i = j / p.rank, r = j - i * p.rank;
+    float s = 0.f;
+    for (int l = 0; l < lanes; ++l) s += xs[(l * R + i) * p.rank + r];
+    h[((int64_t)blockIdx.y * p.rows + rows.row[i]) * p.rank + r] = s;
+  }
+}
+
+// out[row][8 columns a thread] of up to four rows
+template <typename T>
+__global__ void __launch_bounds__(kStepThreads)
+expand_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* h, const int slices) {
+  extern __shared__ __align__(16) float hs[];  // [rank][rows]
+  __shared__ Rows rows;
+  // What is read before the wait is nothing that the shrinking kernel writes, and that one has waited for what is in front
+  // of it before it let this one in.  (Without adapters it does not run.)
+  if (p.n_adapters == 0) before_this();
+  rows_of(p, blockIdx.x, &rows);
+  const int col = (blockIdx.y * kStepThreads + threadIdx.x) * 8, count = rows.count;
+  const bool on = col < p.n_out;
+  if (rows.adapter < 0) {  // no adapter: y goes through
+    before_this();
+    const int n = blockIdx.x;
+    if (on)
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + (int64_t)n * p.out_stride + col) =
+          *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.y) + (int64_t)n * p.y_stride + col);
+    return;
+  }
+  if (count == 0) {
+    before_this();  // (no block ends before the shrinking kernel has)
+    return;
+  }
+  const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)rows.adapter * p.b_stride_i + (on ? col : 0);
+  if (on && (threadIdx.x & 7) == 0)
+    for (int r = 0; r < p.rank; ++r) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(b + (int64_t)r * p.b_stride_r));
+  before_this();
+  for (int j = threadIdx.x; j < kStepRows * p.rank; j += kStepThreads) {
+    const int i = j / p.rank, r = j - i * p.rank;
+    float s = 0.f;
+    if (i < count) {
+      const float* at = h + (int64_t)rows.row[i] * p.rank + r;
+#pragma unroll 8
+      for (int l = 0; l < slices; ++l) s += at[(int64_t)l * p.rows * p.rank];
+      if (p.scale != nullptr) s *= p.scale[rows.adapter];
+    }
+    hs[r * kStepRows + i] = s;
+  }
+  __syncthreads();
+  if (!on) return;
+  float acc[kStepRows][8];
+#pragma unroll
+  for (int i = 0; i < kStepRows; ++i)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[i][e] = 0.f;
+  auto add = [&](auto rows_at_once) {
+    constexpr int R = decltype(rows_at_once)::value;
+#pragma unroll 8
+    for (int r = 0; r < p.rank; ++r) {
+      const uint4 w = __ldg(reinterpret_cast<const uint4*>(b + (int64_t)r * p.b_stride_r));
+      const float4 f = *reinterpret_cast<const float4*>(hs + r * kStepRows);
+      const float x[4] = {f.x, f.y, f.z, f.w};
+      const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 t = two<T>(v[e]);
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+          acc[i][2 * e] = fmaf(x[i], t.x, acc[i][2 * e]);
+          acc[i][2 * e + 1] = fmaf(x[i], t.y, acc[i][2 * e + 1]);
+        }
+      }
+    }
+  };
+  if (count == 1) add(std::integral_constant<int, 1>{});
+  else if (count == 2) add(std::integral_constant<int, 2>{});
+  else add(std::integral_constant<int, 4>{});
+#pragma unroll
+  for (int i = 0; i < kStepRows; ++i) {
+    if (i >= count) continue;
+    const uint4 y = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.y) + (int64_t)rows.row[i] * p.y_stride + col);
+    const uint32_t v[4] = {y.x, y.y, y.z, y.w};
+    uint32_t o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 t = two<T>(v[e]);
+      o[e] = both<T>(t.x + acc[i][2 * e], t.y + acc[i][2 * e + 1]);
+    }
+    *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + (int64_t)rows.row[i] * p.out_stride + col) = make_uint4(o[0], o[1], o[2], o[3]);
+  }
+}
+
+// ---- packed rows (prompts): products on the tensor cores, tiles of 64 rows of one request
+//
+// Bound by x, y and out.  Shrink: a warp has 16 rows and all ranks, tiles of 64 inputs come by 16-byte asynchronous copies,
+// the input's length is cut into slices so that every SM has blocks (their sums are left in f32 and added by the
+// expanding blocks in a fixed order).  Expand: a block keeps its rows' h, rounded once to the 16-bit type (a step of it is
+// 2^-9 of the adapter's share of the result, which is rounded to that type itself), and walks over 128 columns at a
+// time: B's tile from L2 and y's from memory a step ahead, y + product in place in shared memory, 16-byte stores.
+constexpr int kTileRows = 64, kTileK = 64, kTileCols = 128, kPackThreads = 128;
+
+// Tile number t of the batch: rows [row, row + rows) of one request and its adapter (-1: none).  Tiles are numbered through
+// the requests in order; what is behind the last one counts as one more request without an adapter where it is copied.
+struct RowTile {
+  int row, rows, adapter;  // rows 0: there is no such tile
+};
+__device__ __forceinline__ void tile_of(const WsvdAdapterAddParams& p, int t, RowTile* sm) {
+  __shared__ int sums[kPackThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int segments = p.batch + (p.copy_tail ? 1 : 0);
+  const int per = (segments + kPackThreads - 1) / kPackThreads, b0 = min(segments, (int)threadIdx.x * per), b1 = min(segments, b0 + per);
+  auto ends = [&](int b, int* from) {  // rows [*from, result) of segment b, inside [0, rows) whatever cu_new says
+    *from = min(max(p.cu_new[b], 0), p.rows);
+    return b < p.batch ? max(*from, min(p.cu_new[b + 1], p.rows)) : p.rows;
+  };
+  if (threadIdx.x == 0) *sm = RowTile{0, 0, -1};
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    int from;
+    const int to = ends(b, &from);
+    mine += (to - from + kTileRows - 1) / kTileRows;
+  }
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) sums[warp] = incl;
+  __syncthreads();
+  int before = incl - mine;
+  for (int w = 0; w < warp; ++w) before += sums[w];
+  if (t >= before && t < before + mine) {
+    int b = b0;
+    for (;; ++b) {
+      int from;
+      const int to = ends(b, &from), n = (to - from + kTileRows - 1) / kTileRows;
+      if (t < before + n) {
+        const int row = from + (t - before) * kTileRows;
+        int i = b < p.batch ? p.adapter[b] : -1;
+        if (i < -1 || i >= p.n_adapters) {
+          atomicMax(&g_status, kOutsideStorage);
+          i = -1;
+        }
+        *sm = RowTile{row, min(kTileRows, to - row), i};
+        break;
+      }
+      before += n;
+    }
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {  // zeros where it is not on
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(dst), "l"(src), "r"(on ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// RP: the rank rounded up to 16, 32, 64, 128 or 256.  Pitches are an odd number of 16-byte pieces (conflict-free ldmatrix).
+template <int RP>
+struct Shrink {
+  static constexpr int X_PITCH = kTileK * 2 + 16, A_PITCH = RP * 2 + 16;
+  static constexpr int STAGE = kTileRows * X_PITCH + kTileK * A_PITCH;
+  static constexpr int STAGES = RP <= 128 ? 3 : 2;
+};
+template <typename T, int RP>
+__global__ void __launch_bounds__(kPackThreads)
+shrink_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, float* h, const int slice) {
+  using S = Shrink<RP>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ RowTile tile;
+  before_this();
+  let_next_in();
+  tile_of(p, blockIdx.x, &tile);
+  if (tile.rows == 0 || tile.adapter < 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int k0 = blockIdx.y * slice, k1 = min(p.n_in, k0 + slice), steps = (k1 - k0 + kTileK - 1) / kTileK;
+  const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)tile.row * p.x_stride;
+  const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)tile.adapter * p.a_stride_i;
+  const uint32_t ring = smem_addr(smem);
+  const bool wide_a = p.rank % 8 == 0 && p.a_stride_k % 8 == 0 && p.a_stride_i % 8 == 0 && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0;
+  auto request = [&](int step) {
+    if (step < steps) {
+      const int k = k0 + step * kTileK;
+      const uint32_t xd = ring + (step % S::STAGES) * S::STAGE, ad = xd + kTileRows * S::X_PITCH;
+#pragma unroll
+      for (int i = 0; i < kTileRows * (kTileK / 8) / kPackThreads; ++i) {
+        const int piece = threadIdx.x + i * kPackThreads, row = piece / (kTileK / 8), col = (piece % (kTileK / 8)) * 8;
+        const bool on = row < tile.rows && k + col < k1;
+        copy16(xd + row * S::X_PITCH + col * 2, x + (on ? (int64_t)row * p.x_stride + k + col : 0), on);
+      }
+      if (wide_a) {
+#pragma unroll
+        for (int i = 0; i < kTileK * (RP / 8) / kPackThreads; ++i) {
+          const int piece = threadIdx.x + i * kPackThreads, row = piece / (RP / 8), col = (piece % (RP / 8)) * 8;
+          const bool on = k + row < k1 && col < p.rank;
+          copy16(ad + row * S::A_PITCH + col * 2, a + (on ? (int64_t)(k + row) * p.a_stride_k + col : 0), on);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kTileK * (RP / 4) / kPackThreads; ++i) {
+          const int piece = threadIdx.x + i * kPackThreads, row = piece / (RP / 4), col = (piece % (RP / 4)) * 4;
+          const bool on = k + row < k1 && col < p.rank;
+          copy8(ad + row * S::A_PITCH + col * 2, a + (on ? (int64_t)(k + row) * p.a_stride_k + col : 0), on);
+        }
+      }
+    }
+    copies_commit();
+  };
+  float acc[RP / 8][4];
+#pragma unroll
+  for (int j = 0; j < RP / 8; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+#pragma unroll
+  for (int i = 0; i < S::STAGES - 1; ++i) request(i);
+  for (int step = 0; step < steps; ++step) {
+    copies_wait<S::STAGES - 2>();
+    __syncthreads();  // this step's tiles are there for all, and all have done with the stage that is filled next
+    request(step + S::STAGES - 1);
+    const uint32_t xd = ring + (step % S::STAGES) * S::STAGE, ad = xd + kTileRows * S::X_PITCH;
+    const uint32_t xa = xd + (warp * 16 + (lane & 15)) * S::X_PITCH + (lane >> 4) * 16;
+    const uint32_t aa = ad + (lane & 15) * S::A_PITCH + (lane >> 4) * 16;
+#pragma unroll
+    for (int k = 0; k < kTileK / 16; ++k) {
+      uint32_t xr[4];
+      ldmatrix4(xr, xa + k * 32);
+#pragma unroll
+      for (int j = 0; j < RP / 16; ++j) {
+        uint32_t w[4];  // ranks 16 j .. + 7: w[0], w[1] (inputs 0-7, 8-15); + 8 .. + 15: w[2], w[3]
+        ldmatrix4_trans(w, aa + k * 16 * S::A_PITCH + j * 32);
+        mma<T>(acc[2 * j], xr, w[0], w[1]);
+        mma<T>(acc[2 * j + 1], xr, w[2], w[3]);
+      }
+    }
+  }
+  const int g = lane >> 2, c4 = lane & 3;
+#pragma unroll
+  for (int j = 0; j < RP / 8; ++j) {
+    const int r = 8 * j + 2 * c4;
+    if (r >= p.rank) continue;  // (rank is a multiple of 4: both of the pair or none)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = warp * 16 + g + 8 * e;
+      if (row < tile.rows)
+        *reinterpret_cast<float2*>(h + ((int64_t)blockIdx.y * p.rows + tile.row + row) * p.rank + r) = make_float2(acc[j][2 * e], acc[j][2 * e + 1]);
+    }
+  }
+}
+
+constexpr int kColPitch = kTileCols * 2 + 16;  // bytes of a tile row of B or y
+// columns [blockIdx.y * span, + span) of a tile of rows; rp: the rank rounded up to 16
+template <typename T>
+__global__ void __launch_bounds__(kPackThreads)
+expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* h, const int slices, const int rp, const int span) {
+  extern __shared__ __align__(16) unsigned char smem[];  // h [64][rp], then two stages of B [rp][128] and y [64][128]
+  __shared__ RowTile tile;
+  if (p.n_adapters == 0) before_this();
+  tile_of(p, blockIdx.x, &tile);  // (before the wait: see expand_step_kernel)
+  if (tile.rows == 0) {
+    before_this();
+    return;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c0 = blockIdx.y * span, c1 = min(p.n_out, c0 + span), steps = (c1 - c0 + kTileCols - 1) / kTileCols;
+  const T* y = reinterpret_cast<const T*>(p.y) + (int64_t)tile.row * p.y_stride;
+  T* out = reinterpret_cast<T*>(p.out) + (int64_t)tile.row * p.out_stride;
+  if (tile.adapter < 0) {
+    before_this();
+    if (p.out == p.y) return;
+    const int vecs = (c1 - c0) / 8;
+    for (int i = threadIdx.x; i < tile.rows * vecs; i += kPackThreads) {
+      const int row = i / vecs, col = c0 + (i - row * vecs) * 8;
+      *reinterpret_cast<uint4*>(out + (int64_t)row * p.out_stride + col) = *reinterpret_cast<const uint4*>(y + (int64_t)row * p.y_stride + col);
+    }
+    return;
+  }
+  const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)tile.adapter * p.b_stride_i;
+  const int h_pitch = rp * 2 + 16, b_bytes = rp * kColPitch, stage_bytes = b_bytes + kTileRows * kColPitch;
+  const uint32_t hd = smem_addr(smem), ring = hd + kTileRows * h_pitch;
+  auto request = [&](int step) {
+    if (step < steps) {
+      const int c = c0 + step * kTileCols;
+      const uint32_t bd = ring + (step & 1) * stage_bytes, yd = bd + b_bytes;
+      const int col = (threadIdx.x & 15) * 8;
+      const bool in = c + col < c1;
+      for (int row = threadIdx.x >> 4; row < rp; row += kPackThreads / 16) {
+        const bool on = in && row < p.rank;
+        copy16(bd + row * kColPitch + col * 2, b + (on ? (int64_t)row * p.b_stride_r + c + col : 0), on);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {  // the warp's own 16 rows
+        const int row = warp * 16 + 2 * i + (lane >> 4);
+        const bool on = in && row < tile.rows;
+        copy16(yd + row * kColPitch + col * 2, y + (on ? (int64_t)row * p.y_stride + c + col : 0), on);
+      }
+    }
+    copies_commit();
+  };
+  request(0);
+  before_this();
+  const float scale = p.scale != nullptr ? p.scale[tile.adapter] : 1.f;
+  for (int i = threadIdx.x; i < kTileRows * (rp / 2); i += kPackThreads) {
+    const int row = i / (rp / 2), r = (i - row * (rp / 2)) * 2;
+    float2 s = make_float2(0.f, 0.f);
+    if (row < tile.rows && r < p.rank) {
+      const float* at = h + (int64_t)(tile.row + row) * p.rank + r;
+#pragma unroll 4
+      for (int l = 0; l < slices; ++l) {
+        const float2 v = *reinterpret_cast<const float2*>(at + (int64_t)l * p.rows * p.rank);
+        s.x += v.x;
+        s.y += v.y;
+      }
+    }
+    *reinterpret_cast<uint32_t*>(smem + row * h_pitch + r * 2) = both<T>(s.x, s.y);
+  }
+  const int g = lane >> 2, c4 = lane & 3;
+  for (int step = 0; step < steps; ++step) {
+    request(step + 1);
+    copies_wait<1>();
+    __syncthreads();
+    const uint32_t bd = ring + (step & 1) * stage_bytes;
+    unsigned char* yt = smem + kTileRows * h_pitch + (step & 1) * stage_bytes + b_bytes;
+    float acc[kTileCols / 8][4];
+#pragma unroll
+    for (int j = 0; j < kTileCols / 8; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+    for (int k = 0; k < rp / 16; ++k) {
+      uint32_t hr[4];
+      ldmatrix4(hr, hd + (warp * 16 + (lane & 15)) * h_pitch + (lane >> 4) * 16 + k * 32);
+      const uint32_t ba = bd + (16 * k + (lane & 15)) * kColPitch + (lane >> 4) * 16;
+#pragma unroll
+      for (int j = 0; j < kTileCols / 16; ++j) {
+        uint32_t w[4];
+        ldmatrix4_trans(w, ba + j * 32);
+        mma<T>(acc[2 * j], hr, w[0], w[1]);
+        mma<T>(acc[2 * j + 1], hr, w[2], w[3]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kTileCols / 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(yt + (warp * 16 + g + 8 * e) * kColPitch + (8 * j + 2 * c4) * 2);
+        const float2 v = two<T>(*at);
+        *at = both<T>(fmaf(scale, acc[j][2 * e], v.x), fmaf(scale, acc[j][2 * e + 1], v.y));
+      }
+    __syncwarp();  // the warp's rows are its own
+    const int col = (lane & 15) * 8, c = c0 + step * kTileCols + col;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = warp * 16 + 2 * i + (lane >> 4);
+      if (c < c1 && row < tile.rows)
+        *reinterpret_cast<uint4*>(out + (int64_t)row * p.out_stride + c) = *reinterpret_cast<const uint4*>(yt + row * kColPitch + col * 2);
+    }
+    __syncthreads();  // the stage may be filled again
+  }
+}
+
+// ---- host side
+
+bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+// y, out and B in whole 16-byte vectors, A in whole 8-byte ones; packed rows: x in 16-byte vectors too
+bool whole_vectors(const WsvdAdapterAddParams& p) {
+  if (p.rank % 4 || p.n_out % 8) return false;
+  if (!aligned(p.y, 16) || !aligned(p.out, 16) || !aligned(p.b, 16) || !aligned(p.a, 8)) return false;
+  if ((p.y_stride | p.out_stride | p.b_stride_i | p.b_stride_r) % 8 || (p.a_stride_i | p.a_stride_k) % 4) return false;
+  if (p.cu_new == nullptr) return p.n_in <= kMaxSlices * kMaxSlice;
+  return (p.n_in % 8 == 0 && aligned(p.x, 16) && p.x_stride % 8 == 0);
+}
+int rank_padded(int rank) {
+  int r = 16;
+  while (r < rank) r *= 2;
+  return r;
+}
+int packed_tiles(const WsvdAdapterAddParams& p) { return p.rows / kTileRows + p.batch + 1; }
+// Inputs of a slice: enough blocks for every SM to have several, slices of no less than 64 inputs.
+int slice_of(const WsvdAdapterAddParams& p) {
+  const int64_t blocks = p.cu_new != nullptr ? p.rows / kTileRows + 1 : p.rows, want = p.cu_new != nullptr ? 148 * 3 : 148 * 8;
+  int64_t slices = (want + blocks - 1) / blocks;
+  const int64_t most = (p.n_in + 63) / 64;
+  const int64_t least = p.cu_new != nullptr ? 1 : (p.n_in + kMaxSlice - 1) / kMaxSlice;  // (a slice of four rows fits shared memory)
+  if (slices < least) slices = least;
+  if (slices > most) slices = most;
+  if (slices > kMaxSlices) slices = kMaxSlices;
+  if (slices < 1) slices = 1;
+  return (int)(((p.n_in + slices - 1) / slices + 63) / 64 * 64);
+}
+int slices_of(const WsvdAdapterAddParams& p) { return (p.n_in + slice_of(p) - 1) / slice_of(p); }
+
+template <typename T>
+cudaError_t launch_step(const WsvdAdapterAddParams& p, float* h, cudaStream_t s) {
+  const int slice = slice_of(p), slices = slices_of(p);
+  const int lanes = kStepThreads / (p.rank / 4);
+  const size_t xs = (size_t)slice * kStepRows, red = (size_t)lanes * kStepRows * p.rank;
+  cudaError_t e = p.n_adapters == 0 ? cudaSuccess
+                                    : launch_overlapped(shrink_step_kernel<T>, dim3(p.rows, slices), kStepThreads, (xs > red ? xs : red) * sizeof(float),
+                                                        s, p, h, slice);
+  if (e != cudaSuccess) return e;
+  return launch_overlapped(expand_step_kernel<T>, dim3(p.rows, (p.n_out + kStepCols - 1) / kStepCols), kStepThreads,
+                           (size_t)kStepRows * p.rank * sizeof(float), s, p, (const float*)h, slices);
+}
+
+// more than 48 KB of dynamic shared memory has to be asked for, once per kernel and device
+template <typename K>
+cudaError_t allow_smem(K kernel, bool (&ready)[64], size_t bytes) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess || (device < 64 && ready[device])) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && device < 64) ready[device] = true;
+  return e;
+}
+
+template <typename T, int RP>
+cudaError_t launch_shrink(const WsvdAdapterAddParams& p, float* h, cudaStream_t s) {
+  static bool ready[64];
+  constexpr size_t smem = (size_t)Shrink<RP>::STAGES * Shrink<RP>::STAGE;
+  const cudaError_t e = allow_smem(shrink_packed_kernel<T, RP>, ready, smem);
+  if (e != cudaSuccess) return e;
+  return launch_overlapped(shrink_packed_kernel<T, RP>, dim3(packed_tiles(p), slices_of(p)), kPackThreads, smem, s, p, h, slice_of(p));
+}
+
+template <typename T>
+cudaError_t launch_packed(const WsvdAdapterAddParams& p, float* h, cudaStream_t s) {
+  cudaError_t e = cudaSuccess;
+  if (p.n_adapters > 0) {
+    switch (rank_padded(p.rank)) {
+      case 16: e = launch_shrink<T, 16>(p, h, s); break;
+      case 32: e = launch_shrink<T, 32>(p, h, s); break;
+      case 64: e = launch_shrink<T, 64>(p, h, s); break;
+      case 128: e = launch_shrink<T, 128>(p, h, s); break;
+      default: e = launch_shrink<T, 256>(p, h, s); break;
+    }
+    if (e != cudaSuccess) return e;
+  }
+  static bool ready[64];
+  const int rp = (p.rank + 15) / 16 * 16;
+  auto bytes = [](int r) { return (size_t)kTileRows * (r * 2 + 16) + 2 * ((size_t)r * kColPitch + kTileRows * kColPitch); };
+  e = allow_smem(expand_packed_kernel<T>, ready, bytes(256));
+  if (e != cudaSuccess) return e;
+  // column spans: as many blocks as one wave holds (three per SM), each with as many columns as that leaves
+  const int64_t tiles = p.rows / kTileRows + 1, cols = (p.n_out + kTileCols - 1) / kTileCols;
+  int64_t spans = (148 * 3 + tiles - 1) / tiles;
+  if (spans > cols) spans = cols;
+  const int span = (int)((cols + spans - 1) / spans) * kTileCols;
+  return launch_overlapped(expand_packed_kernel<T>, dim3(packed_tiles(p), (p.n_out + span - 1) / span), kPackThreads, bytes(rp), s, p,
+                           (const float*)h, slices_of(p), rp, span);
+}
+
+template <typename T>
+cudaError_t launch_adapters(const WsvdAdapterAddParams& p, float* h, cudaStream_t s) {
+  if (whole_vectors(p)) return p.cu_new != nullptr ? launch_packed<T>(p, h, s) : launch_step<T>(p, h, s);
   shrink_any_kernel<T><<<p.rows, 128, 0, s>>>(p, h);
   expand_any_kernel<T><<<dim3(p.rows, (p.n_out + 255) / 256), 256, 0, s>>>(p, h);
+  return cudaGetLastError();
 }
 
 }  // namespace
@@ -69,8 +678,9 @@ cudaError_t reset_adapter_status() {
 extern "C" {
 
 size_t wsvd_adapter_add_workspace_bytes(const WsvdAdapterAddParams* p) {
-  if (!p || p->rows <= 0 || p->rank <= 0) return 0;
-  return (size_t)p->rows * p->rank * sizeof(float);
+  if (!p || p->rows <= 0 || p->rank <= 0 || p->n_in <= 0 || p->batch < 0) return 0;
+  // (on the kernels for any shape one slice is used)
+  return (size_t)wsvd::slices_of(*p) * p->rows * p->rank * sizeof(float);
 }
 
 int wsvd_adapter_add(const WsvdAdapterAddParams* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -87,9 +697,8 @@ int wsvd_adapter_add(const WsvdAdapterAddParams* p, void* workspace, size_t work
   if (workspace_bytes < wsvd_adapter_add_workspace_bytes(p)) return WSVD_ERR_WORKSPACE_TOO_SMALL;
   if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return WSVD_ERR_BAD_STRIDE;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (p->dtype == WSVD_F16) wsvd::launch_any<__half>(*p, reinterpret_cast<float*>(workspace), s);
-  else wsvd::launch_any<__nv_bfloat16>(*p, reinterpret_cast<float*>(workspace), s);
-  const cudaError_t e = cudaGetLastError();
+  float* h = reinterpret_cast<float*>(workspace);
+  const cudaError_t e = p->dtype == WSVD_F16 ? wsvd::launch_adapters<__half>(*p, h, s) : wsvd::launch_adapters<__nv_bfloat16>(*p, h, s);
   return e == cudaSuccess ? WSVD_OK : wsvd::record_cuda_error(e);
 }
 

@@ -44,8 +44,13 @@ __device__ __forceinline__ int sequence_of(const int32_t* cu, int batch, int n) 
   return lo;
 }
 
-// Launch of a kernel that waits (griddepcontrol.wait) before it reads or writes anything: its blocks may be set up
-// while the kernel in front of it in the stream still ends.
+// Kernels that are launched by launch_overlapped: everything in front of this one in the stream has finished ...
+__device__ __forceinline__ void before_this() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+// ... and the blocks of the next one may be set up (once all blocks of this one have said so or ended).
+__device__ __forceinline__ void let_next_in() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+
+// Launch of a kernel whose blocks may be set up while the kernel in front of it in the stream still ends: it calls
+// before_this() before it reads or writes what another kernel may have to do with.
 template <typename K, typename... Args>
 cudaError_t launch_overlapped(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args) {
   cudaLaunchConfig_t cfg = {};

@@ -203,8 +203,8 @@ kv_append_vec_kernel(const __grid_constant__ WsvdKvRopeAppendParams p, const int
   int64_t* row_slot = reinterpret_cast<int64_t*>(smem);     // -1: not stored, -2: padding
   int64_t* row_place = row_slot + most_rows;
   float2* turn = reinterpret_cast<float2*>(row_place + most_rows);  // [row][8][groups]: neighbouring units, neighbouring words
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  before_this();
+  let_next_in();
   const uint32_t total = (uint32_t)p.rows * per_row.d, first = blockIdx.x * (uint32_t)(kVecThreads * U);
   const int row0 = per_row.div(first);
   const int rows = (int)per_row.div(min(total, first + kVecThreads * U) - 1) - row0 + 1;

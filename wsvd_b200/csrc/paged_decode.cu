@@ -241,8 +241,8 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c4 = lane & 3;
   const int n_it = p.n_kv_heads * chunks;  // items (KV head, chunk of its query heads) of a sequence
 
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  before_this();
+  let_next_in();
 
   auto tiles_of = [&](int b) {
     int n = min(p.b_seq_len[b], p.max_len);
@@ -667,7 +667,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kMergeWarps * 32)
 paged_merge_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Partials part, int group, int hpi, int chunks) {
   constexpr int E = D / 32;
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  before_this();
   const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int req = p.b_req_idx[b];
   if (p.b_seq_len[b] <= 0 || p.max_len <= 0 || req < 0 || req >= p.n_req) return;
