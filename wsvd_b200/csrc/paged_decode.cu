@@ -841,7 +841,7 @@ extern "C" {
 
 size_t wsvd_paged_decode_workspace_bytes(const WsvdPagedDecodeParams* p) {
   if (!p || p->batch <= 0 || p->n_q_heads <= 0 || p->n_kv_heads <= 0 || p->n_q_heads % p->n_kv_heads || p->head_dim <= 0) return 0;
-  return wsvd::fits_tensor_cores(*p) ? wsvd::room_of(*p).total : 0;
+  return wsvd::room_of(*p).total;  // (of the tensor-core kernel: whatever the strides, addresses and lengths)
 }
 
 int wsvd_paged_decode(const WsvdPagedDecodeParams* p, void* workspace, size_t workspace_bytes, void* stream) {
@@ -863,7 +863,7 @@ int wsvd_paged_decode(const WsvdPagedDecodeParams* p, void* workspace, size_t wo
   if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return WSVD_ERR_BAD_STRIDE;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (need > 0) {
+  if (wsvd::fits_tensor_cores(*p)) {
     if (p->dtype == WSVD_F16)
       e = i8 ? wsvd::launch_tensor_cores<__half, true>(*p, workspace, s) : wsvd::launch_tensor_cores<__half, false>(*p, workspace, s);
     else

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 from typing import Callable, Optional, Tuple
 
 import torch
@@ -461,6 +462,9 @@ _pack_paged = _lib.packer(_lib.PagedDecodeParams)
 _pack_adapter = _lib.packer(_lib.AdapterAddParams)
 
 
+# The checks below, one by one with their messages, take 12 us of a call that takes 8 without them.  So each op first asks
+# in one expression whether everything is as it should be, and goes through them only if it is not.
+
 def _tensor(name, t, dtypes, ndim, inner_contiguous=True):
     """As `_cuda_tensor`, the device left to `_on_one_gpu`."""
     if not isinstance(t, torch.Tensor):
@@ -473,42 +477,30 @@ def _tensor(name, t, dtypes, ndim, inner_contiguous=True):
         raise ValueError(f"{name}: innermost dimension must be contiguous")
 
 
-def _on_one_gpu(tensors):
-    """The index of the GPU that all of `tensors` (name, tensor or None) are on."""
-    index = tensors[0][1].get_device()
-    for name, t in tensors:
-        if t is not None and t.get_device() != index or index < 0:
-            if t is not None and not t.is_cuda:
-                raise ValueError(f"{name} must be a CUDA tensor (no CPU path exists)")
+def _on_one_gpu(**tensors):
+    index = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor (no CPU path exists)")
+        if index is None:
+            index = t.get_device()
+        elif t.get_device() != index:
             raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
-    return index
 
 
 def _no_gradient(op, *tensors):
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError(f"{op} has no backward: call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{op} has no backward: call it under torch.no_grad() or on detached tensors")
 
 
-def _new(alloc_tensor_func, shape, dtype, device, stream):
-    """A buffer of the op's own.  On a stream of the caller's its memory must not go back to the current stream's pool while
-    that one still works on it."""
-    t = alloc_tensor_func(shape, dtype=dtype, device=device)
-    if stream is not None:
-        t.record_stream(stream)
-    return t
-
-
-def _metadata(infer_state, B):
-    """(b_seq_len, b_req_idx, page table) of a batch of B sequences."""
-    lens, idx, table = infer_state.b_seq_len, infer_state.b_req_idx, infer_state.req_manager.req_to_token_indexs
+def _metadata(lens, idx, table, B):
     _tensor("b_seq_len", lens, (torch.int32,), 1)
     _tensor("b_req_idx", idx, (torch.int32,), 1)
     _tensor("req_to_token_indexs", table, (torch.int32,), 2)
     if lens.shape[0] != B or idx.shape[0] != B:
         raise ValueError("batch metadata must have one entry per sequence")
-    return lens, idx, table
 
 
 def _dense_cache(cache_k, cache_v, k_scale, v_scale, dtype, Hkv, D):
@@ -528,6 +520,79 @@ def _dense_cache(cache_k, cache_v, k_scale, v_scale, dtype, Hkv, D):
         raise TypeError("only int8 caches have scales")
 
 
+def _scales_fit(k_scale, v_scale, shape, index):
+    """Whether these are the scales of an int8 cache of this shape."""
+    return (k_scale.dtype is torch.float16 and v_scale.dtype is torch.float16 and k_scale.shape == shape[:2]
+            and v_scale.shape == shape[:2] and k_scale.get_device() == index and v_scale.get_device() == index)
+
+
+def _new(alloc_tensor_func, like, shape, dtype, stream):
+    """A buffer of the op's own.  On a stream of the caller's its memory must not go back to the current stream's pool while
+    that one still works on it."""
+    if alloc_tensor_func is torch.empty:  # (half of its time)
+        t = like.new_empty(shape) if dtype is like.dtype else like.new_empty(shape, dtype=dtype)
+    else:
+        t = alloc_tensor_func(shape, dtype=dtype, device=like.device)
+    if stream is not None:
+        t.record_stream(stream)
+    return t
+
+
+def _run(name, index, stream, *args):
+    """Call a C entry on GPU `index`, on `stream` or that GPU's current stream."""
+    entry = getattr(_lib.lib(), name)
+    if stream is None and _raw_stream is not None and torch.cuda.current_device() == index:
+        check(entry(*args, _raw_stream(index)), name)
+        return
+    with torch.cuda.device(index):
+        check(entry(*args, _stream(stream)), name)
+
+
+def _check_append(k, v, lens, idx, table, cache_k, cache_v, inv_freq, cache_k_scale, cache_v_scale, q, q_out, cu_new, pos_offset,
+                  rope_layout):
+    _tensor("k", k, _HALVES, 3)
+    dtype = k.dtype
+    _tensor("v", v, (dtype,), 3)
+    N, Hkv, D = k.shape
+    if v.shape != k.shape:
+        raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
+    _tensor("inv_freq", inv_freq, (torch.float32,), 1)
+    if Hkv < 1:
+        raise ValueError("k and v must have heads")
+    if D < 2 or D % 2 or D > 256 or 2 * inv_freq.shape[0] > D:
+        raise ValueError(f"head_dim must be even and at most 256, with at most head_dim / 2 frequencies: {D}, {inv_freq.shape[0]}")
+    _dense_cache(cache_k, cache_v, cache_k_scale, cache_v_scale, dtype, Hkv, D)
+    B = N
+    if cu_new is not None:
+        _tensor("cu_new", cu_new, (torch.int32,), 1)
+        B = cu_new.shape[0] - 1
+        if B < 0:
+            raise ValueError("cu_new must have batch + 1 entries")
+    _metadata(lens, idx, table, B)
+    if pos_offset is not None:
+        _tensor("pos_offset", pos_offset, (torch.int32,), 1)
+        if pos_offset.shape[0] != B:
+            raise ValueError("pos_offset must have batch entries")
+    if rope_layout not in ROPE:
+        raise ValueError(f"rope_layout must be one of {list(ROPE)}")
+    if q is not None:
+        _tensor("q", q, (dtype,), 3)
+        if q.shape[0] != N or q.shape[2] != D:
+            raise ValueError(f"q must be [{N}, Hq, {D}], got {tuple(q.shape)}")
+        if q_out is not None:
+            _tensor("q_out", q_out, (dtype,), 3)
+            if q_out.shape != q.shape:
+                raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
+            if q_out.data_ptr() == q.data_ptr() and q_out.stride() != q.stride() and q.numel() > 0:
+                raise ValueError("q_out may be q itself, not another view of its storage")
+    elif q_out is not None:
+        raise ValueError("q_out without q")
+    _no_gradient("kv_rope_append", k, v, q, q_out, cache_k, cache_v)
+    _on_one_gpu(k=k, v=v, q=q, q_out=q_out, cache_k=cache_k, cache_v=cache_v, cache_k_scale=cache_k_scale,
+                cache_v_scale=cache_v_scale, inv_freq=inv_freq, b_seq_len=lens, b_req_idx=idx, req_to_token_indexs=table,
+                cu_new=cu_new, pos_offset=pos_offset)
+
+
 def kv_rope_append(k, v, infer_state, cache_k, cache_v, inv_freq, *, cache_k_scale=None, cache_v_scale=None, q=None,
                    q_out=None, cu_new=None, pos_offset=None, rope_layout="half", stream=None):
     """Store new keys and values in the paged cache (in place), the keys rotated to their positions on the way; with `q`,
@@ -545,68 +610,88 @@ def kv_rope_append(k, v, infer_state, cache_k, cache_v, inv_freq, *, cache_k_sca
     Rows behind cu_new[B] are padding: nothing of them is stored, a `q_out` of the caller's keeps its rows, the op's own has
     zeros there.  A row without a place in the table or the cache is skipped and reported by `kernel_status`.
     The reference's dense caches are made by its test script (efficiency/test_timing_layer.py)."""
-    _tensor("k", k, _HALVES, 3)
-    dtype = k.dtype
-    _tensor("v", v, (dtype,), 3)
-    N, Hkv, D = k.shape
-    if v.shape != k.shape:
-        raise ValueError(f"k and v must have one shape, got {tuple(k.shape)} and {tuple(v.shape)}")
-    _tensor("inv_freq", inv_freq, (torch.float32,), 1)
-    rot = 2 * inv_freq.shape[0]
-    if D % 2 or D > 256 or rot > D:
-        raise ValueError(f"head_dim must be even and at most 256, with at most head_dim / 2 frequencies: {D}, {rot // 2}")
-    _dense_cache(cache_k, cache_v, cache_k_scale, cache_v_scale, dtype, Hkv, D)
-    if cu_new is None:
-        B = N
-    else:
-        _tensor("cu_new", cu_new, (torch.int32,), 1)
-        B = cu_new.shape[0] - 1
-        if B < 0:
-            raise ValueError("cu_new must have batch + 1 entries")
-    lens, idx, table = _metadata(infer_state, B)
-    if pos_offset is not None:
-        _tensor("pos_offset", pos_offset, (torch.int32,), 1)
-        if pos_offset.shape[0] != B:
-            raise ValueError("pos_offset must have batch entries")
-    if rope_layout not in ROPE:
-        raise ValueError(f"rope_layout must be one of {list(ROPE)}")
-    own = False
-    Hq = 0
-    if q is not None:
-        _tensor("q", q, (dtype,), 3)
-        Hq = q.shape[1]
-        if q.shape[0] != N or q.shape[2] != D:
-            raise ValueError(f"q must be [{N}, Hq, {D}], got {tuple(q.shape)}")
-        if q_out is not None:
-            _tensor("q_out", q_out, (dtype,), 3)
-            if q_out.shape != q.shape:
-                raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
-            if q_out.data_ptr() == q.data_ptr() and q_out.stride() != q.stride():
-                raise ValueError("q_out may be q itself, not another view of its storage")
-    elif q_out is not None:
-        raise ValueError("q_out without q")
-    _no_gradient("kv_rope_append", k, v, q, q_out, cache_k, cache_v)
-    index = _on_one_gpu((("k", k), ("v", v), ("q", q), ("q_out", q_out), ("cache_k", cache_k), ("cache_v", cache_v),
-                         ("cache_k_scale", cache_k_scale), ("cache_v_scale", cache_v_scale), ("inv_freq", inv_freq),
-                         ("b_seq_len", lens), ("b_req_idx", idx), ("req_to_token_indexs", table), ("cu_new", cu_new),
-                         ("pos_offset", pos_offset)))
-    if q is not None and q_out is None:
-        own = True
-        q_out = _new(torch.empty, (N, Hq, D), dtype, q.device, stream)
-    i8 = cache_k.dtype == torch.int8
+    lens, idx, table = infer_state.b_seq_len, infer_state.b_req_idx, infer_state.req_manager.req_to_token_indexs
+    try:
+        N, Hkv, D = shape = k.shape
+        k0, k1, k2 = k.stride()
+        v0, v1, v2 = v.stride()
+        ck0, ck1, ck2 = cache_k.stride()
+        cv0, cv1, cv2 = cache_v.stride()
+        table0, table1 = table.stride()
+        dtype, held, index = k.dtype, cache_k.dtype, k.get_device()
+        B = N if cu_new is None else cu_new.shape[0] - 1
+        rot = 2 * inv_freq.shape[0]
+        store = cache_k.shape
+        fine = (
+            index >= 0 and v.get_device() == index and cache_k.get_device() == index and cache_v.get_device() == index
+            and inv_freq.get_device() == index and lens.get_device() == index and idx.get_device() == index
+            and table.get_device() == index and dtype in _HALVES and v.dtype is dtype and cache_v.dtype is held
+            and (held is dtype and cache_k_scale is None and cache_v_scale is None
+                 or held is torch.int8 and _scales_fit(cache_k_scale, cache_v_scale, store, index))
+            and v.shape == shape and store[1:] == shape[1:] and cache_v.shape == store and k2 == v2 == ck2 == cv2 == table1 == 1
+            and D % 2 == 0 and 2 <= D <= 256 and rot <= D and Hkv > 0 and inv_freq.dtype is torch.float32
+            and lens.dtype is torch.int32 and idx.dtype is torch.int32 and table.dtype is torch.int32
+            and lens.shape == (B,) and idx.shape == (B,) and rope_layout in ROPE and q_out is None and inv_freq.stride() == (1,)
+            and lens.stride() == (1,) and idx.stride() == (1,)
+            and (q is None or q.shape[0] == N and q.shape[2] == D and q.dtype is dtype and q.get_device() == index and q.stride(2) == 1)
+            and (cu_new is None or cu_new.dtype is torch.int32 and cu_new.get_device() == index and cu_new.stride() == (1,))
+            and (pos_offset is None or pos_offset.dtype is torch.int32 and pos_offset.shape == (B,)
+                 and pos_offset.get_device() == index and pos_offset.stride() == (1,))
+            and not (torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or cache_k.requires_grad or
+                                                  cache_v.requires_grad or q is not None and q.requires_grad)))
+    except (AttributeError, TypeError, ValueError, IndexError):
+        fine = False
+    if not fine:
+        _check_append(k, v, lens, idx, table, cache_k, cache_v, inv_freq, cache_k_scale, cache_v_scale, q, q_out, cu_new, pos_offset,
+                      rope_layout)
+    own = q is not None and q_out is None
+    if own:
+        q_out = _new(torch.empty, q, q.shape, dtype, stream)
+    code, i8 = _CODE[dtype], held is torch.int8
     args = _pack_append(
-        k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-        *((0, 0, 0, 0, 0, 0) if q is None else
-          (q.data_ptr(), q.stride(0), q.stride(1), q_out.data_ptr(), q_out.stride(0), q_out.stride(1))),
-        cache_k.data_ptr(), cache_k.stride(0), cache_k.stride(1), cache_v.data_ptr(), cache_v.stride(0), cache_v.stride(1),
+        k.data_ptr(), k0, k1, v.data_ptr(), v0, v1,
+        *((0, 0, 0, 0, 0, 0) if q is None else (q.data_ptr(), *q.stride()[:2], q_out.data_ptr(), *q_out.stride()[:2])),
+        cache_k.data_ptr(), ck0, ck1, cache_v.data_ptr(), cv0, cv1,
         *((cache_k_scale.data_ptr(), *cache_k_scale.stride(), cache_v_scale.data_ptr(), *cache_v_scale.stride()) if i8 else
           (0, 0, 0, 0, 0, 0)),
-        inv_freq.data_ptr(), table.data_ptr(), table.stride(0), idx.data_ptr(), lens.data_ptr(),
-        0 if cu_new is None else cu_new.data_ptr(), 0 if pos_offset is None else pos_offset.data_ptr(), cache_k.shape[0],
-        N, B, Hq, Hkv, D, rot, table.shape[1], table.shape[0], _CODE[dtype], I8 if i8 else _CODE[dtype], ROPE[rope_layout], own)
-    with _on_device(k.device):
-        check(_lib.lib().wsvd_kv_rope_append(args, _stream(stream)), "wsvd_kv_rope_append")
+        inv_freq.data_ptr(), table.data_ptr(), table0, idx.data_ptr(), lens.data_ptr(),
+        0 if cu_new is None else cu_new.data_ptr(), 0 if pos_offset is None else pos_offset.data_ptr(), store[0],
+        N, B, 0 if q is None else q.shape[1], Hkv, D, rot, table.shape[1], table.shape[0], code, I8 if i8 else code,
+        ROPE[rope_layout], own)
+    _run("wsvd_kv_rope_append", index, stream, args)
     return q_out
+
+
+@functools.lru_cache(maxsize=256)
+def paged_decode_workspace_bytes(batch, n_q_heads, n_kv_heads, head_dim) -> int:
+    """Bytes of scratch that `paged_decode` needs for these sizes, whatever the lengths (nothing in it has to be set)."""
+    p = _lib.PagedDecodeParams()
+    p.batch, p.n_q_heads, p.n_kv_heads, p.head_dim = batch, n_q_heads, n_kv_heads, head_dim
+    return int(_lib.lib().wsvd_paged_decode_workspace_bytes(ctypes.byref(p)))
+
+
+def _check_paged(q, lens, idx, table, cache_k, cache_v, k_scale, v_scale, out, window, workspace):
+    _tensor("q", q, _HALVES, 3)
+    B, Hq, D = q.shape
+    _tensor("cache_k", cache_k, (q.dtype, torch.int8), 3)
+    Hkv = cache_k.shape[1]
+    if D < 1 or D > 256:
+        raise ValueError(f"head_dim {D} not in [1, 256]")
+    _dense_cache(cache_k, cache_v, k_scale, v_scale, q.dtype, Hkv, D)
+    if Hkv < 1 or Hq < 1 or Hq % Hkv:
+        raise ValueError(f"q heads ({Hq}) must be a multiple of KV heads ({Hkv})")
+    _metadata(lens, idx, table, B)
+    if out is not None:
+        _tensor("out", out, (q.dtype,), 3)
+        if out.shape != q.shape:
+            raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    if window < 0:
+        raise ValueError("window must not be negative")
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    _no_gradient("paged_decode", q, cache_k, cache_v, out)
+    _on_one_gpu(q=q, cache_k=cache_k, cache_v=cache_v, k_scale=k_scale, v_scale=v_scale, b_seq_len=lens, b_req_idx=idx,
+                req_to_token_indexs=table, out=out, workspace=workspace)
 
 
 def paged_decode(q, infer_state, cache_k, cache_v, k_scale=None, v_scale=None, *, out=None, return_lse=False, window=0,
@@ -622,65 +707,64 @@ def paged_decode(q, infer_state, cache_k, cache_v, k_scale=None, v_scale=None, *
     reported by `kernel_status`, a length is clamped to the table's width.  `sm_scale` 0 means 1/sqrt(D).
     `workspace`: an optional CUDA byte/float buffer of `paged_decode_workspace_bytes` bytes; calls that may
     run at the same time need one each.  (`dense_decode` is the reference's f16 baseline.)"""
-    _tensor("q", q, _HALVES, 3)
-    B, Hq, D = q.shape
-    dtype = q.dtype
-    _tensor("cache_k", cache_k, (dtype, torch.int8), 3)
-    Hkv = cache_k.shape[1]
-    if D < 1 or D > 256:
-        raise ValueError(f"head_dim {D} not in [1, 256]")
-    _dense_cache(cache_k, cache_v, k_scale, v_scale, dtype, Hkv, D)
-    if Hkv < 1 or Hq < 1 or Hq % Hkv:
-        raise ValueError(f"q heads ({Hq}) must be a multiple of KV heads ({Hkv})")
-    lens, idx, table = _metadata(infer_state, B)
-    if out is not None:
-        _tensor("out", out, (dtype,), 3)
-        if out.shape != q.shape:
-            raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+    lens, idx, table = infer_state.b_seq_len, infer_state.b_req_idx, infer_state.req_manager.req_to_token_indexs
     window = int(window)
-    if window < 0:
-        raise ValueError("window must not be negative")
-    if workspace is not None and not workspace.is_contiguous():
-        raise ValueError("workspace must be contiguous")
-    _no_gradient("paged_decode", q, cache_k, cache_v, out)
-    _on_one_gpu((("q", q), ("cache_k", cache_k), ("cache_v", cache_v), ("k_scale", k_scale), ("v_scale", v_scale),
-                 ("b_seq_len", lens), ("b_req_idx", idx), ("req_to_token_indexs", table), ("out", out),
-                 ("workspace", workspace)))
-    device = q.device
+    try:
+        B, Hq, D = shape = q.shape
+        T, Hkv, _ = store = cache_k.shape
+        q0, q1, q2 = q.stride()
+        k0, k1, k2 = cache_k.stride()
+        v0, v1, v2 = cache_v.stride()
+        table0, table1 = table.stride()
+        dtype, held, index = q.dtype, cache_k.dtype, q.get_device()
+        fine = (
+            index >= 0 and cache_k.get_device() == index and cache_v.get_device() == index and lens.get_device() == index
+            and idx.get_device() == index and table.get_device() == index and dtype in _HALVES and cache_v.dtype is held
+            and (held is dtype and k_scale is None and v_scale is None
+                 or held is torch.int8 and _scales_fit(k_scale, v_scale, store, index))
+            and store[2] == D and cache_v.shape == store and q2 == k2 == v2 == table1 == 1 and 1 <= D <= 256
+            and Hkv > 0 and Hq > 0 and Hq % Hkv == 0 and lens.dtype is torch.int32 and idx.dtype is torch.int32
+            and table.dtype is torch.int32 and lens.shape == (B,) and idx.shape == (B,) and lens.stride() == (1,)
+            and idx.stride() == (1,) and window >= 0
+            and (out is None or out.shape == shape and out.dtype is dtype and out.get_device() == index and out.stride(2) == 1)
+            and (workspace is None or workspace.get_device() == index and workspace.is_contiguous())
+            and not (torch.is_grad_enabled() and (q.requires_grad or cache_k.requires_grad or cache_v.requires_grad or
+                                                  out is not None and out.requires_grad)))
+    except (AttributeError, TypeError, ValueError, IndexError):
+        fine = False
+    if not fine:
+        _check_paged(q, lens, idx, table, cache_k, cache_v, k_scale, v_scale, out, window, workspace)
     if out is None:
-        out = _new(alloc_tensor_func, (B, Hq, D), dtype, device, stream)
-    lse = _new(alloc_tensor_func, (B, Hq), torch.float32, device, stream) if return_lse else None
-    i8 = cache_k.dtype == torch.int8
+        out = _new(alloc_tensor_func, q, shape, dtype, stream)
+    lse = _new(alloc_tensor_func, q, (B, Hq), torch.float32, stream) if return_lse else None
+    if workspace is None:
+        workspace = _new(alloc_tensor_func, q, (paged_decode_workspace_bytes(B, Hq, Hkv, D) // 2,), dtype, stream)
+        have = workspace.numel() * 2
+    else:
+        have = workspace.numel() * workspace.element_size()
+    code, i8 = _CODE[dtype], held is torch.int8
+    out0, out1, _ = out.stride()
     args = _pack_paged(
-        q.data_ptr(), q.stride(0), q.stride(1), cache_k.data_ptr(), cache_k.stride(0), cache_k.stride(1),
-        cache_v.data_ptr(), cache_v.stride(0), cache_v.stride(1),
+        q.data_ptr(), q0, q1, cache_k.data_ptr(), k0, k1, cache_v.data_ptr(), v0, v1,
         *((k_scale.data_ptr(), *k_scale.stride(), v_scale.data_ptr(), *v_scale.stride()) if i8 else (0, 0, 0, 0, 0, 0)),
-        table.data_ptr(), table.stride(0), idx.data_ptr(), lens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1),
-        0 if lse is None else lse.data_ptr(), cache_k.shape[0], B, Hq, Hkv, D, table.shape[1], table.shape[0], _CODE[dtype],
-        I8 if i8 else _CODE[dtype], min(window, 2 ** 31 - 1), float(sm_scale))
-    lib = _lib.lib()
-    with _on_device(device):
-        if workspace is None:
-            need = lib.wsvd_paged_decode_workspace_bytes(args)
-            workspace = _new(alloc_tensor_func, ((need + 3) // 4,), torch.float32, device, stream)
-        check(lib.wsvd_paged_decode(args, workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream)),
-              "wsvd_paged_decode")
+        table.data_ptr(), table0, idx.data_ptr(), lens.data_ptr(), out.data_ptr(), out0, out1,
+        0 if lse is None else lse.data_ptr(), T, B, Hq, Hkv, D, table.shape[1], table.shape[0], code, I8 if i8 else code,
+        min(window, 2 ** 31 - 1), float(sm_scale))
+    _run("wsvd_paged_decode", index, stream, args, workspace.data_ptr(), have)
     return (out, lse) if return_lse else out
 
 
-def adapter_add(y, x, a, b, adapter, *, scale=None, cu_new=None, out=None, workspace: Optional[torch.Tensor] = None,
-                alloc_tensor_func: Callable = torch.empty, stream=None):
-    """Low-rank adapters of many requests beside a shared projection: ``out[n] = y[n] + scale[i] * (x[n] @ a[i]) @ b[i]``
-    with ``i = adapter[request of row n]`` (-1: ``out[n] = y[n]``).
+@functools.lru_cache(maxsize=256)
+def adapter_add_workspace_bytes(rows, batch, n_in, rank, packed) -> int:
+    """Bytes of scratch that `adapter_add` needs for these sizes (packed: with a cu_new; nothing in it has to be set)."""
+    p = _lib.AdapterAddParams()
+    p.rows, p.batch, p.n_in, p.rank, p.cu_new = rows, batch, n_in, rank, 1 if packed else None
+    return int(_lib.lib().wsvd_adapter_add_workspace_bytes(ctypes.byref(p)))
 
-    x [N, n_in], y [N, n_out] (the projection's result), a [n_adapters, n_in, rank], b [n_adapters, rank, n_out], all f16 or all
-    bf16 (rows at any stride: y and out may be column slices); adapter [B] int32; scale [n_adapters] f32, None means
-    1.  Rows are packed by request, `cu_new` [B + 1] int32 as in `kv_rope_append` (None: one row per request).  Returns
-    out; `out=y` adds in place.  x a is summed in f32.  Rows behind cu_new[B] are padding: a caller's `out` keeps its rows,
-    the op's own has y's there.  An adapter that does not exist adds nothing and is reported by `kernel_status`."""
+
+def _check_adapters(y, x, a, b, adapter, scale, cu_new, out, workspace):
     _tensor("x", x, _HALVES, 2)
-    dtype = x.dtype
-    one = (dtype,)
+    one = (x.dtype,)
     _tensor("y", y, one, 2)
     _tensor("a", a, one, 3)
     _tensor("b", b, one, 3)
@@ -713,28 +797,64 @@ def adapter_add(y, x, a, b, adapter, *, scale=None, cu_new=None, out=None, works
         _tensor("out", out, one, 2)
         if out.shape != y.shape:
             raise ValueError(f"out must be {tuple(y.shape)}, got {tuple(out.shape)}")
-        if out.data_ptr() == y.data_ptr() and out.stride() != y.stride():
+        if out.data_ptr() == y.data_ptr() and out.stride() != y.stride() and y.numel() > 0:
             raise ValueError("out may be y itself, not another view of its storage")
     if workspace is not None and not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
     _no_gradient("adapter_add", y, x, a, b, out)
-    _on_one_gpu((("x", x), ("y", y), ("a", a), ("b", b), ("adapter", adapter), ("scale", scale), ("cu_new", cu_new),
-                 ("out", out), ("workspace", workspace)))
-    device = x.device
+    _on_one_gpu(x=x, y=y, a=a, b=b, adapter=adapter, scale=scale, cu_new=cu_new, out=out, workspace=workspace)
+
+
+def adapter_add(y, x, a, b, adapter, *, scale=None, cu_new=None, out=None, workspace: Optional[torch.Tensor] = None,
+                alloc_tensor_func: Callable = torch.empty, stream=None):
+    """Low-rank adapters of many requests beside a shared projection: ``out[n] = y[n] + scale[i] * (x[n] @ a[i]) @ b[i]``
+    with ``i = adapter[request of row n]`` (-1: ``out[n] = y[n]``).
+
+    x [N, n_in], y [N, n_out] (the projection's result), a [n_adapters, n_in, rank], b [n_adapters, rank, n_out], all f16 or all
+    bf16 (rows at any stride: y and out may be column slices); adapter [B] int32; scale [n_adapters] f32, None means
+    1.  Rows are packed by request, `cu_new` [B + 1] int32 as in `kv_rope_append` (None: one row per request).  Returns
+    out; `out=y` adds in place.  x a is summed in f32.  Rows behind cu_new[B] are padding: a caller's `out` keeps its rows,
+    the op's own has y's there.  An adapter that does not exist adds nothing and is reported by `kernel_status`.
+    `workspace`: an optional CUDA buffer of `adapter_add_workspace_bytes` bytes; calls that may run at the same time need one
+    each."""
+    try:
+        N, n_in = x.shape
+        count, _, rank = a.shape
+        n_out, B = y.shape[1], adapter.shape[0]
+        x0, x1 = x.stride()
+        y0, y1 = y.stride()
+        a0, a1, a2 = a.stride()
+        b0, b1, b2 = b.stride()
+        dtype, index = x.dtype, x.get_device()
+        fine = (
+            index >= 0 and y.get_device() == index and a.get_device() == index and b.get_device() == index
+            and adapter.get_device() == index and dtype in _HALVES and y.dtype is dtype and a.dtype is dtype
+            and b.dtype is dtype and adapter.dtype is torch.int32 and adapter.stride() == (1,) and y.shape == (N, n_out)
+            and a.shape[1] == n_in and b.shape == (count, rank, n_out) and 1 <= rank <= 256 and n_in > 0 and n_out > 0
+            and x1 == y1 == a2 == b2 == 1
+            and (scale is None or scale.dtype is torch.float32 and scale.shape == (count,) and scale.get_device() == index
+                 and scale.stride() == (1,))
+            and (B == N if cu_new is None else cu_new.dtype is torch.int32 and cu_new.shape == (B + 1,)
+                 and cu_new.get_device() == index and cu_new.stride() == (1,))
+            and (out is None or out is y) and (workspace is None or workspace.get_device() == index and workspace.is_contiguous())
+            and not (torch.is_grad_enabled() and (x.requires_grad or y.requires_grad or a.requires_grad or b.requires_grad)))
+    except (AttributeError, TypeError, ValueError, IndexError):
+        fine = False
+    if not fine:
+        _check_adapters(y, x, a, b, adapter, scale, cu_new, out, workspace)
     own = out is None
     if own:
-        out = _new(alloc_tensor_func, (N, n_out), dtype, device, stream)
+        out = _new(alloc_tensor_func, y, (N, n_out), dtype, stream)
+    if workspace is None:
+        workspace = _new(alloc_tensor_func, y, (adapter_add_workspace_bytes(N, B, n_in, rank, cu_new is not None) // 2,), dtype, stream)
+        have = workspace.numel() * 2
+    else:
+        have = workspace.numel() * workspace.element_size()
     args = _pack_adapter(
-        y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), a.data_ptr(), a.stride(0), a.stride(1), b.data_ptr(), b.stride(0),
-        b.stride(1), out.data_ptr(), out.stride(0), adapter.data_ptr(), 0 if scale is None else scale.data_ptr(),
-        0 if cu_new is None else cu_new.data_ptr(), N, B, n_in, n_out, rank, count, _CODE[dtype], own)
-    lib = _lib.lib()
-    with _on_device(device):
-        if workspace is None:
-            need = lib.wsvd_adapter_add_workspace_bytes(args)
-            workspace = _new(alloc_tensor_func, ((need + 3) // 4,), torch.float32, device, stream)
-        check(lib.wsvd_adapter_add(args, workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(stream)),
-              "wsvd_adapter_add")
+        y.data_ptr(), y0, x.data_ptr(), x0, a.data_ptr(), a0, a1, b.data_ptr(), b0, b1, out.data_ptr(), out.stride(0),
+        adapter.data_ptr(), 0 if scale is None else scale.data_ptr(), 0 if cu_new is None else cu_new.data_ptr(), N, B, n_in, n_out,
+        rank, count, _CODE[dtype], own)
+    _run("wsvd_adapter_add", index, stream, args, workspace.data_ptr(), have)
     return out
 
 
