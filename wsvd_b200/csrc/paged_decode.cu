@@ -201,19 +201,24 @@ struct Cfg {
   static constexpr int D = D_, NT = NT_, HEADS = 8 * NT_;               // query heads of an item, at most
   static constexpr int ROW = D * (I8 ? 1 : 2), PIECES = ROW / 16;       // bytes and 16-byte pieces of a cached row
   static constexpr int PITCH = (PIECES | 1) * 16;                       // an odd number of pieces: conflict-free ldmatrix
-  static constexpr int TOK = ROW >= 128 ? 16 : 32, SUBS = TOK / 16;     // tokens of a warp's step
+  static constexpr int TOK = ROW > 128 ? 16 : 32, SUBS = TOK / 16;      // tokens of a warp's step
   static constexpr int STAGES = ROW >= 512 ? 2 : 3;
   static constexpr int TILE = kWarps * TOK;
   static constexpr int STAGE_BYTES = 2 * TOK * PITCH;                   // K rows, then V rows
   static constexpr int O_LD = D + 4;
+  static constexpr uint32_t FULL = TOK == 32 ? 0xffffffffu : 0xffffu;
+  // f16 weights are lifted by 2^15: what is left of them below f16's range is then 2^-40 of the largest one
+  static constexpr float LIFT = std::is_same<M, __half>::value ? 15.f : 0.f;
 };
 
-// What the ring holds besides rows: which tokens count, and where a sequence and head begin and end.
+// What the ring holds besides rows: which tokens count, and (read where a run begins or ends) of which item.
 struct Step {
+  uint32_t mask;
+  int32_t flags;  // 1: first step of a run in this CTA, 2: last one
+};
+struct Run {
   int64_t item_first;  // the item's first tile in the batch's order
-  uint32_t mask;       // its tokens that count
-  int32_t flags;       // 1: first step of a run in this CTA, 2: last one
-  int32_t b, it, tiles;
+  int32_t b, it, hk, tiles;
 };
 
 // Partial sums of a run: [slot][head of the item][D] f32, (maximum, sum) beside them, and per item the first slot and how many.
@@ -231,8 +236,9 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
   constexpr int D = C::D, NT = C::NT, S = C::STAGES, TOK = C::TOK;
   extern __shared__ __align__(16) unsigned char smem[];
   __shared__ Step ring[kWarps][S];
+  __shared__ Run ring_run[kWarps][S];
   __shared__ int32_t ring_slot[C::I8 ? kWarps : 1][C::I8 ? S : 1][TOK];
-  __shared__ float2 sm_scale[C::I8 ? kWarps : 1][TOK];
+  __shared__ float4 sm_scale[C::I8 ? kWarps : 1][TOK];  // k scale, v scale, log2 |v scale|
   __shared__ float2 sm_ml[kWarps][C::HEADS];
   __shared__ int64_t sm_scan[kWarps + 1];
   __shared__ int64_t sm_before;
@@ -291,72 +297,83 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
   if (busy) {
     // ---- the cursor: the step whose rows are requested next
     int left = (int)(hi - lo);  // tiles not yet requested
-    int cb = sm_b, cit, ct, cnt = tiles_of(sm_b), first, end;
+    int cb = sm_b, cnt = tiles_of(sm_b), cit, ct, hk, first, end, s;
+    int64_t seq_first = sm_before;
     {
       const int64_t in = lo - sm_before;
       cit = (int)(in / cnt);
       ct = (int)(in - (int64_t)cit * cnt);
     }
-    int64_t seq_first = sm_before;
     const int32_t* page;
-    auto enter = [&]() {  // sequence cb
+    auto enter_sequence = [&]() {
       const Span sp = span_of(p, cb);
-      first = sp.first;
-      end = sp.end;
+      first = sp.first + warp * TOK + lane;
+      end = lane < TOK ? sp.end : 0;
       page = sp.page;
     };
-    enter();
-    bool fresh = true;  // the run begins with this step
-    int slot = -1;
-    auto fetch_slots = [&]() {  // of the cursor's step: lane i has token i's
-      const int s = first + ct * C::TILE + warp * TOK + lane;
-      slot = -1;
-      if (lane < TOK && s < end) slot = page[s];
+    // A lane's pieces of a step's rows: where 32 lanes are whole rows, every lane has one column of them
+    constexpr bool kColumns = 32 % C::PIECES == 0;
+    constexpr int ES = C::I8 ? 1 : 2;
+    const int k_row = (int)(p.k_stride_t * ES), v_row = (int)(p.v_stride_t * ES);
+    const char *kb, *vb;
+    auto enter_item = [&]() {
+      hk = cit / chunks;
+      const int col = kColumns ? (lane % C::PIECES) * 16 : 0;
+      kb = reinterpret_cast<const char*>(p.k) + (int64_t)hk * p.k_stride_h * ES + col;
+      vb = reinterpret_cast<const char*>(p.v) + (int64_t)hk * p.v_stride_h * ES + col;
+      s = first;
     };
-    const int64_t n_slots = p.n_token_slots;
-    const int k_row = (int)(p.k_stride_t * (C::I8 ? 1 : 2)), v_row = (int)(p.v_stride_t * (C::I8 ? 1 : 2));
+    enter_sequence();
+    enter_item();
+    s += ct * C::TILE;
+    int fresh = 1;  // the run begins with this step
+    const uint32_t n_slots = (uint32_t)min((int64_t)INT32_MAX, p.n_token_slots);
     const uint32_t my_ring = smem_addr(smem) + warp * S * C::STAGE_BYTES;
-    fetch_slots();
+    // lane i has token i's slot, fetched a step ahead
+    int slot = s < end ? page[s] : 0;
 
     auto request = [&](int stage) {
       if (left > 0) {
-        const int s = first + ct * C::TILE + warp * TOK + lane;
-        const bool want = lane < TOK && s < end, ok = want && slot >= 0 && (int64_t)slot < n_slots;
-        if (want && !ok) atomicMax(&g_status, kOutsideStorage);
+        const bool ok = s < end && (uint32_t)slot < n_slots;
+        if (s < end && !ok) atomicMax(&g_status, kOutsideStorage);
         const uint32_t mask = __ballot_sync(0xffffffffu, ok);
-        const int from = ok ? slot : -1;
-        const int hk = cit / chunks;
-        const char* kb = reinterpret_cast<const char*>(p.k) + (int64_t)hk * p.k_stride_h * (C::I8 ? 1 : 2);
-        const char* vb = reinterpret_cast<const char*>(p.v) + (int64_t)hk * p.v_stride_h * (C::I8 ? 1 : 2);
+        const int from = ok ? slot : 0;
         const uint32_t dst = my_ring + stage * C::STAGE_BYTES;
+        auto copy = [&](auto all) {
 #pragma unroll
-        for (int i = 0; i < TOK * C::PIECES / 32; ++i) {
-          const int piece = lane + 32 * i, row = piece / C::PIECES, col = piece - row * C::PIECES;
-          const int t = __shfl_sync(0xffffffffu, from, row);
-          const bool on = t >= 0;
-          const char* ks = kb + (on ? (int64_t)t * k_row + col * 16 : 0);
-          const char* vs = vb + (on ? (int64_t)t * v_row + col * 16 : 0);
-          copy16(dst + row * C::PITCH + col * 16, ks, on);
-          copy16(dst + TOK * C::PITCH + row * C::PITCH + col * 16, vs, on);
-        }
+          for (int i = 0; i < TOK * C::PIECES / 32; ++i) {
+            const int piece = lane + 32 * i, row = piece / C::PIECES, col = kColumns ? 0 : (piece - row * C::PIECES) * 16;
+            const uint32_t to = dst + row * C::PITCH + (piece - row * C::PIECES) * 16;
+            const int t = __shfl_sync(0xffffffffu, from, row);
+            const bool on = decltype(all)::value || ((mask >> row) & 1);
+            copy16(to, kb + (int64_t)t * k_row + col, on);
+            copy16(to + TOK * C::PITCH, vb + (int64_t)t * v_row + col, on);
+          }
+        };
+        if (mask == C::FULL) copy(std::true_type{});
+        else copy(std::false_type{});
         if constexpr (C::I8)
-          if (lane < TOK) ring_slot[warp][stage][lane] = from;
+          if (lane < TOK) ring_slot[warp][stage][lane] = ok ? slot : -1;
         const bool last = ct + 1 == cnt || left == 1;
-        if (lane == 0) ring[warp][stage] = Step{seq_first + (int64_t)cit * cnt, mask, (fresh ? 1 : 0) | (last ? 2 : 0), cb, cit, cnt};
+        if (lane == 0) {
+          ring[warp][stage] = Step{mask, fresh | (last ? 2 : 0)};
+          if (fresh || last || C::I8) ring_run[warp][stage] = Run{seq_first + (int64_t)cit * cnt, cb, cit, hk, cnt};
+        }
         fresh = last;
-        --left;
-        if (++ct == cnt) {
-          ct = 0;
-          if (++cit == n_it) {
-            cit = 0;
-            if (left > 0) {
+        if (--left > 0) {
+          s += C::TILE;
+          if (++ct == cnt) {
+            ct = 0;
+            if (++cit == n_it) {
+              cit = 0;
               seq_first += (int64_t)cnt * n_it;
               do { cnt = tiles_of(++cb); } while (cnt == 0);
-              enter();
+              enter_sequence();
             }
+            enter_item();
           }
+          slot = s < end ? page[s] : 0;
         }
-        if (left > 0) fetch_slots();
       }
       copies_commit();
     };
@@ -369,9 +386,9 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
       next_sk = next_sv = __float2half_rn(0.f);
       const int t = lane < TOK ? ring_slot[warp][stage][lane] : -1;
       if (t < 0) return;
-      const int64_t hk = ring[warp][stage].it / chunks;
-      next_sk = reinterpret_cast<const __half*>(p.k_scale)[(int64_t)t * p.ks_stride_t + hk * p.ks_stride_h];
-      next_sv = reinterpret_cast<const __half*>(p.v_scale)[(int64_t)t * p.vs_stride_t + hk * p.vs_stride_h];
+      const int64_t head = ring_run[warp][stage].hk;
+      next_sk = reinterpret_cast<const __half*>(p.k_scale)[(int64_t)t * p.ks_stride_t + head * p.ks_stride_h];
+      next_sv = reinterpret_cast<const __half*>(p.v_scale)[(int64_t)t * p.vs_stride_t + head * p.vs_stride_h];
     };
     if constexpr (C::I8) {
       __syncwarp();
@@ -386,20 +403,23 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
     for (int step = 0; step < steps; ++step) {
       request(stage == 0 ? S - 1 : stage - 1);
       if constexpr (C::I8)
-        if (lane < TOK) sm_scale[warp][lane] = make_float2(__half2float(next_sk), __half2float(next_sv));
+        if (lane < TOK) {
+          const float sv = __half2float(next_sv);
+          sm_scale[warp][lane] = make_float4(__half2float(next_sk), sv, __log2f(fmaxf(fabsf(sv), 5.9604644775390625e-8f)), 0.f);
+        }
       copies_wait<S - 1>();
       __syncwarp();
       const Step now = ring[warp][stage];
       if constexpr (C::I8)
         if (step + 1 < steps) fetch_scales(stage + 1 == S ? 0 : stage + 1);
-      const int hk = now.it / chunks, h0 = hk * group + (now.it - hk * chunks) * hpi;
-      const int heads = min(hpi, group - (now.it - hk * chunks) * hpi);
       if (now.flags & 1) {
+        const Run run = ring_run[warp][stage];
+        const int in = (run.it - run.hk * chunks) * hpi, h0 = run.hk * group + in, heads = min(hpi, group - in);
         // queries as B operand: lane (head g, dims 2 c4, 2 c4 + 1 and + 8 of every 16; bytes: dims 4 c4 .. 4 c4 + 3)
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           const bool on = 8 * j + g < heads;
-          const T* qr = reinterpret_cast<const T*>(p.q) + (int64_t)now.b * p.q_stride_b + (int64_t)(h0 + (on ? 8 * j + g : 0)) * p.q_stride_h;
+          const T* qr = reinterpret_cast<const T*>(p.q) + (int64_t)run.b * p.q_stride_b + (int64_t)(h0 + (on ? 8 * j + g : 0)) * p.q_stride_h;
           float amax = 0.f;
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
@@ -476,8 +496,7 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
       }
 
       // ---- weights
-      float sv[C::SUBS][2];
-      float top[NT][2];
+      float sv[C::SUBS][2], top[NT][2];
 #pragma unroll
       for (int j = 0; j < NT; ++j) top[j][0] = m[j][0], top[j][1] = m[j][1];
 #pragma unroll
@@ -485,23 +504,22 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int tok = 16 * u + g + 8 * e;
-          const bool on = (now.mask >> tok) & 1;
-          float sk = 1.f, lsv = 0.f;
-          sv[u][e] = 1.f;
+          float4 scales;
           if constexpr (C::I8) {
-            const float2 s = sm_scale[warp][tok];
-            sk = s.x;
-            sv[u][e] = s.y;
-            lsv = __log2f(fmaxf(fabsf(sv[u][e]), 5.9604644775390625e-8f));
+            scales = sm_scale[warp][tok];
+            sv[u][e] = scales.y;
           }
 #pragma unroll
           for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float& v = z[u][j][2 * e + i];
-              v = on ? v * (C::I8 ? cq[j][i] * sk : c) : -INFINITY;
-              top[j][i] = fmaxf(top[j][i], C::I8 ? v + lsv : v);
-            }
+            for (int i = 0; i < 2; ++i) z[u][j][2 * e + i] *= C::I8 ? cq[j][i] * scales.x : c;
+          if (now.mask != C::FULL && !((now.mask >> tok) & 1))
+#pragma unroll
+            for (int j = 0; j < NT; ++j) z[u][j][2 * e] = z[u][j][2 * e + 1] = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) top[j][i] = fmaxf(top[j][i], C::I8 ? z[u][j][2 * e + i] + scales.z : z[u][j][2 * e + i]);
         }
       bool moved = false;
 #pragma unroll
@@ -537,7 +555,7 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
             float w[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              w[i] = ex2(z[u][j][2 * e + i] - m[j][i]);
+              w[i] = ex2(z[u][j][2 * e + i] - (m[j][i] - C::LIFT));
               l[j][i] += w[i];
               if (C::I8) w[i] *= sv[u][e];
             }
@@ -580,10 +598,10 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
           }
         }
       }
-      __syncwarp();  // the stage may be filled again
-
       if (now.flags & 2) {
         // ---- the end of a run: the warps' sums joined (warps 0 and 1 write, 2 and 3 add), then the result or a partial
+        const Run run = ring_run[warp][stage];
+        const int in = (run.it - run.hk * chunks) * hpi, h0 = run.hk * group + in, heads = min(hpi, group - in);
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -620,11 +638,11 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
           }
           __syncthreads();
         }
-        const int c0 = share_owner(now.item_first, total, shares), c1 = share_owner(now.item_first + now.tiles - 1, total, shares);
-        const int64_t item = (int64_t)now.b * n_it + now.it;
+        const int c0 = share_owner(run.item_first, total, shares), c1 = share_owner(run.item_first + run.tiles - 1, total, shares);
+        const int64_t item = (int64_t)run.b * n_it + run.it;
         const int64_t at = (item + blockIdx.x) * hpi;  // (items and CTAs only grow: no two runs have the same sum)
         if (c0 == (int)blockIdx.x && threadIdx.x == 0) part.items[item] = make_int2((int)(item + c0), c1 - c0 + 1);
-        T* out = reinterpret_cast<T*>(p.out) + (int64_t)now.b * p.out_stride_b + (int64_t)h0 * p.out_stride_h;
+        T* out = reinterpret_cast<T*>(p.out) + (int64_t)run.b * p.out_stride_b + (int64_t)h0 * p.out_stride_h;
         for (int i = threadIdx.x; i < heads * D; i += kThreads) {
           const int h = i / D, d = i - h * D;
           const float o = sm_o[h * C::O_LD + d] + sm_o[(hpi + h) * C::O_LD + d];
@@ -636,14 +654,15 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
           if (c0 == c1) {
             out[(int64_t)h * p.out_stride_h + d] = narrow<T>(sum == 0.f ? 0.f : o / sum);
             if (d == 0 && p.lse != nullptr)
-              p.lse[(int64_t)now.b * p.n_q_heads + h0 + h] = sum == 0.f ? -INFINITY : (all + log2f(sum)) * kLn2;
+              p.lse[(int64_t)run.b * p.n_q_heads + h0 + h] = sum == 0.f ? -INFINITY : (all - C::LIFT + log2f(sum)) * kLn2;
           } else {
-            part.o[(at + h) * D + d] = o;
-            if (d == 0) part.ml[at + h] = make_float2(all, sum);
+            part.o[(at + h) * D + d] = o;  // (relative to the same maximum as the sum)
+            if (d == 0) part.ml[at + h] = make_float2(all - C::LIFT, sum);
           }
         }
         __syncthreads();
       }
+      __syncwarp();  // the stage may be filled again
       stage = stage + 1 == S ? 0 : stage + 1;
     }
   }
