@@ -204,7 +204,6 @@ kv_append_vec_kernel(const __grid_constant__ WsvdKvRopeAppendParams p, const int
   int64_t* row_place = row_slot + most_rows;
   float2* turn = reinterpret_cast<float2*>(row_place + most_rows);  // [row][8][groups]: neighbouring units, neighbouring words
   before_this();
-  let_next_in();
   const uint32_t total = (uint32_t)p.rows * per_row.d, first = blockIdx.x * (uint32_t)(kVecThreads * U);
   const int row0 = per_row.div(first);
   const int rows = (int)per_row.div(min(total, first + kVecThreads * U) - 1) - row0 + 1;

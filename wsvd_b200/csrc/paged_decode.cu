@@ -124,7 +124,9 @@ __global__ void __launch_bounds__(kAnyWarps * 32) paged_decode_any_kernel(const 
 // scale, so that the weights with the v scale in them stay at or below one.
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kMaxShares = 1024;  // upper bound of the grid, for the workspace
+// bounds of the shares, for the workspace: CTAs of a GPU of so many SMs, CTAs of an item
+constexpr int kMaxSms = 160, kMaxCtas = 4, kMaxParts = 128;
+constexpr int kMaxDevices = 64;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {  // zeros where it is not on
@@ -145,17 +147,25 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
 }
 __device__ __forceinline__ uint32_t turned(uint32_t v) {  // an 8 x 8 fragment of 16-bit values, transposed
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
   return r;
 }
 template <typename M>
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (sizeof(M) == 2 && std::is_same<M, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8_s8(int32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_s8_u8(int32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 template <typename M>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
@@ -187,6 +197,12 @@ __device__ __forceinline__ uint32_t bytes_to_f16(uint32_t u) {
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&k1152));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
+// Brings a line to L1 without waiting for it (the streams of rows go past L1, so it is still there when it is read).
+__device__ __forceinline__ void touch(const void* p) {
+  uint32_t ignored;
+  asm volatile("ld.global.ca.b32 %0, [%1];\n" : "=r"(ignored) : "l"(p));
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
@@ -200,15 +216,25 @@ struct Cfg {
   static constexpr bool I8 = I8_;
   static constexpr int D = D_, NT = NT_, HEADS = 8 * NT_;               // query heads of an item, at most
   static constexpr int ROW = D * (I8 ? 1 : 2), PIECES = ROW / 16;       // bytes and 16-byte pieces of a cached row
-  static constexpr int PITCH = (PIECES | 1) * 16;                       // an odd number of pieces: conflict-free ldmatrix
+  // conflict-free ldmatrix: the pieces of a row changed about by the row's number, or rows of an odd number of pieces
+  static constexpr bool SWZ = PIECES == 8 || PIECES == 16 || PIECES == 32;
+  static constexpr int PITCH = SWZ ? ROW : (PIECES | 1) * 16;
   static constexpr int TOK = ROW > 128 ? 16 : 32, SUBS = TOK / 16;      // tokens of a warp's step
-  static constexpr int STAGES = ROW >= 512 ? 2 : 3;
-  static constexpr int TILE = kWarps * TOK;
-  static constexpr int STAGE_BYTES = 2 * TOK * PITCH;                   // K rows, then V rows
-  static constexpr int O_LD = D + 4;
+  static constexpr int SLOT_BYTES = TOK * PITCH;                        // a ring slot: K or V rows of a step
+  static constexpr int RING = kWarps * 4 * SLOT_BYTES;
+  // CTAs of an SM that registers have to leave room for
+  static constexpr int CTAS = NT == 2 ? 2 : D <= 128 ? 3 : I8 ? 3 : 2;
+  // where a row's piece is, from the row's first byte (rows start on their own size where pieces change places)
+  static __device__ __forceinline__ uint32_t at(int row, int piece) {
+    return row * PITCH + (SWZ ? (piece ^ (row & 7)) * 16 : piece * 16);
+  }
+  // the address of the piece `more` (even) behind the one at `addr`: at(row, piece) + ... for piece 0 or 1
+  static __device__ __forceinline__ uint32_t skip(uint32_t addr, int more) { return SWZ ? addr ^ (more * 16) : addr + more * 16; }
   static constexpr uint32_t FULL = TOK == 32 ? 0xffffffffu : 0xffffu;
-  // f16 weights are lifted by 2^15: what is left of them below f16's range is then 2^-40 of the largest one
-  static constexpr float LIFT = std::is_same<M, __half>::value ? 15.f : 0.f;
+  // The reference of the weights is a past maximum until one is 2^SLACK above it: sums are rescaled once or twice instead of
+  // at every new maximum.  f16 weights are lifted so far that they use all of f16's range above one: 2^7 2^8 = 2^15, and
+  // what is left of them below it is 2^-31 of the reference.
+  static constexpr float SLACK = 8.f, LIFT = std::is_same<M, __half>::value ? 7.f : 0.f;
 };
 
 // What the ring holds besides rows: which tokens count, and (read where a run begins or ends) of which item.
@@ -218,7 +244,14 @@ struct Step {
 };
 struct Run {
   int64_t item_first;  // the item's first tile in the batch's order
-  int32_t b, it, hk, tiles;
+  int32_t b, it, hk, tiles, tokens;
+};
+
+// How a sequence is cut into items: `hw` neighbouring KV heads, a warp each (the CTA's other warps, where heads are few, take
+// other tokens of the same ones), and a chunk of at most 16 of the `group` query heads of each, `hpi` of `chunks`.
+// Four heads of a token-major cache are one run of memory per token, and no warp has to wait for another.
+struct Items {
+  int group, hpi, chunks, nt, hw;
 };
 
 // Partial sums of a run: [slot][head of the item][D] f32, (maximum, sum) beside them, and per item the first slot and how many.
@@ -229,23 +262,22 @@ struct Partials {
 };
 
 template <typename C>
-__global__ void __launch_bounds__(kThreads)
-paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Partials part, int group, int hpi, int chunks) {
+__global__ void __launch_bounds__(kThreads, C::CTAS)
+paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Partials part, const Items items) {
   using T = typename C::T;
   using M = typename C::M;
-  constexpr int D = C::D, NT = C::NT, S = C::STAGES, TOK = C::TOK;
-  extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ Step ring[kWarps][S];
-  __shared__ Run ring_run[kWarps][S];
-  __shared__ int32_t ring_slot[C::I8 ? kWarps : 1][C::I8 ? S : 1][TOK];
-  __shared__ float4 sm_scale[C::I8 ? kWarps : 1][TOK];  // k scale, v scale, log2 |v scale|
-  __shared__ float2 sm_ml[kWarps][C::HEADS];
-  __shared__ int64_t sm_scan[kWarps + 1];
+  constexpr int D = C::D, NT = C::NT, TOK = C::TOK, META = 4;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  __shared__ Step ring[kWarps][META];
+  __shared__ Run ring_run[kWarps][META];
+  __shared__ __half2 sm_scale[C::I8 ? kWarps : 1][TOK];  // k and v scale of the present step's tokens
+  __shared__ int64_t sm_scan[kWarps];
   __shared__ int64_t sm_before;
   __shared__ int sm_b;
-  float* sm_o = reinterpret_cast<float*>(smem + kWarps * S * C::STAGE_BYTES);  // [2][hpi][O_LD]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c4 = lane & 3;
-  const int n_it = p.n_kv_heads * chunks;  // items (KV head, chunk of its query heads) of a sequence
+  const int group = items.group, hpi = items.hpi, chunks = items.chunks;
+  const int n_it = p.n_kv_heads / items.hw * chunks;  // items of a sequence
+  const int head_of_warp = warp & (items.hw - 1), part_of_warp = warp / items.hw, tile = TOK * kWarps / items.hw;
 
   before_this();
   let_next_in();
@@ -255,10 +287,10 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
     const int req = p.b_req_idx[b];
     if (n <= 0 || req < 0 || req >= p.n_req) return 0;
     if (p.window > 0) n = min(n, p.window);
-    return (n + C::TILE - 1) / C::TILE;
+    return (n + tile - 1) / tile;
   };
 
-  // ---- this CTA's share [lo, hi) of the tiles in the order (sequence, item, tile)
+  // ---- this CTA's share [lo, hi) of the tiles in the order (sequence, item, tile); a warp takes its tokens of each
   const int per = (p.batch + kThreads - 1) / kThreads, b0 = min(p.batch, (int)threadIdx.x * per), b1 = min(p.batch, b0 + per);
   int64_t mine = 0;
   for (int b = b0; b < b1; ++b) mine += tiles_of(b);
@@ -278,36 +310,37 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
   }
   total *= n_it;
   before *= n_it;
-  const int shares = (int)min((int64_t)gridDim.x, total);
-  const bool busy = (int)blockIdx.x < shares;
-  const int64_t lo = busy ? share_begin(blockIdx.x, total, shares) : 0, hi = busy ? share_begin(blockIdx.x + 1, total, shares) : 0;
+  const int shares = (int)min((int64_t)gridDim.x, total), share = blockIdx.x;
+  const bool busy = share < shares;
+  const int64_t lo = busy ? share_begin(share, total, shares) : 0, hi = busy ? share_begin(share + 1, total, shares) : 0;
   if (busy && lo >= before && lo < before + mine * n_it) {
     int b = b0;
-    int64_t at = before;
+    int64_t first = before;
     for (;; ++b) {
       const int64_t n = (int64_t)tiles_of(b) * n_it;
-      if (lo < at + n) break;
-      at += n;
+      if (lo < first + n) break;
+      first += n;
     }
     sm_b = b;
-    sm_before = at;
+    sm_before = first;
   }
   __syncthreads();
 
   if (busy) {
     // ---- the cursor: the step whose rows are requested next
     int left = (int)(hi - lo);  // tiles not yet requested
-    int cb = sm_b, cnt = tiles_of(sm_b), cit, ct, hk, first, end, s;
+    int cb = sm_b, cnt = tiles_of(cb), cit, ct, hk, first, end, s, tokens;
     int64_t seq_first = sm_before;
     {
-      const int64_t in = lo - sm_before;
-      cit = (int)(in / cnt);
+      const int64_t in = lo - seq_first;
+      cit = (in >> 32) == 0 ? (int)((uint32_t)in / (uint32_t)cnt) : (int)(in / cnt);
       ct = (int)(in - (int64_t)cit * cnt);
     }
     const int32_t* page;
     auto enter_sequence = [&]() {
       const Span sp = span_of(p, cb);
-      first = sp.first + warp * TOK + lane;
+      first = sp.first + part_of_warp * TOK + lane;
+      tokens = sp.end - sp.first;
       end = lane < TOK ? sp.end : 0;
       page = sp.page;
     };
@@ -317,7 +350,7 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
     const int k_row = (int)(p.k_stride_t * ES), v_row = (int)(p.v_stride_t * ES);
     const char *kb, *vb;
     auto enter_item = [&]() {
-      hk = cit / chunks;
+      hk = cit / chunks * items.hw + head_of_warp;
       const int col = kColumns ? (lane % C::PIECES) * 16 : 0;
       kb = reinterpret_cast<const char*>(p.k) + (int64_t)hk * p.k_stride_h * ES + col;
       vb = reinterpret_cast<const char*>(p.v) + (int64_t)hk * p.v_stride_h * ES + col;
@@ -325,43 +358,64 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
     };
     enter_sequence();
     enter_item();
-    s += ct * C::TILE;
+    s += ct * tile;
     int fresh = 1;  // the run begins with this step
     const uint32_t n_slots = (uint32_t)min((int64_t)INT32_MAX, p.n_token_slots);
-    const uint32_t my_ring = smem_addr(smem) + warp * S * C::STAGE_BYTES;
-    // lane i has token i's slot, fetched a step ahead
+    const uint32_t my_ring = smem_addr(smem) + warp * 4 * C::SLOT_BYTES;
+    // lane i has token i's slot, fetched a step ahead; what the first steps and runs wait for is touched early
     int slot = s < end ? page[s] : 0;
+    if (s + tile < end) touch(page + s + tile);
 
-    auto request = [&](int stage) {
+    // rows of one step, K or V, to a ring slot; lane i holds token i's slot, `mask` which tokens count
+    auto copy_rows = [&](uint32_t dst, const char* base, int from, int stride, uint32_t mask) {
+      auto copy = [&](auto all) {
+#pragma unroll
+        for (int i = 0; i < TOK * C::PIECES / 32; ++i) {
+          const int piece = lane + 32 * i, row = piece / C::PIECES, col = kColumns ? 0 : (piece - row * C::PIECES) * 16;
+          const int t = __shfl_sync(0xffffffffu, from, row);
+          copy16(dst + C::at(row, piece - row * C::PIECES), base + (int64_t)t * stride + col,
+                 decltype(all)::value || ((mask >> row) & 1));
+        }
+      };
+      if (mask == C::FULL) copy(std::true_type{});
+      else copy(std::false_type{});
+    };
+    // K of the cursor's step, and what the step is; the cursor goes on.  V of that step is requested later.
+    int v_from = 0;
+    uint32_t v_mask = 0;
+    const char* v_base = vb;
+    __half2 scales_now = __float2half2_rn(0.f), scales_next = scales_now;  // of the next step, and of the one behind it
+    auto request_k = [&](uint32_t dst, int meta) {
+      scales_now = scales_next;
       if (left > 0) {
         const bool ok = s < end && (uint32_t)slot < n_slots;
-        if (s < end && !ok) atomicMax(&g_status, kOutsideStorage);
         const uint32_t mask = __ballot_sync(0xffffffffu, ok);
-        const int from = ok ? slot : 0;
-        const uint32_t dst = my_ring + stage * C::STAGE_BYTES;
-        auto copy = [&](auto all) {
-#pragma unroll
-          for (int i = 0; i < TOK * C::PIECES / 32; ++i) {
-            const int piece = lane + 32 * i, row = piece / C::PIECES, col = kColumns ? 0 : (piece - row * C::PIECES) * 16;
-            const uint32_t to = dst + row * C::PITCH + (piece - row * C::PIECES) * 16;
-            const int t = __shfl_sync(0xffffffffu, from, row);
-            const bool on = decltype(all)::value || ((mask >> row) & 1);
-            copy16(to, kb + (int64_t)t * k_row + col, on);
-            copy16(to + TOK * C::PITCH, vb + (int64_t)t * v_row + col, on);
+        if (mask != C::FULL && s < end && !ok) atomicMax(&g_status, kOutsideStorage);
+        if (fresh) {  // the queries of a new run, a line a lane
+          const int in = cit % chunks * hpi, line = lane * 64;
+          if (line < min(hpi, group - in) * D)
+            touch(reinterpret_cast<const T*>(p.q) + (int64_t)cb * p.q_stride_b + (int64_t)(hk * group + in + line / D) * p.q_stride_h + line % D);
+        }
+        v_from = ok ? slot : 0;
+        v_mask = mask;
+        v_base = vb;
+        copy_rows(dst, kb, v_from, k_row, mask);
+        if constexpr (C::I8) {  // two-byte loads, read a step later
+          if (ok) {
+            scales_next.x = reinterpret_cast<const __half*>(p.k_scale)[(int64_t)slot * p.ks_stride_t + (int64_t)hk * p.ks_stride_h];
+            scales_next.y = reinterpret_cast<const __half*>(p.v_scale)[(int64_t)slot * p.vs_stride_t + (int64_t)hk * p.vs_stride_h];
+          } else {
+            scales_next = __float2half2_rn(0.f);
           }
-        };
-        if (mask == C::FULL) copy(std::true_type{});
-        else copy(std::false_type{});
-        if constexpr (C::I8)
-          if (lane < TOK) ring_slot[warp][stage][lane] = ok ? slot : -1;
+        }
         const bool last = ct + 1 == cnt || left == 1;
         if (lane == 0) {
-          ring[warp][stage] = Step{mask, fresh | (last ? 2 : 0)};
-          if (fresh || last || C::I8) ring_run[warp][stage] = Run{seq_first + (int64_t)cit * cnt, cb, cit, hk, cnt};
+          ring[warp][meta] = Step{mask, fresh | (last ? 2 : 0)};
+          if (fresh || last) ring_run[warp][meta] = Run{seq_first + (int64_t)cit * cnt, cb, cit, hk, cnt, tokens};
         }
         fresh = last;
         if (--left > 0) {
-          s += C::TILE;
+          s += tile;
           if (++ct == cnt) {
             ct = 0;
             if (++cit == n_it) {
@@ -374,80 +428,84 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
           }
           slot = s < end ? page[s] : 0;
         }
+      } else {
+        v_mask = 0;
+        v_base = nullptr;
       }
       copies_commit();
     };
-
-    for (int i = 0; i < S - 1; ++i) request(i);
-
-    // int8: the scales of a step are two-byte loads a step ahead of their use, a token a lane
-    __half next_sk, next_sv;
-    auto fetch_scales = [&](int stage) {
-      next_sk = next_sv = __float2half_rn(0.f);
-      const int t = lane < TOK ? ring_slot[warp][stage][lane] : -1;
-      if (t < 0) return;
-      const int64_t head = ring_run[warp][stage].hk;
-      next_sk = reinterpret_cast<const __half*>(p.k_scale)[(int64_t)t * p.ks_stride_t + head * p.ks_stride_h];
-      next_sv = reinterpret_cast<const __half*>(p.v_scale)[(int64_t)t * p.vs_stride_t + head * p.vs_stride_h];
+    auto request_v = [&](uint32_t dst) {
+      if (v_base != nullptr) copy_rows(dst, v_base, v_from, v_row, v_mask);
+      copies_commit();
     };
-    if constexpr (C::I8) {
-      __syncwarp();
-      fetch_scales(0);
-    }
+
+    // Four slots: K and V of the present step and of the next one; those of the one behind it take the place of the
+    // present ones as soon as the scores and the sums are there.
+    request_k(my_ring, 0);
+    request_v(my_ring + C::SLOT_BYTES);
+    request_k(my_ring + 2 * C::SLOT_BYTES, 1);
+    request_v(my_ring + 3 * C::SLOT_BYTES);
 
     const float c = (p.sm_scale != 0.f ? p.sm_scale : rsqrtf((float)D)) * kLog2e;
     uint32_t q[NT][D / 16][2];
     float cq[NT][2], m[NT][2], l[NT][2], acc[D / 16][NT][4];
     const int steps = (int)(hi - lo);
-    int stage = 0;
     for (int step = 0; step < steps; ++step) {
-      request(stage == 0 ? S - 1 : stage - 1);
       if constexpr (C::I8)
-        if (lane < TOK) {
-          const float sv = __half2float(next_sv);
-          sm_scale[warp][lane] = make_float4(__half2float(next_sk), sv, __log2f(fmaxf(fabsf(sv), 5.9604644775390625e-8f)), 0.f);
-        }
-      copies_wait<S - 1>();
+        if (lane < TOK) sm_scale[warp][lane] = scales_now;
+      const uint32_t slot_k = my_ring + (step & 1) * 2 * C::SLOT_BYTES, slot_v = slot_k + C::SLOT_BYTES;
+      copies_wait<3>();
       __syncwarp();
-      const Step now = ring[warp][stage];
-      if constexpr (C::I8)
-        if (step + 1 < steps) fetch_scales(stage + 1 == S ? 0 : stage + 1);
+      const Step now = ring[warp][step % META];
       if (now.flags & 1) {
-        const Run run = ring_run[warp][stage];
-        const int in = (run.it - run.hk * chunks) * hpi, h0 = run.hk * group + in, heads = min(hpi, group - in);
-        // queries as B operand: lane (head g, dims 2 c4, 2 c4 + 1 and + 8 of every 16; bytes: dims 4 c4 .. 4 c4 + 3)
+        const Run run = ring_run[warp][step % META];
+        const int in = run.it % chunks * hpi, h0 = run.hk * group + in, heads = min(hpi, group - in);
+        // queries as B operand: lane (head g, dims 2 c4, 2 c4 + 1 and + 8 of every 16; bytes: dims 4 c4 .. + 3 and + 16 of
+        // every 32, high bytes in the even entries, low ones in the odd)
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           const bool on = 8 * j + g < heads;
           const T* qr = reinterpret_cast<const T*>(p.q) + (int64_t)run.b * p.q_stride_b + (int64_t)(h0 + (on ? 8 * j + g : 0)) * p.q_stride_h;
           float amax = 0.f;
+          bool finite = true;
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int d = 16 * k + (C::I8 ? 4 * c4 + 2 * e : 2 * c4 + 8 * e);
+              const int d = C::I8 ? 32 * (k / 2) + 2 * (k & 1) + 16 * e + 4 * c4 : 16 * k + 2 * c4 + 8 * e;
               q[j][k][e] = on ? *reinterpret_cast<const uint32_t*>(qr + d) : 0u;
               if constexpr (C::I8) {
                 const float2 f = unpack2<T>(q[j][k][e]);
                 amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+                finite &= fabsf(f.x) < INFINITY && fabsf(f.y) < INFINITY;
               }
             }
           }
-          cq[j][0] = cq[j][1] = c;
           if constexpr (C::I8) {
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            int e = 0;
-            if (amax > 0.f && amax < INFINITY) e = max(-126, ilogbf(amax));
+            finite = (__ballot_sync(0xffffffffu, finite) >> (4 * g) & 15) == 15;
+            // (the exponent of the largest; below 2^-100 all is as good as 0)
+            const int e = amax > 0.f && finite ? max(-100, (__float_as_int(amax) >> 23) - 127) : 0;
+            const float up = power_of_two(14 - e);
 #pragma unroll
-            for (int k = 0; k < D / 16; ++k)
+            for (int k = 0; k < D / 16; k += 2)
 #pragma unroll
               for (int t = 0; t < 2; ++t) {
-                const float2 f = unpack2<T>(q[j][k][t]);
-                q[j][k][t] = pack2<M>(scalbnf(f.x, -e), scalbnf(f.y, -e));
+                const float2 f0 = unpack2<T>(q[j][k][t]), f1 = unpack2<T>(q[j][k + 1][t]);
+                const int v[4] = {__float2int_rn(f0.x * up), __float2int_rn(f0.y * up),
+                                  __float2int_rn(f1.x * up), __float2int_rn(f1.y * up)};
+                uint32_t high = 0, low = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  high |= ((uint32_t)(v[i] >> 8) & 255u) << (8 * i);
+                  low |= ((uint32_t)v[i] & 255u) << (8 * i);
+                }
+                q[j][k][t] = high;
+                q[j][k + 1][t] = low;
               }
             // the factor of head 8 j + g; this lane's columns are heads 2 c4 and 2 c4 + 1
-            const float f = scalbnf(c, e);
+            const float f = finite ? c * power_of_two(e - 14) : NAN;
             cq[j][0] = __shfl_sync(0xffffffffu, f, 8 * c4);
             cq[j][1] = __shfl_sync(0xffffffffu, f, 8 * c4 + 4);
           }
@@ -460,66 +518,92 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
         }
       }
 
-      // ---- scores: rows tokens, columns heads
-      const uint32_t kst = my_ring + stage * C::STAGE_BYTES, vst = kst + TOK * C::PITCH;
+      // ---- scores: rows tokens, columns heads.  Two or more sums at a time: a product waits 22 cycles for the one before.
       float z[C::SUBS][NT][4];
+      const uint32_t k_base = slot_k + C::at(lane & 15, lane >> 4);
+      if constexpr (!C::I8) {
+        constexpr int SUMS = C::SUBS == 1 ? 2 : 1;
+        float part[C::SUBS][NT][SUMS][4];
 #pragma unroll
-      for (int u = 0; u < C::SUBS; ++u) {
+        for (int i = 0; i < C::SUBS * NT * SUMS * 4; ++i) (&part[0][0][0][0])[i] = 0.f;
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) z[u][j][i] = 0.f;
-        const uint32_t base = kst + (16 * u + (lane & 15)) * C::PITCH + (lane >> 4) * 16;
-        if constexpr (!C::I8) {
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
+          for (int u = 0; u < C::SUBS; ++u) {
             uint32_t a[4];
-            ldmatrix4(a, base + k * 32);
+            ldmatrix4(a, C::skip(k_base + u * 16 * C::PITCH, 2 * k));
 #pragma unroll
-            for (int j = 0; j < NT; ++j) mma<M>(z[u][j], a[0], a[1], a[2], a[3], q[j][k][0], q[j][k][1]);
+            for (int j = 0; j < NT; ++j) mma<M>(part[u][j][k % SUMS], a[0], a[1], a[2], a[3], q[j][k][0], q[j][k][1]);
           }
-        } else {
 #pragma unroll
-          for (int k = 0; k < D / 16; k += 2) {
-            uint32_t r[4];
-            ldmatrix4(r, base + k * 16);
+        for (int u = 0; u < C::SUBS; ++u)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t x = r[2 * e] ^ 0x80808080u, y = r[2 * e + 1] ^ 0x80808080u;
-              const uint32_t a0 = bytes_to_f16<0x4140>(x), a2 = bytes_to_f16<0x4342>(x), a1 = bytes_to_f16<0x4140>(y),
-                             a3 = bytes_to_f16<0x4342>(y);
+          for (int j = 0; j < NT; ++j)
 #pragma unroll
-              for (int j = 0; j < NT; ++j) mma<M>(z[u][j], a0, a1, a2, a3, q[j][k + e][0], q[j][k + e][1]);
+            for (int i = 0; i < 4; ++i) z[u][j][i] = SUMS == 1 ? part[u][j][0][i] : part[u][j][0][i] + part[u][j][SUMS - 1][i];
+      } else {
+        int32_t high[C::SUBS][NT][4], low[C::SUBS][NT][4];
+#pragma unroll
+        for (int i = 0; i < C::SUBS * NT * 4; ++i) (&high[0][0][0])[i] = (&low[0][0][0])[i] = 0;
+#pragma unroll
+        for (int k = 0; k < D / 16; k += 2)
+#pragma unroll
+          for (int u = 0; u < C::SUBS; ++u) {
+            uint32_t a[4];
+            ldmatrix4(a, C::skip(k_base + u * 16 * C::PITCH, k));
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              mma_s8_s8(high[u][j], a, q[j][k][0], q[j][k][1]);
+              mma_s8_u8(low[u][j], a, q[j][k + 1][0], q[j][k + 1][1]);
             }
           }
-        }
+#pragma unroll
+        for (int u = 0; u < C::SUBS; ++u)
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) z[u][j][i] = (float)(high[u][j][i] * 256 + low[u][j][i]);  // (below 2^30)
       }
 
+      __syncwarp();
+      request_k(slot_k, (step + 2) % META);
+
       // ---- weights
-      float sv[C::SUBS][2], top[NT][2];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) top[j][0] = m[j][0], top[j][1] = m[j][1];
+      float sv[C::SUBS][2], lsv[C::SUBS][2], top[NT][2];
 #pragma unroll
       for (int u = 0; u < C::SUBS; ++u)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int tok = 16 * u + g + 8 * e;
-          float4 scales;
+          float sk = 1.f;
           if constexpr (C::I8) {
-            scales = sm_scale[warp][tok];
-            sv[u][e] = scales.y;
+            const float2 f = __half22float2(sm_scale[warp][16 * u + g + 8 * e]);
+            sk = f.x;
+            sv[u][e] = f.y;
+            lsv[u][e] = __log2f(fmaxf(fabsf(f.y), 5.9604644775390625e-8f));  // (no less than f16's smallest: a scale of 0 is none)
           }
 #pragma unroll
           for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) z[u][j][2 * e + i] *= C::I8 ? cq[j][i] * scales.x : c;
-          if (now.mask != C::FULL && !((now.mask >> tok) & 1))
+            for (int i = 0; i < 2; ++i) z[u][j][2 * e + i] *= C::I8 ? cq[j][i] * sk : c;
+        }
+      if (now.mask != C::FULL) {
 #pragma unroll
-            for (int j = 0; j < NT; ++j) z[u][j][2 * e] = z[u][j][2 * e + 1] = -INFINITY;
+        for (int u = 0; u < C::SUBS; ++u)
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
+          for (int i = 0; i < 4; ++i)
+            if (!((now.mask >> (16 * u + g + 8 * (i >> 1))) & 1))
 #pragma unroll
-            for (int i = 0; i < 2; ++i) top[j][i] = fmaxf(top[j][i], C::I8 ? z[u][j][2 * e + i] + scales.z : z[u][j][2 * e + i]);
+              for (int j = 0; j < NT; ++j) z[u][j][i] = -INFINITY;
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          top[j][i] = m[j][i];
+#pragma unroll
+          for (int u = 0; u < C::SUBS; ++u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) top[j][i] = fmaxf(top[j][i], C::I8 ? z[u][j][2 * e + i] + lsv[u][e] : z[u][j][2 * e + i]);
         }
       bool moved = false;
 #pragma unroll
@@ -528,7 +612,7 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
         for (int i = 0; i < 2; ++i) {
 #pragma unroll
           for (int o = 4; o <= 16; o <<= 1) top[j][i] = fmaxf(top[j][i], __shfl_xor_sync(0xffffffffu, top[j][i], o));
-          moved |= top[j][i] != m[j][i];
+          moved |= top[j][i] > m[j][i] + C::SLACK;
         }
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -545,6 +629,8 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
             }
           }
       }
+      copies_wait<3>();
+      __syncwarp();
 #pragma unroll
       for (int u = 0; u < C::SUBS; ++u) {
         uint32_t hi_b[NT][2], lo_b[NT][2];
@@ -566,11 +652,11 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
           }
         // ---- values: rows dims, columns heads
         if constexpr (!C::I8) {
-          const uint32_t base = vst + (16 * u + (lane & 7) + 8 * (lane >> 4)) * C::PITCH + ((lane >> 3) & 1) * 16;
+          const uint32_t base = slot_v + C::at(16 * u + (lane & 7) + 8 * (lane >> 4), (lane >> 3) & 1);
 #pragma unroll
           for (int t = 0; t < D / 16; ++t) {
             uint32_t a[4];
-            ldmatrix4_trans(a, base + t * 32);
+            ldmatrix4_trans(a, C::skip(base, 2 * t));
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
               mma<M>(acc[t][j], a[0], a[1], a[2], a[3], hi_b[j][0], hi_b[j][1]);
@@ -579,11 +665,11 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
           }
         } else {
           // a transposed pair of bytes is two dims of one token: row g of the product is dim 2 g, row g + 8 dim 2 g + 1
-          const uint32_t base = vst + (16 * u + (lane & 7) + 8 * ((lane >> 3) & 1)) * C::PITCH + (lane >> 4) * 16;
+          const uint32_t base = slot_v + C::at(16 * u + (lane & 7) + 8 * ((lane >> 3) & 1), lane >> 4);
 #pragma unroll
           for (int t = 0; t < D / 16; t += 2) {
             uint32_t r[4];
-            ldmatrix4_trans(r, base + t * 16);
+            ldmatrix4_trans(r, C::skip(base, t));
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const uint32_t x = r[2 * e] ^ 0x80808080u, y = r[2 * e + 1] ^ 0x80808080u;
@@ -598,72 +684,47 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
           }
         }
       }
+      __syncwarp();
+      request_v(slot_v);
+
       if (now.flags & 2) {
-        // ---- the end of a run: the warps' sums joined (warps 0 and 1 write, 2 and 3 add), then the result or a partial
-        const Run run = ring_run[warp][stage];
-        const int in = (run.it - run.hk * chunks) * hpi, h0 = run.hk * group + in, heads = min(hpi, group - in);
+        // ---- the end of a run: this warp's partial sums, or the result where no other warp has tokens
+        const Run run = ring_run[warp][step % META];
+        const int in = run.it % chunks * hpi, h0 = run.hk * group + in, heads = min(hpi, group - in);
+        const int c0 = share_owner(run.item_first, total, shares), c1 = share_owner(run.item_first + run.tiles - 1, total, shares);
+        const int64_t item = (int64_t)run.b * n_it + run.it;
+        const bool alone = items.hw == kWarps ? c0 == c1 : run.tokens <= TOK;  // no other warp has tokens of these heads
+        // (items and shares only grow: no two runs have the same sum)
+        const int64_t at = ((item + share) * kWarps + warp) * hpi;
+        if (c0 == share && threadIdx.x == 0) part.items[item] = make_int2((int)(item + c0), alone ? 0 : c1 - c0 + 1);
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
 #pragma unroll
             for (int o = 4; o <= 16; o <<= 1) l[j][i] += __shfl_xor_sync(0xffffffffu, l[j][i], o);
-            if (g == 0) sm_ml[warp][8 * j + 2 * c4 + i] = make_float2(m[j][i], l[j][i]);
+            const int h = 8 * j + 2 * c4 + i;
+            if (h >= heads || (alone && part_of_warp > 0)) continue;
+            if (alone) {
+              T* out = reinterpret_cast<T*>(p.out) + (int64_t)run.b * p.out_stride_b + (int64_t)(h0 + h) * p.out_stride_h;
+              const float f = l[j][i] == 0.f ? 0.f : 1.f / l[j][i];
+#pragma unroll
+              for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                  out[16 * t + (C::I8 ? 2 * g + e : g + 8 * e)] = narrow<T>(l[j][i] == 0.f ? 0.f : acc[t][j][2 * e + i] * f);
+              if (g == 0 && p.lse != nullptr)
+                p.lse[(int64_t)run.b * p.n_q_heads + h0 + h] = l[j][i] == 0.f ? -INFINITY : (m[j][i] - C::LIFT + log2f(l[j][i])) * kLn2;
+            } else {
+              float* o = part.o + (at + h) * D;  // (relative to the same maximum as the sum)
+#pragma unroll
+              for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) o[16 * t + (C::I8 ? 2 * g + e : g + 8 * e)] = acc[t][j][2 * e + i];
+              if (g == 0) part.ml[at + h] = make_float2(m[j][i] - C::LIFT, l[j][i]);
+            }
           }
-        __syncthreads();
-#pragma unroll
-        for (int pass = 0; pass < 2; ++pass) {
-          if ((warp >> 1) == pass) {
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const int h = 8 * j + 2 * c4 + i;
-                if (h >= heads) continue;
-                float all = sm_ml[0][h].x;
-#pragma unroll
-                for (int w = 1; w < kWarps; ++w) all = fmaxf(all, sm_ml[w][h].x);
-                const float f = ex2(m[j][i] - all);
-                float* o = sm_o + ((warp & 1) * hpi + h) * C::O_LD;
-#pragma unroll
-                for (int t = 0; t < D / 16; ++t)
-#pragma unroll
-                  for (int e = 0; e < 2; ++e) {
-                    const int d = 16 * t + (C::I8 ? 2 * g + e : g + 8 * e);
-                    const float v = acc[t][j][2 * e + i] * f;
-                    if (pass == 0) o[d] = v;
-                    else o[d] += v;
-                  }
-              }
-          }
-          __syncthreads();
-        }
-        const int c0 = share_owner(run.item_first, total, shares), c1 = share_owner(run.item_first + run.tiles - 1, total, shares);
-        const int64_t item = (int64_t)run.b * n_it + run.it;
-        const int64_t at = (item + blockIdx.x) * hpi;  // (items and CTAs only grow: no two runs have the same sum)
-        if (c0 == (int)blockIdx.x && threadIdx.x == 0) part.items[item] = make_int2((int)(item + c0), c1 - c0 + 1);
-        T* out = reinterpret_cast<T*>(p.out) + (int64_t)run.b * p.out_stride_b + (int64_t)h0 * p.out_stride_h;
-        for (int i = threadIdx.x; i < heads * D; i += kThreads) {
-          const int h = i / D, d = i - h * D;
-          const float o = sm_o[h * C::O_LD + d] + sm_o[(hpi + h) * C::O_LD + d];
-          float all = sm_ml[0][h].x, sum = 0.f;
-#pragma unroll
-          for (int w = 1; w < kWarps; ++w) all = fmaxf(all, sm_ml[w][h].x);
-#pragma unroll
-          for (int w = 0; w < kWarps; ++w) sum += sm_ml[w][h].y * ex2(sm_ml[w][h].x - all);
-          if (c0 == c1) {
-            out[(int64_t)h * p.out_stride_h + d] = narrow<T>(sum == 0.f ? 0.f : o / sum);
-            if (d == 0 && p.lse != nullptr)
-              p.lse[(int64_t)run.b * p.n_q_heads + h0 + h] = sum == 0.f ? -INFINITY : (all - C::LIFT + log2f(sum)) * kLn2;
-          } else {
-            part.o[(at + h) * D + d] = o;  // (relative to the same maximum as the sum)
-            if (d == 0) part.ml[at + h] = make_float2(all - C::LIFT, sum);
-          }
-        }
-        __syncthreads();
       }
-      __syncwarp();  // the stage may be filled again
-      stage = stage + 1 == S ? 0 : stage + 1;
     }
   }
 
@@ -679,32 +740,35 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
   }
 }
 
-// Joins the partial sums of one (sequence, query head): a warp takes every eighth of them, a lane D / 32 dims, four partials'
+// Joins the partial sums of one (sequence, query head): a warp takes every W-th of them, a lane D / 32 dims, four partials'
 // loads in flight; the warps' sums meet in shared memory.  Always the same order.
-constexpr int kMergeWarps = 8;
-template <typename T, int D>
-__global__ void __launch_bounds__(kMergeWarps * 32)
-paged_merge_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Partials part, int group, int hpi, int chunks) {
+template <typename T, int D, int W>
+__global__ void __launch_bounds__(W * 32)
+paged_merge_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Partials part, const Items items) {
   constexpr int E = D / 32;
-  before_this();
+  // (It does not let the next kernel in: that one's CTAs would be set up beside these, unevenly, and its shares are equal.
+  // What is read before the wait has been there before the decode kernel began.)
   const int h = blockIdx.x, b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int req = p.b_req_idx[b];
-  if (p.b_seq_len[b] <= 0 || p.max_len <= 0 || req < 0 || req >= p.n_req) return;
-  const int hk = h / group, in = h - hk * group;
-  const int2 info = part.items[(int64_t)b * p.n_kv_heads * chunks + hk * chunks + in / hpi];
-  if (info.y <= 1) return;
-  const int64_t first = (int64_t)info.x * hpi + in % hpi;
+  const int req = p.b_req_idx[b], len = p.b_seq_len[b];
+  before_this();
+  if (len <= 0 || p.max_len <= 0 || req < 0 || req >= p.n_req) return;
+  const int hk = h / items.group, in = h - hk * items.group, hw = items.hw, splits = kWarps / hw;
+  const int2 info = part.items[((int64_t)b * (p.n_kv_heads / hw) + hk / hw) * items.chunks + in / items.hpi];
+  const int parts = info.y * splits;
+  if (parts == 0) return;
+  // part k is that of CTA k / splits of the item, of its warp for this KV head and the tokens' split k % splits
+  const int64_t first = ((int64_t)info.x * kWarps + hk % hw) * items.hpi + in % items.hpi;
   float m = -FLT_MAX, l = 0.f, o[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int i0 = warp; i0 < info.y; i0 += 4 * kMergeWarps) {
+  for (int i0 = warp; i0 < parts; i0 += 4 * W) {
     float2 ml[4];
     float v[4][E];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int k = i0 + i * kMergeWarps;
-      const bool on = k < info.y;
-      const int64_t at = first + (int64_t)(on ? k : 0) * hpi;
+      const int k = i0 + i * W;
+      const bool on = k < parts;
+      const int64_t at = first + (int64_t)(on ? k * hw : 0) * items.hpi;
       ml[i] = on ? part.ml[at] : make_float2(-FLT_MAX, 0.f);
 #pragma unroll
       for (int e = 0; e < E; ++e) v[i][e] = on ? part.o[at * D + lane + 32 * e] : 0.f;
@@ -725,38 +789,33 @@ paged_merge_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Partia
     }
     m = top;
   }
-  __shared__ float sm_o[kMergeWarps][D];
-  __shared__ float2 sm_ml[kMergeWarps];
+  __shared__ float sm_o[W][D];
+  __shared__ float2 sm_ml[W];
   if (lane == 0) sm_ml[warp] = make_float2(m, l);
 #pragma unroll
   for (int e = 0; e < E; ++e) sm_o[warp][lane + 32 * e] = o[e];
   __syncthreads();
   float top = sm_ml[0].x, sum = 0.f;
 #pragma unroll
-  for (int w = 1; w < kMergeWarps; ++w) top = fmaxf(top, sm_ml[w].x);
-  const int d = threadIdx.x;
-  float r = 0.f;
+  for (int w = 1; w < W; ++w) top = fmaxf(top, sm_ml[w].x);
 #pragma unroll
-  for (int w = 0; w < kMergeWarps; ++w) {
-    const float f = ex2(sm_ml[w].x - top);
-    sum = fmaf(sm_ml[w].y, f, sum);
-    if (d < D) r = fmaf(sm_o[w][d], f, r);
-  }
-  if (d < D)
+  for (int w = 0; w < W; ++w) sum = fmaf(sm_ml[w].y, ex2(sm_ml[w].x - top), sum);
+  for (int d = threadIdx.x; d < D; d += W * 32) {
+    float r = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) r = fmaf(sm_o[w][d], ex2(sm_ml[w].x - top), r);
     reinterpret_cast<T*>(p.out)[(int64_t)b * p.out_stride_b + (int64_t)h * p.out_stride_h + d] = narrow<T>(sum == 0.f ? 0.f : r / sum);
-  if (d == 0 && p.lse != nullptr) p.lse[(int64_t)b * p.n_q_heads + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
+  }
+  if (threadIdx.x == 0 && p.lse != nullptr) p.lse[(int64_t)b * p.n_q_heads + h] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
 }
 
 // ---- host side
 
-// How the query heads of a KV head are cut into items: all of them, or chunks of 16.
-struct Items {
-  int group, hpi, chunks, nt;
-};
 Items items_of(const WsvdPagedDecodeParams& p) {
   const int group = p.n_q_heads / p.n_kv_heads;
   const int chunks = (group + 15) / 16, hpi = (group + chunks - 1) / chunks;
-  return {group, hpi, chunks, hpi <= 8 ? 1 : 2};
+  const int hw = p.n_kv_heads % 4 == 0 ? 4 : p.n_kv_heads % 2 == 0 ? 2 : 1;
+  return {group, hpi, chunks, hpi <= 8 ? 1 : 2, hw};
 }
 size_t pad256(size_t b) { return (b + 255) & ~(size_t)255; }
 struct Room {
@@ -764,7 +823,8 @@ struct Room {
 };
 Room room_of(const WsvdPagedDecodeParams& p) {
   const Items it = items_of(p);
-  const size_t items = (size_t)p.batch * p.n_kv_heads * it.chunks, rows = (items + kMaxShares) * it.hpi;
+  const size_t items = (size_t)p.batch * (p.n_kv_heads / it.hw) * it.chunks, ctas = (size_t)kMaxSms * kMaxCtas;
+  const size_t rows = (items + (items * kMaxParts < ctas ? items * kMaxParts : ctas)) * kWarps * it.hpi;
   Room r;
   r.o = 0;
   r.ml = r.o + pad256(rows * p.head_dim * sizeof(float));
@@ -784,43 +844,38 @@ bool fits_tensor_cores(const WsvdPagedDecodeParams& p) {
   return (reinterpret_cast<uintptr_t>(p.q) & 3) == 0 && p.q_stride_b % 2 == 0 && p.q_stride_h % 2 == 0;
 }
 
-int sm_count(int device) {
-  static int counts[64];
-  if (device < 0 || device >= 64) return 148;
-  if (counts[device] == 0) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) n = 148;
-    counts[device] = n;
-  }
-  return counts[device];
-}
-
 template <typename C>
 cudaError_t launch_fast(const WsvdPagedDecodeParams& p, const Items& it, const Partials& part, cudaStream_t s) {
-  constexpr size_t kRing = (size_t)kWarps * C::STAGES * C::STAGE_BYTES;
-  const size_t smem = kRing + 2 * (size_t)it.hpi * C::O_LD * sizeof(float);
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return e;
-  static bool ready[64];
-  if (device >= 64 || !ready[device]) {
-    e = cudaFuncSetAttribute(paged_decode_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)(kRing + 2 * C::HEADS * C::O_LD * sizeof(float)));
+  if (device < 0 || device >= kMaxDevices) return cudaErrorInvalidDevice;
+  // how many CTAs the GPU holds at once, asked once per device (what is written twice is the same)
+  static int resident[kMaxDevices];
+  if (resident[device] == 0) {
+    e = cudaFuncSetAttribute(paged_decode_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::RING);
+    int per_sm = 0, sms = 0;
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, paged_decode_kernel<C>, kThreads, C::RING);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e != cudaSuccess) return e;
-    if (device < 64) ready[device] = true;
+    resident[device] = max(1, min(kMaxSms, sms) * min(per_sm, C::CTAS));
   }
-  // CTAs per SM: what shared memory holds (1 KB of it is the system's, about 1.5 KB the kernel's own variables)
-  const int fit = (int)((228 * 1024) / (smem + 2560)), per_sm = fit < 1 ? 1 : fit > 3 ? 3 : fit;
+  // a share a CTA, but no more than a merge of one item can take at a time
+  const int64_t items = (int64_t)p.batch * (p.n_kv_heads / it.hw) * it.chunks;
+  const int tile = C::TOK * kWarps / it.hw;
   const int reach = p.window > 0 && p.window < p.max_len ? p.window : p.max_len;
-  const int64_t most = (int64_t)p.batch * p.n_kv_heads * it.chunks * ((reach + C::TILE - 1) / C::TILE);
-  int64_t grid = (int64_t)sm_count(device) * per_sm;
-  if (grid > kMaxShares) grid = kMaxShares;
-  if (grid > most) grid = most;
+  int64_t grid = resident[device];
+  if (grid > items * kMaxParts) grid = items * kMaxParts;
+  const int64_t tiles = items * ((reach + tile - 1) / tile);
+  if (grid > tiles) grid = tiles;
   if (grid < 1) grid = 1;
-  e = launch_overlapped(paged_decode_kernel<C>, dim3((unsigned)grid), kThreads, smem, s, p, part, it.group, it.hpi, it.chunks);
-  if (e != cudaSuccess || grid == 1 || reach <= C::TILE) return e;  // (one tile an item: no partials)
-  return launch_overlapped(paged_merge_kernel<typename C::T, C::D>, dim3(p.n_q_heads, p.batch), kMergeWarps * 32, 0, s, p, part, it.group,
-                it.hpi, it.chunks);
+  e = launch_overlapped(paged_decode_kernel<C>, dim3((unsigned)grid), kThreads, (size_t)C::RING, s, p, part, it);
+  if (e != cudaSuccess || reach <= C::TOK) return e;  // (one warp an item and head: no partials)
+  // (an item has about grid / items + 1 CTAs: one round of loads for four warps, else many warps)
+  const dim3 heads(p.n_q_heads, p.batch);
+  if (grid * (kWarps / it.hw) <= 14 * items)
+    return launch_overlapped(paged_merge_kernel<typename C::T, C::D, 4>, heads, 4 * 32, 0, s, p, part, it);
+  return launch_overlapped(paged_merge_kernel<typename C::T, C::D, 16>, heads, 16 * 32, 0, s, p, part, it);
 }
 
 template <typename T, bool I8, int NT>
