@@ -3,6 +3,8 @@
 //   out[n] = y[n] + scale[i] (x[n] A_i) B_i,   i = adapter[request of row n]
 //
 // Two kernels: h = x A in f32 (shrink) and out = y + scale h B (expand).
+#include <cooperative_groups.h>
+
 #include <type_traits>
 
 #include "dense_ops.cuh"
@@ -275,64 +277,82 @@ expand_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* 
 
 // ---- packed rows (prompts): products on the tensor cores, tiles of 64 rows of one request
 //
-// Bound by x, y and out.  Shrink: a warp has 16 rows and all ranks, tiles of 64 inputs come by 16-byte asynchronous copies,
-// the input's length is cut into slices so that every SM has blocks (their sums are left in f32 and added by the
-// expanding blocks in a fixed order).  Expand: a block keeps its rows' h, rounded once to the 16-bit type (a step of it is
-// 2^-9 of the adapter's share of the result, which is rounded to that type itself), and walks over 128 columns at a
-// time: B's tile from L2 and y's from memory a step ahead, y + product in place in shared memory, 16-byte stores.
+// Bound by x, y and out.  Shrink: a warp has 16 rows and all ranks, tiles of 64 inputs come by 16-byte asynchronous copies;
+// the input's length is cut into slices over the CTAs of a cluster, so that every SM has work, and their sums meet in
+// shared memory in a fixed order.  h is rounded once to the 16-bit type (a step of it is 2^-9 of the adapter's share of the
+// result, which is rounded to that type itself).  Expand: equal shares of (tile, 128 columns) over the CTAs that the GPU
+// holds at once; a CTA keeps its tile's h, B's columns come from L2 and y's from memory a step ahead, y + product in place
+// in shared memory, 16-byte stores.
 constexpr int kTileRows = 64, kTileK = 64, kTileCols = 128, kPackThreads = 128;
 
-// Tile number t of the batch: rows [row, row + rows) of one request and its adapter (-1: none).  Tiles are numbered through
-// the requests in order; what is behind the last one counts as one more request without an adapter where it is copied.
+// The row tiles of the batch, numbered through the requests in order; what is behind the last one counts as one more request
+// without an adapter where it is copied.  Every thread knows the tiles [before, before + mine) of its requests.
 struct RowTile {
-  int row, rows, adapter;  // rows 0: there is no such tile
+  int row, rows, adapter;  // rows 0: there is no such tile; adapter -1: none
 };
-__device__ __forceinline__ void tile_of(const WsvdAdapterAddParams& p, int t, RowTile* sm) {
-  __shared__ int sums[kPackThreads / 32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int segments = p.batch + (p.copy_tail ? 1 : 0);
-  const int per = (segments + kPackThreads - 1) / kPackThreads, b0 = min(segments, (int)threadIdx.x * per), b1 = min(segments, b0 + per);
-  auto ends = [&](int b, int* from) {  // rows [*from, result) of segment b, inside [0, rows) whatever cu_new says
+struct RowTiles {
+  const WsvdAdapterAddParams& p;
+  int b0, b1, before, mine, total;
+
+  // rows [*from, result) of request b, inside [0, rows) whatever cu_new says
+  __device__ __forceinline__ int span(int b, int* from) const {
     *from = min(max(p.cu_new[b], 0), p.rows);
     return b < p.batch ? max(*from, min(p.cu_new[b + 1], p.rows)) : p.rows;
-  };
-  if (threadIdx.x == 0) *sm = RowTile{0, 0, -1};
-  int mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    int from;
-    const int to = ends(b, &from);
-    mine += (to - from + kTileRows - 1) / kTileRows;
   }
-  int incl = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += v;
-  }
-  if (lane == 31) sums[warp] = incl;
-  __syncthreads();
-  int before = incl - mine;
-  for (int w = 0; w < warp; ++w) before += sums[w];
-  if (t >= before && t < before + mine) {
-    int b = b0;
-    for (;; ++b) {
+  __device__ __forceinline__ RowTiles(const WsvdAdapterAddParams& params) : p(params) {
+    __shared__ int sums[kPackThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int requests = p.batch + (p.copy_tail ? 1 : 0), per = (requests + kPackThreads - 1) / kPackThreads;
+    b0 = min(requests, (int)threadIdx.x * per);
+    b1 = min(requests, b0 + per);
+    mine = 0;
+    for (int b = b0; b < b1; ++b) {
       int from;
-      const int to = ends(b, &from), n = (to - from + kTileRows - 1) / kTileRows;
-      if (t < before + n) {
-        const int row = from + (t - before) * kTileRows;
-        int i = b < p.batch ? p.adapter[b] : -1;
-        if (i < -1 || i >= p.n_adapters) {
-          atomicMax(&g_status, kOutsideStorage);
-          i = -1;
-        }
-        *sm = RowTile{row, min(kTileRows, to - row), i};
-        break;
-      }
-      before += n;
+      const int to = span(b, &from);
+      mine += (to - from + kTileRows - 1) / kTileRows;
+    }
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    if (lane == 31) sums[warp] = incl;
+    __syncthreads();
+    before = incl - mine;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kPackThreads / 32; ++w) {
+      if (w < warp) before += sums[w];
+      total += sums[w];
     }
   }
-  __syncthreads();
-}
+  // tile number t, for all threads (between two block barriers)
+  __device__ __forceinline__ RowTile find(int t) const {
+    __shared__ RowTile tile;
+    __syncthreads();
+    if (t >= before && t < before + mine) {
+      int first = before;
+      for (int b = b0; b < b1; ++b) {
+        int from;
+        const int to = span(b, &from), n = (to - from + kTileRows - 1) / kTileRows;
+        if (t < first + n) {
+          const int row = from + (t - first) * kTileRows;
+          int i = b < p.batch ? p.adapter[b] : -1;
+          if (i < -1 || i >= p.n_adapters) {
+            atomicMax(&g_status, kOutsideStorage);
+            i = -1;
+          }
+          tile = RowTile{row, min(kTileRows, to - row), i};
+          break;
+        }
+        first += n;
+      }
+    }
+    __syncthreads();
+    return tile;
+  }
+};
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {  // zeros where it is not on
@@ -371,18 +391,20 @@ struct Shrink {
   static constexpr int STAGE = kTileRows * X_PITCH + kTileK * A_PITCH;
   static constexpr int STAGES = RP <= 128 ? 3 : 2;
 };
+// h [rows][rp]: rp is the rank rounded up to 16
 template <typename T, int RP>
 __global__ void __launch_bounds__(kPackThreads)
-shrink_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, float* h, const int slice) {
+shrink_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, T* h, const int slice, const int rp) {
   using S = Shrink<RP>;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ RowTile tile;
   before_this();
   let_next_in();
-  tile_of(p, blockIdx.x, &tile);
-  if (tile.rows == 0 || tile.adapter < 0) return;
+  const RowTiles tiles(p);
+  if ((int)blockIdx.x >= tiles.total) return;  // (the CTAs of a cluster have one tile)
+  const RowTile tile = tiles.find(blockIdx.x);
+  if (tile.adapter < 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int k0 = blockIdx.y * slice, k1 = min(p.n_in, k0 + slice), steps = (k1 - k0 + kTileK - 1) / kTileK;
+  const int k0 = min(p.n_in, (int)blockIdx.y * slice), k1 = min(p.n_in, k0 + slice), steps = (k1 - k0 + kTileK - 1) / kTileK;
   const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)tile.row * p.x_stride;
   const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)tile.adapter * p.a_stride_i;
   const uint32_t ring = smem_addr(smem);
@@ -442,128 +464,148 @@ shrink_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, float* h, c
       }
     }
   }
+  // the slices' sums: each CTA leaves its own in its shared memory, and adds up its part of the rows from all of them
+  copies_wait<0>();
+  __syncthreads();
+  constexpr int LD = RP + 4;  // (four more words a row: no bank twice)
+  float* sums = reinterpret_cast<float*>(smem);
   const int g = lane >> 2, c4 = lane & 3;
 #pragma unroll
-  for (int j = 0; j < RP / 8; ++j) {
-    const int r = 8 * j + 2 * c4;
-    if (r >= p.rank) continue;  // (rank is a multiple of 4: both of the pair or none)
+  for (int j = 0; j < RP / 8; ++j)
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int row = warp * 16 + g + 8 * e;
-      if (row < tile.rows)
-        *reinterpret_cast<float2*>(h + ((int64_t)blockIdx.y * p.rows + tile.row + row) * p.rank + r) = make_float2(acc[j][2 * e], acc[j][2 * e + 1]);
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<float2*>(sums + (warp * 16 + g + 8 * e) * LD + 8 * j + 2 * c4) = make_float2(acc[j][2 * e], acc[j][2 * e + 1]);
+  const auto cluster = cooperative_groups::this_cluster();
+  cluster.sync();
+  const int slices = cluster.num_blocks(), part = kTileRows / slices, from = (int)cluster.block_rank() * part;
+  for (int i = threadIdx.x; i < part * (rp / 2); i += kPackThreads) {
+    const int row = from + i / (rp / 2), r = (i % (rp / 2)) * 2;
+    if (row >= tile.rows) continue;
+    float2 v = make_float2(0.f, 0.f);
+    for (int c = 0; c < slices; ++c) {
+      const float2 w = *reinterpret_cast<const float2*>(cluster.map_shared_rank(sums, c) + row * LD + r);
+      v.x += w.x;
+      v.y += w.y;
     }
+    *reinterpret_cast<uint32_t*>(h + (int64_t)(tile.row + row) * rp + r) = both<T>(v.x, v.y);  // (ranks up to rp: zeros)
   }
+  cluster.sync();  // (nobody's shared memory goes while another reads it)
 }
 
 constexpr int kColPitch = kTileCols * 2 + 16;  // bytes of a tile row of B or y
-// columns [blockIdx.y * span, + span) of a tile of rows; rp: the rank rounded up to 16
 template <typename T>
 __global__ void __launch_bounds__(kPackThreads)
-expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* h, const int slices, const int rp, const int span) {
+expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const T* h, const int rp) {
   extern __shared__ __align__(16) unsigned char smem[];  // h [64][rp], then two stages of B [rp][128] and y [64][128]
-  __shared__ RowTile tile;
+  // (What is read before the wait is nothing that the shrinking kernel writes: see expand_step_kernel.)
   if (p.n_adapters == 0) before_this();
-  tile_of(p, blockIdx.x, &tile);  // (before the wait: see expand_step_kernel)
-  if (tile.rows == 0) {
-    before_this();
-    return;
-  }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c0 = blockIdx.y * span, c1 = min(p.n_out, c0 + span), steps = (c1 - c0 + kTileCols - 1) / kTileCols;
-  const T* y = reinterpret_cast<const T*>(p.y) + (int64_t)tile.row * p.y_stride;
-  T* out = reinterpret_cast<T*>(p.out) + (int64_t)tile.row * p.out_stride;
-  if (tile.adapter < 0) {
-    before_this();
-    if (p.out == p.y) return;
-    const int vecs = (c1 - c0) / 8;
-    for (int i = threadIdx.x; i < tile.rows * vecs; i += kPackThreads) {
-      const int row = i / vecs, col = c0 + (i - row * vecs) * 8;
-      *reinterpret_cast<uint4*>(out + (int64_t)row * p.out_stride + col) = *reinterpret_cast<const uint4*>(y + (int64_t)row * p.y_stride + col);
-    }
-    return;
-  }
-  const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)tile.adapter * p.b_stride_i;
+  const RowTiles tiles(p);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c4 = lane & 3;
+  const int blocks = (p.n_out + kTileCols - 1) / kTileCols;
+  const int64_t units = (int64_t)tiles.total * blocks;
+  const int shares = (int)min((int64_t)gridDim.x, units);
+  int64_t unit = (int)blockIdx.x < shares ? share_begin(blockIdx.x, units, shares) : 0;
+  const int64_t end = (int)blockIdx.x < shares ? share_begin(blockIdx.x + 1, units, shares) : 0;
   const int h_pitch = rp * 2 + 16, b_bytes = rp * kColPitch, stage_bytes = b_bytes + kTileRows * kColPitch;
   const uint32_t hd = smem_addr(smem), ring = hd + kTileRows * h_pitch;
-  auto request = [&](int step) {
-    if (step < steps) {
-      const int c = c0 + step * kTileCols;
-      const uint32_t bd = ring + (step & 1) * stage_bytes, yd = bd + b_bytes;
-      const int col = (threadIdx.x & 15) * 8;
-      const bool in = c + col < c1;
-      for (int row = threadIdx.x >> 4; row < rp; row += kPackThreads / 16) {
-        const bool on = in && row < p.rank;
-        copy16(bd + row * kColPitch + col * 2, b + (on ? (int64_t)row * p.b_stride_r + c + col : 0), on);
+  bool waited = p.n_adapters == 0;
+  auto wait_once = [&]() {
+    if (!waited) before_this();
+    waited = true;
+  };
+  while (unit < end) {
+    // the share's columns of one tile of rows
+    const int t = (int)(unit / blocks);
+    const int c0 = (int)(unit - (int64_t)t * blocks) * kTileCols;
+    const int steps = (int)min(end - unit, (int64_t)blocks - c0 / kTileCols), c1 = min(p.n_out, c0 + steps * kTileCols);
+    unit += steps;
+    const RowTile tile = tiles.find(t);
+    const T* y = reinterpret_cast<const T*>(p.y) + (int64_t)tile.row * p.y_stride;
+    T* out = reinterpret_cast<T*>(p.out) + (int64_t)tile.row * p.out_stride;
+    if (tile.adapter < 0) {
+      wait_once();
+      if (p.out == p.y) continue;
+      const int vecs = (c1 - c0) / 8;
+      for (int i = threadIdx.x; i < tile.rows * vecs; i += kPackThreads) {
+        const int row = i / vecs, col = c0 + (i - row * vecs) * 8;
+        *reinterpret_cast<uint4*>(out + (int64_t)row * p.out_stride + col) =
+            *reinterpret_cast<const uint4*>(y + (int64_t)row * p.y_stride + col);
       }
+      continue;
+    }
+    const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)tile.adapter * p.b_stride_i;
+    const int col = (threadIdx.x & 15) * 8;
+    auto request = [&](int step) {
+      if (step < steps) {
+        const int c = c0 + step * kTileCols;
+        const uint32_t bd = ring + (step & 1) * stage_bytes, yd = bd + b_bytes;
+        const bool in = c + col < c1;
+        for (int row = threadIdx.x >> 4; row < rp; row += kPackThreads / 16) {
+          const bool on = in && row < p.rank;
+          copy16(bd + row * kColPitch + col * 2, b + (on ? (int64_t)row * p.b_stride_r + c + col : 0), on);
+        }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {  // the warp's own 16 rows
-        const int row = warp * 16 + 2 * i + (lane >> 4);
-        const bool on = in && row < tile.rows;
-        copy16(yd + row * kColPitch + col * 2, y + (on ? (int64_t)row * p.y_stride + c + col : 0), on);
+        for (int i = 0; i < 8; ++i) {  // the warp's own 16 rows
+          const int row = warp * 16 + 2 * i + (lane >> 4);
+          const bool on = in && row < tile.rows;
+          copy16(yd + row * kColPitch + col * 2, y + (on ? (int64_t)row * p.y_stride + c + col : 0), on);
+        }
       }
+      copies_commit();
+    };
+    request(0);
+    wait_once();
+    const float scale = p.scale != nullptr ? p.scale[tile.adapter] : 1.f;
+    for (int i = threadIdx.x; i < kTileRows * (rp / 8); i += kPackThreads) {
+      const int row = i / (rp / 8), r = (i % (rp / 8)) * 8;
+      const bool on = row < tile.rows;
+      copy16(hd + row * h_pitch + r * 2, h + (on ? (int64_t)(tile.row + row) * rp + r : 0), on);
     }
     copies_commit();
-  };
-  request(0);
-  before_this();
-  const float scale = p.scale != nullptr ? p.scale[tile.adapter] : 1.f;
-  for (int i = threadIdx.x; i < kTileRows * (rp / 2); i += kPackThreads) {
-    const int row = i / (rp / 2), r = (i - row * (rp / 2)) * 2;
-    float2 s = make_float2(0.f, 0.f);
-    if (row < tile.rows && r < p.rank) {
-      const float* at = h + (int64_t)(tile.row + row) * p.rank + r;
-#pragma unroll 4
-      for (int l = 0; l < slices; ++l) {
-        const float2 v = *reinterpret_cast<const float2*>(at + (int64_t)l * p.rows * p.rank);
-        s.x += v.x;
-        s.y += v.y;
+    for (int step = 0; step < steps; ++step) {
+      request(step + 1);
+      copies_wait<1>();
+      __syncthreads();
+      const uint32_t bd = ring + (step & 1) * stage_bytes;
+      unsigned char* yt = smem + kTileRows * h_pitch + (step & 1) * stage_bytes + b_bytes;
+      float acc[kTileCols / 8][4];
+#pragma unroll
+      for (int j = 0; j < kTileCols / 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+      for (int k = 0; k < rp / 16; ++k) {
+        uint32_t hr[4];
+        ldmatrix4(hr, hd + (warp * 16 + (lane & 15)) * h_pitch + (lane >> 4) * 16 + k * 32);
+        const uint32_t ba = bd + (16 * k + (lane & 15)) * kColPitch + (lane >> 4) * 16;
+#pragma unroll
+        for (int j = 0; j < kTileCols / 16; ++j) {
+          uint32_t w[4];
+          ldmatrix4_trans(w, ba + j * 32);
+          mma<T>(acc[2 * j], hr, w[0], w[1]);
+          mma<T>(acc[2 * j + 1], hr, w[2], w[3]);
+        }
       }
+#pragma unroll
+      for (int j = 0; j < kTileCols / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          uint32_t* at = reinterpret_cast<uint32_t*>(yt + (warp * 16 + g + 8 * e) * kColPitch + (8 * j + 2 * c4) * 2);
+          const float2 v = two<T>(*at);
+          *at = both<T>(fmaf(scale, acc[j][2 * e], v.x), fmaf(scale, acc[j][2 * e + 1], v.y));
+        }
+      __syncwarp();  // the warp's rows are its own
+      const int c = c0 + step * kTileCols + col;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = warp * 16 + 2 * i + (lane >> 4);
+        if (c < c1 && row < tile.rows)
+          *reinterpret_cast<uint4*>(out + (int64_t)row * p.out_stride + c) = *reinterpret_cast<const uint4*>(yt + row * kColPitch + col * 2);
+      }
+      __syncthreads();  // the stage may be filled again
     }
-    *reinterpret_cast<uint32_t*>(smem + row * h_pitch + r * 2) = both<T>(s.x, s.y);
+    copies_wait<0>();
   }
-  const int g = lane >> 2, c4 = lane & 3;
-  for (int step = 0; step < steps; ++step) {
-    request(step + 1);
-    copies_wait<1>();
-    __syncthreads();
-    const uint32_t bd = ring + (step & 1) * stage_bytes;
-    unsigned char* yt = smem + kTileRows * h_pitch + (step & 1) * stage_bytes + b_bytes;
-    float acc[kTileCols / 8][4];
-#pragma unroll
-    for (int j = 0; j < kTileCols / 8; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
-    for (int k = 0; k < rp / 16; ++k) {
-      uint32_t hr[4];
-      ldmatrix4(hr, hd + (warp * 16 + (lane & 15)) * h_pitch + (lane >> 4) * 16 + k * 32);
-      const uint32_t ba = bd + (16 * k + (lane & 15)) * kColPitch + (lane >> 4) * 16;
-#pragma unroll
-      for (int j = 0; j < kTileCols / 16; ++j) {
-        uint32_t w[4];
-        ldmatrix4_trans(w, ba + j * 32);
-        mma<T>(acc[2 * j], hr, w[0], w[1]);
-        mma<T>(acc[2 * j + 1], hr, w[2], w[3]);
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < kTileCols / 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        uint32_t* at = reinterpret_cast<uint32_t*>(yt + (warp * 16 + g + 8 * e) * kColPitch + (8 * j + 2 * c4) * 2);
-        const float2 v = two<T>(*at);
-        *at = both<T>(fmaf(scale, acc[j][2 * e], v.x), fmaf(scale, acc[j][2 * e + 1], v.y));
-      }
-    __syncwarp();  // the warp's rows are its own
-    const int col = (lane & 15) * 8, c = c0 + step * kTileCols + col;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int row = warp * 16 + 2 * i + (lane >> 4);
-      if (c < c1 && row < tile.rows)
-        *reinterpret_cast<uint4*>(out + (int64_t)row * p.out_stride + c) = *reinterpret_cast<const uint4*>(yt + row * kColPitch + col * 2);
-    }
-    __syncthreads();  // the stage may be filled again
-  }
+  wait_once();  // (no block ends before the shrinking kernel has)
 }
 
 // ---- host side
@@ -583,16 +625,16 @@ int rank_padded(int rank) {
   return r;
 }
 int packed_tiles(const WsvdAdapterAddParams& p) { return p.rows / kTileRows + p.batch + 1; }
-// Inputs of a slice: enough blocks for every SM to have several, slices of no less than 64 inputs.
+int rank_16(const WsvdAdapterAddParams& p) { return (p.rank + 15) / 16 * 16; }
+// Steps: inputs of a slice, enough blocks for every SM to have several, slices of 64 to kMaxSlice inputs (of four rows in f32:
+// what fits shared memory).
 int slice_of(const WsvdAdapterAddParams& p) {
-  const int64_t blocks = p.cu_new != nullptr ? p.rows / kTileRows + 1 : p.rows, want = p.cu_new != nullptr ? 148 * 3 : 148 * 8;
-  int64_t slices = (want + blocks - 1) / blocks;
-  const int64_t most = (p.n_in + 63) / 64;
-  const int64_t least = p.cu_new != nullptr ? 1 : (p.n_in + kMaxSlice - 1) / kMaxSlice;  // (a slice of four rows fits shared memory)
+  const int64_t blocks = p.rows > 0 ? p.rows : 1;
+  int64_t slices = (148 * 8 + blocks - 1) / blocks;
+  const int64_t least = (p.n_in + kMaxSlice - 1) / kMaxSlice, most = (p.n_in + 63) / 64;
   if (slices < least) slices = least;
   if (slices > most) slices = most;
   if (slices > kMaxSlices) slices = kMaxSlices;
-  if (slices < 1) slices = 1;
   return (int)(((p.n_in + slices - 1) / slices + 63) / 64 * 64);
 }
 int slices_of(const WsvdAdapterAddParams& p) { return (p.n_in + slice_of(p) - 1) / slice_of(p); }
@@ -604,34 +646,40 @@ cudaError_t launch_step(const WsvdAdapterAddParams& p, float* h, cudaStream_t s)
   const size_t xs = (size_t)slice * kStepRows, red = (size_t)lanes * kStepRows * p.rank;
   cudaError_t e = p.n_adapters == 0 ? cudaSuccess
                                     : launch_overlapped(shrink_step_kernel<T>, dim3(p.rows, slices), kStepThreads, (xs > red ? xs : red) * sizeof(float),
-                                                        s, p, h, slice);
+                                                        s, 1, p, h, slice);
   if (e != cudaSuccess) return e;
   return launch_overlapped(expand_step_kernel<T>, dim3(p.rows, (p.n_out + kStepCols - 1) / kStepCols), kStepThreads,
-                           (size_t)kStepRows * p.rank * sizeof(float), s, p, (const float*)h, slices);
+                           (size_t)kStepRows * p.rank * sizeof(float), s, 1, p, (const float*)h, slices);
 }
 
 // more than 48 KB of dynamic shared memory has to be asked for, once per kernel and device
 template <typename K>
-cudaError_t allow_smem(K kernel, bool (&ready)[64], size_t bytes) {
+cudaError_t allow_smem(K kernel, bool (&ready)[kMaxDevices], size_t bytes) {
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
-  if (e != cudaSuccess || (device < 64 && ready[device])) return e;
+  if (e == cudaSuccess && (device < 0 || device >= kMaxDevices)) e = cudaErrorInvalidDevice;
+  if (e != cudaSuccess || ready[device]) return e;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (e == cudaSuccess && device < 64) ready[device] = true;
+  if (e == cudaSuccess) ready[device] = true;
   return e;
 }
 
 template <typename T, int RP>
-cudaError_t launch_shrink(const WsvdAdapterAddParams& p, float* h, cudaStream_t s) {
-  static bool ready[64];
-  constexpr size_t smem = (size_t)Shrink<RP>::STAGES * Shrink<RP>::STAGE;
+cudaError_t launch_shrink(const WsvdAdapterAddParams& p, T* h, cudaStream_t s) {
+  static bool ready[kMaxDevices];
+  constexpr size_t ring = (size_t)Shrink<RP>::STAGES * Shrink<RP>::STAGE, sums = (size_t)kTileRows * (RP + 4) * sizeof(float);
+  constexpr size_t smem = ring > sums ? ring : sums;
   const cudaError_t e = allow_smem(shrink_packed_kernel<T, RP>, ready, smem);
   if (e != cudaSuccess) return e;
-  return launch_overlapped(shrink_packed_kernel<T, RP>, dim3(packed_tiles(p), slices_of(p)), kPackThreads, smem, s, p, h, slice_of(p));
+  // slices: enough CTAs for every SM to have three, none shorter than 256 inputs
+  int slices = 1;
+  while (slices < 8 && (int64_t)(p.rows / kTileRows + 1) * slices < 148 * 3 && p.n_in / (2 * slices) >= 256) slices *= 2;
+  const int slice = ((p.n_in + slices - 1) / slices + kTileK - 1) / kTileK * kTileK;
+  return launch_overlapped(shrink_packed_kernel<T, RP>, dim3(packed_tiles(p), slices), kPackThreads, smem, s, slices, p, h, slice, rank_16(p));
 }
 
 template <typename T>
-cudaError_t launch_packed(const WsvdAdapterAddParams& p, float* h, cudaStream_t s) {
+cudaError_t launch_packed(const WsvdAdapterAddParams& p, T* h, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
   if (p.n_adapters > 0) {
     switch (rank_padded(p.rank)) {
@@ -643,23 +691,32 @@ cudaError_t launch_packed(const WsvdAdapterAddParams& p, float* h, cudaStream_t 
     }
     if (e != cudaSuccess) return e;
   }
-  static bool ready[64];
-  const int rp = (p.rank + 15) / 16 * 16;
+  static bool ready[kMaxDevices];
+  const int rp = rank_16(p);
   auto bytes = [](int r) { return (size_t)kTileRows * (r * 2 + 16) + 2 * ((size_t)r * kColPitch + kTileRows * kColPitch); };
   e = allow_smem(expand_packed_kernel<T>, ready, bytes(256));
   if (e != cudaSuccess) return e;
-  // column spans: as many blocks as one wave holds (three per SM), each with as many columns as that leaves
-  const int64_t tiles = p.rows / kTileRows + 1, cols = (p.n_out + kTileCols - 1) / kTileCols;
-  int64_t spans = (148 * 3 + tiles - 1) / tiles;
-  if (spans > cols) spans = cols;
-  const int span = (int)((cols + spans - 1) / spans) * kTileCols;
-  return launch_overlapped(expand_packed_kernel<T>, dim3(packed_tiles(p), (p.n_out + span - 1) / span), kPackThreads, bytes(rp), s, p,
-                           (const float*)h, slices_of(p), rp, span);
+  // CTAs that the GPU holds at once, asked once per device and rank (what is written twice is the same)
+  int device = 0;
+  e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  static int resident[kMaxDevices][17];
+  int& fits = resident[device][rp / 16];
+  if (fits == 0) {
+    int per_sm = 0, sms = 0;
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, expand_packed_kernel<T>, kPackThreads, bytes(rp));
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e != cudaSuccess) return e;
+    fits = per_sm * sms > 0 ? per_sm * sms : 1;
+  }
+  const int64_t units = (int64_t)packed_tiles(p) * ((p.n_out + kTileCols - 1) / kTileCols);
+  return launch_overlapped(expand_packed_kernel<T>, dim3((unsigned)(units < fits ? units : fits)), kPackThreads, bytes(rp), s, 1, p, (const T*)h, rp);
 }
 
 template <typename T>
-cudaError_t launch_adapters(const WsvdAdapterAddParams& p, float* h, cudaStream_t s) {
-  if (whole_vectors(p)) return p.cu_new != nullptr ? launch_packed<T>(p, h, s) : launch_step<T>(p, h, s);
+cudaError_t launch_adapters(const WsvdAdapterAddParams& p, void* workspace, cudaStream_t s) {
+  float* h = reinterpret_cast<float*>(workspace);
+  if (whole_vectors(p)) return p.cu_new != nullptr ? launch_packed<T>(p, reinterpret_cast<T*>(workspace), s) : launch_step<T>(p, h, s);
   shrink_any_kernel<T><<<p.rows, 128, 0, s>>>(p, h);
   expand_any_kernel<T><<<dim3(p.rows, (p.n_out + 255) / 256), 256, 0, s>>>(p, h);
   return cudaGetLastError();
@@ -679,7 +736,8 @@ extern "C" {
 
 size_t wsvd_adapter_add_workspace_bytes(const WsvdAdapterAddParams* p) {
   if (!p || p->rows <= 0 || p->rank <= 0 || p->n_in <= 0 || p->batch < 0) return 0;
-  // (on the kernels for any shape one slice is used)
+  // packed rows: h in f32 or, its rows padded, in 16 bits; one row per request: a sum per slice of the input
+  if (p->cu_new) return (size_t)p->rows * (p->rank < 16 ? 16 : p->rank) * sizeof(float);
   return (size_t)wsvd::slices_of(*p) * p->rows * p->rank * sizeof(float);
 }
 
@@ -697,8 +755,8 @@ int wsvd_adapter_add(const WsvdAdapterAddParams* p, void* workspace, size_t work
   if (workspace_bytes < wsvd_adapter_add_workspace_bytes(p)) return WSVD_ERR_WORKSPACE_TOO_SMALL;
   if ((reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return WSVD_ERR_BAD_STRIDE;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  float* h = reinterpret_cast<float*>(workspace);
-  const cudaError_t e = p->dtype == WSVD_F16 ? wsvd::launch_adapters<__half>(*p, h, s) : wsvd::launch_adapters<__nv_bfloat16>(*p, h, s);
+  const cudaError_t e = p->dtype == WSVD_F16 ? wsvd::launch_adapters<__half>(*p, workspace, s)
+                                             : wsvd::launch_adapters<__nv_bfloat16>(*p, workspace, s);
   return e == cudaSuccess ? WSVD_OK : wsvd::record_cuda_error(e);
 }
 

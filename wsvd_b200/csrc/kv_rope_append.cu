@@ -336,7 +336,7 @@ cudaError_t launch_vec(const WsvdKvRopeAppendParams& p, int lanes, int per_row, 
   const int most_rows = (kVecThreads * U - 1) / per_row + 2;
   const size_t smem = (size_t)most_rows * (2 * sizeof(int64_t) + p.rot_dim / 2 * sizeof(float2));
   return launch_overlapped(kv_append_vec_kernel<T, I8, U>, dim3((unsigned)((total + kVecThreads * U - 1) / (kVecThreads * U))),
-                           kVecThreads, smem, s, p, lanes, Divisor::of(per_row), most_rows);
+                           kVecThreads, smem, s, 1, p, lanes, Divisor::of(per_row), most_rows);
 }
 
 template <typename T, bool I8>

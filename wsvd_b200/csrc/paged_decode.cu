@@ -126,7 +126,6 @@ __global__ void __launch_bounds__(kAnyWarps * 32) paged_decode_any_kernel(const 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 // bounds of the shares, for the workspace: CTAs of a GPU of so many SMs, CTAs of an item
 constexpr int kMaxSms = 160, kMaxCtas = 4, kMaxParts = 128;
-constexpr int kMaxDevices = 64;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {  // zeros where it is not on
@@ -869,13 +868,13 @@ cudaError_t launch_fast(const WsvdPagedDecodeParams& p, const Items& it, const P
   const int64_t tiles = items * ((reach + tile - 1) / tile);
   if (grid > tiles) grid = tiles;
   if (grid < 1) grid = 1;
-  e = launch_overlapped(paged_decode_kernel<C>, dim3((unsigned)grid), kThreads, (size_t)C::RING, s, p, part, it);
+  e = launch_overlapped(paged_decode_kernel<C>, dim3((unsigned)grid), kThreads, (size_t)C::RING, s, 1, p, part, it);
   if (e != cudaSuccess || reach <= C::TOK) return e;  // (one warp an item and head: no partials)
   // (an item has about grid / items + 1 CTAs: one round of loads for four warps, else many warps)
   const dim3 heads(p.n_q_heads, p.batch);
   if (grid * (kWarps / it.hw) <= 14 * items)
-    return launch_overlapped(paged_merge_kernel<typename C::T, C::D, 4>, heads, 4 * 32, 0, s, p, part, it);
-  return launch_overlapped(paged_merge_kernel<typename C::T, C::D, 16>, heads, 16 * 32, 0, s, p, part, it);
+    return launch_overlapped(paged_merge_kernel<typename C::T, C::D, 4>, heads, 4 * 32, 0, s, 1, p, part, it);
+  return launch_overlapped(paged_merge_kernel<typename C::T, C::D, 16>, heads, 16 * 32, 0, s, 1, p, part, it);
 }
 
 template <typename T, bool I8, int NT>
