@@ -279,11 +279,11 @@ expand_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* 
 //
 // Bound by x, y and out.  Shrink: a warp has 16 rows and all ranks, tiles of 64 inputs come by 16-byte asynchronous copies;
 // the input's length is cut into slices over the CTAs of a cluster, so that every SM has work, and their sums meet in
-// shared memory in a fixed order.  h is rounded once to the 16-bit type (a step of it is 2^-9 of the adapter's share of the
-// result, which is rounded to that type itself).  Expand: equal shares of (tile, 128 columns) over the CTAs that the GPU
+// shared memory in a fixed order (left to the expanding CTAs in f32 they cost those 12 us).  h is rounded once to the 16-bit
+// type (a step of it is 2^-9 of the adapter's share of the result, which is rounded to that type itself).  Expand: equal shares of (tile, 128 columns) over the CTAs that the GPU
 // holds at once; a CTA keeps its tile's h, B's columns come from L2 and y's from memory a step ahead, y + product in place
 // in shared memory, 16-byte stores.
-constexpr int kTileRows = 64, kTileK = 64, kTileCols = 128, kPackThreads = 128;
+constexpr int kTileRows = 64, kTileCols = 64, kPackThreads = 128, kColPieces = kTileCols / 8;
 
 // The row tiles of the batch, numbered through the requests in order; what is behind the last one counts as one more request
 // without an adapter where it is copied.  Every thread knows the tiles [before, before + mine) of its requests.
@@ -374,24 +374,33 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
+__device__ __forceinline__ void stmatrix4(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};\n" ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+}
 template <typename T>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 // RP: the rank rounded up to 16, 32, 64, 128 or 256.  Pitches are an odd number of 16-byte pieces (conflict-free ldmatrix).
+// Up to 64 ranks a warp takes half of the rows and every other 16 inputs, so that A is read from shared memory twice and not
+// four times (shared memory is what bounds the loop: 56 KB a stage with the rows alone dealt out, 40 KB so, 32 KB with the
+// inputs alone, whose 128 accumulators cost a resident CTA); above, a warp takes 16 rows.
 template <int RP>
 struct Shrink {
-  static constexpr int X_PITCH = kTileK * 2 + 16, A_PITCH = RP * 2 + 16;
-  static constexpr int STAGE = kTileRows * X_PITCH + kTileK * A_PITCH;
-  static constexpr int STAGES = RP <= 128 ? 3 : 2;
+  static constexpr int K = 64, STAGES = RP <= 128 ? 3 : 2;  // inputs of a stage
+  static constexpr bool BY_INPUT = RP <= 64;
+  static constexpr int MT = BY_INPUT ? 2 : 1;               // 16-row tiles of a warp
+  static constexpr int X_PITCH = K * 2 + 16, A_PITCH = RP * 2 + 16;
+  static constexpr int STAGE = kTileRows * X_PITCH + K * A_PITCH;
+  static constexpr int LD = RP + 4;  // of the warps' sums (four more words a row: no bank twice)
 };
-// h [rows][rp]: rp is the rank rounded up to 16
+// h [rows][rp] in 16 bits: rp is the rank rounded up to 16.  The CTAs of a cluster (along y) have one tile and a slice each.
 template <typename T, int RP>
 __global__ void __launch_bounds__(kPackThreads)
 shrink_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, T* h, const int slice, const int rp) {
@@ -400,92 +409,143 @@ shrink_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, T* h, const
   before_this();
   let_next_in();
   const RowTiles tiles(p);
-  if ((int)blockIdx.x >= tiles.total) return;  // (the CTAs of a cluster have one tile)
+  if ((int)blockIdx.x >= tiles.total) return;
   const RowTile tile = tiles.find(blockIdx.x);
   if (tile.adapter < 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int k0 = min(p.n_in, (int)blockIdx.y * slice), k1 = min(p.n_in, k0 + slice), steps = (k1 - k0 + kTileK - 1) / kTileK;
+  const int k0 = min(p.n_in, (int)blockIdx.y * slice), k1 = min(p.n_in, k0 + slice), steps = (k1 - k0 + S::K - 1) / S::K;
   const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)tile.row * p.x_stride;
   const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)tile.adapter * p.a_stride_i;
   const uint32_t ring = smem_addr(smem);
   const bool wide_a = p.rank % 8 == 0 && p.a_stride_k % 8 == 0 && p.a_stride_i % 8 == 0 && (reinterpret_cast<uintptr_t>(p.a) & 15) == 0;
-  auto request = [&](int step) {
-    if (step < steps) {
-      const int k = k0 + step * kTileK;
-      const uint32_t xd = ring + (step % S::STAGES) * S::STAGE, ad = xd + kTileRows * S::X_PITCH;
+  // A thread's pieces of a stage: one column and every so many rows of x, and of A in 16- or 8-byte pieces.  (Addresses are
+  // carried on: working them out took as long as the products.)
+  constexpr int XP = S::K / 8, XROWS = kPackThreads / XP, XN = kTileRows / XROWS;
+  const int x_row = threadIdx.x / XP, x_col = (threadIdx.x % XP) * 8;
+  const T* x_at = x + (int64_t)x_row * p.x_stride + k0 + x_col;
+  const int64_t x_skip = XROWS * p.x_stride;
+  uint32_t x_on = 0;
 #pragma unroll
-      for (int i = 0; i < kTileRows * (kTileK / 8) / kPackThreads; ++i) {
-        const int piece = threadIdx.x + i * kPackThreads, row = piece / (kTileK / 8), col = (piece % (kTileK / 8)) * 8;
-        const bool on = row < tile.rows && k + col < k1;
-        copy16(xd + row * S::X_PITCH + col * 2, x + (on ? (int64_t)row * p.x_stride + k + col : 0), on);
+  for (int i = 0; i < XN; ++i) x_on |= (uint32_t)(x_row + i * XROWS < tile.rows) << i;
+  const uint32_t x_to = x_row * S::X_PITCH + x_col * 2;
+  const int ap = wide_a ? RP / 8 : RP / 4, a_rows = kPackThreads / ap, a_row = threadIdx.x / ap, a_col = threadIdx.x % ap * (RP / ap);
+  const bool a_on = a_col < p.rank;
+  const T* a_at = a + (int64_t)(k0 + a_row) * p.a_stride_k + (a_on ? a_col : 0);
+  const int64_t a_skip = a_rows * p.a_stride_k, a_step = S::K * p.a_stride_k;
+  const uint32_t a_to = kTileRows * S::X_PITCH + a_row * S::A_PITCH + a_col * 2;
+  int next = 0;
+  uint32_t next_stage = ring;
+  auto request = [&]() {
+    if (next < steps) {
+      const int k = k0 + next * S::K;
+      const bool col_on = k + x_col < k1;
+      const T* from = x_at;
+#pragma unroll
+      for (int i = 0; i < XN; ++i, from += x_skip) {
+        const bool on = col_on && ((x_on >> i) & 1);
+        copy16(next_stage + x_to + i * XROWS * S::X_PITCH, on ? from : x, on);
       }
+      x_at += S::K;
+      from = a_at;
       if (wide_a) {
+        constexpr int ROWS = kPackThreads / (RP / 8);
 #pragma unroll
-        for (int i = 0; i < kTileK * (RP / 8) / kPackThreads; ++i) {
-          const int piece = threadIdx.x + i * kPackThreads, row = piece / (RP / 8), col = (piece % (RP / 8)) * 8;
-          const bool on = k + row < k1 && col < p.rank;
-          copy16(ad + row * S::A_PITCH + col * 2, a + (on ? (int64_t)(k + row) * p.a_stride_k + col : 0), on);
+        for (int i = 0; i < S::K / ROWS; ++i, from += a_skip) {
+          const bool on = a_on && k + a_row + i * ROWS < k1;
+          copy16(next_stage + a_to + i * ROWS * S::A_PITCH, on ? from : a, on);
         }
       } else {
+        constexpr int ROWS = kPackThreads / (RP / 4);
 #pragma unroll
-        for (int i = 0; i < kTileK * (RP / 4) / kPackThreads; ++i) {
-          const int piece = threadIdx.x + i * kPackThreads, row = piece / (RP / 4), col = (piece % (RP / 4)) * 4;
-          const bool on = k + row < k1 && col < p.rank;
-          copy8(ad + row * S::A_PITCH + col * 2, a + (on ? (int64_t)(k + row) * p.a_stride_k + col : 0), on);
+        for (int i = 0; i < S::K / ROWS; ++i, from += a_skip) {
+          const bool on = a_on && k + a_row + i * ROWS < k1;
+          copy8(next_stage + a_to + i * ROWS * S::A_PITCH, on ? from : a, on);
         }
       }
+      a_at += a_step;
     }
+    ++next;
+    next_stage = next_stage == ring + (S::STAGES - 1) * S::STAGE ? ring : next_stage + S::STAGE;
     copies_commit();
   };
-  float acc[RP / 8][4];
+  float acc[S::MT][RP / 8][4];
 #pragma unroll
-  for (int j = 0; j < RP / 8; ++j)
+  for (int i = 0; i < S::MT * RP / 8 * 4; ++i) (&acc[0][0][0])[i] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
-#pragma unroll
-  for (int i = 0; i < S::STAGES - 1; ++i) request(i);
+  for (int i = 0; i < S::STAGES - 1; ++i) request();
+  uint32_t xd = ring;
+  const int warp_row = S::BY_INPUT ? (warp >> 1) * 32 : warp * 16;
   for (int step = 0; step < steps; ++step) {
     copies_wait<S::STAGES - 2>();
     __syncthreads();  // this step's tiles are there for all, and all have done with the stage that is filled next
-    request(step + S::STAGES - 1);
-    const uint32_t xd = ring + (step % S::STAGES) * S::STAGE, ad = xd + kTileRows * S::X_PITCH;
-    const uint32_t xa = xd + (warp * 16 + (lane & 15)) * S::X_PITCH + (lane >> 4) * 16;
+    request();
+    const uint32_t ad = xd + kTileRows * S::X_PITCH;
+    const uint32_t xa = xd + (warp_row + (lane & 15)) * S::X_PITCH + (lane >> 4) * 16;
     const uint32_t aa = ad + (lane & 15) * S::A_PITCH + (lane >> 4) * 16;
 #pragma unroll
-    for (int k = 0; k < kTileK / 16; ++k) {
-      uint32_t xr[4];
-      ldmatrix4(xr, xa + k * 32);
+    for (int kk = 0; kk < S::K / 16 / (S::BY_INPUT ? 2 : 1); ++kk) {
+      const int k = S::BY_INPUT ? 2 * kk + (warp & 1) : kk;
+      uint32_t xr[S::MT][4];
 #pragma unroll
-      for (int j = 0; j < RP / 16; ++j) {
-        uint32_t w[4];  // ranks 16 j .. + 7: w[0], w[1] (inputs 0-7, 8-15); + 8 .. + 15: w[2], w[3]
-        ldmatrix4_trans(w, aa + k * 16 * S::A_PITCH + j * 32);
-        mma<T>(acc[2 * j], xr, w[0], w[1]);
-        mma<T>(acc[2 * j + 1], xr, w[2], w[3]);
+      for (int i = 0; i < S::MT; ++i) ldmatrix4(xr[i], xa + i * 16 * S::X_PITCH + k * 32);
+      constexpr int AT = RP / 16 < 4 ? RP / 16 : 4;  // loads in flight in front of their products
+#pragma unroll
+      for (int j0 = 0; j0 < RP / 16; j0 += AT) {
+        uint32_t w[AT][4];  // ranks 16 j .. + 7: w[j][0], w[j][1] (inputs 0-7, 8-15); + 8 .. + 15: w[j][2], w[j][3]
+#pragma unroll
+        for (int j = 0; j < AT; ++j) ldmatrix4_trans(w[j], aa + k * 16 * S::A_PITCH + (j0 + j) * 32);
+#pragma unroll
+        for (int j = 0; j < AT; ++j)
+#pragma unroll
+          for (int i = 0; i < S::MT; ++i) {
+            mma<T>(acc[i][2 * (j0 + j)], xr[i], w[j][0], w[j][1]);
+            mma<T>(acc[i][2 * (j0 + j) + 1], xr[i], w[j][2], w[j][3]);
+          }
       }
     }
+    xd = xd == ring + (S::STAGES - 1) * S::STAGE ? ring : xd + S::STAGE;
   }
-  // the slices' sums: each CTA leaves its own in its shared memory, and adds up its part of the rows from all of them
+  // the sums of the warps with other inputs, then those of the slices: each CTA leaves its own in its shared memory and adds up
+  // its part of the rows from all of them
   copies_wait<0>();
   __syncthreads();
-  constexpr int LD = RP + 4;  // (four more words a row: no bank twice)
   float* sums = reinterpret_cast<float*>(smem);
   const int g = lane >> 2, c4 = lane & 3;
 #pragma unroll
-  for (int j = 0; j < RP / 8; ++j)
+  for (int pass = S::BY_INPUT ? 0 : 1; pass < 2; ++pass) {
+    if (!S::BY_INPUT || (warp & 1) != pass)
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
-      *reinterpret_cast<float2*>(sums + (warp * 16 + g + 8 * e) * LD + 8 * j + 2 * c4) = make_float2(acc[j][2 * e], acc[j][2 * e + 1]);
+      for (int i = 0; i < S::MT; ++i)
+#pragma unroll
+        for (int j = 0; j < RP / 8; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float2* at = reinterpret_cast<float2*>(sums + (warp_row + 16 * i + g + 8 * e) * S::LD + 8 * j + 2 * c4);
+            float2 v = make_float2(acc[i][j][2 * e], acc[i][j][2 * e + 1]);
+            if (S::BY_INPUT && pass == 1) {
+              const float2 w = *at;
+              v.x += w.x;
+              v.y += w.y;
+            }
+            *at = v;
+          }
+    if (pass == 0) __syncthreads();
+  }
   const auto cluster = cooperative_groups::this_cluster();
   cluster.sync();
   const int slices = cluster.num_blocks(), part = kTileRows / slices, from = (int)cluster.block_rank() * part;
   for (int i = threadIdx.x; i < part * (rp / 2); i += kPackThreads) {
     const int row = from + i / (rp / 2), r = (i % (rp / 2)) * 2;
     if (row >= tile.rows) continue;
-    float2 v = make_float2(0.f, 0.f);
-    for (int c = 0; c < slices; ++c) {
-      const float2 w = *reinterpret_cast<const float2*>(cluster.map_shared_rank(sums, c) + row * LD + r);
-      v.x += w.x;
-      v.y += w.y;
+    float2 w[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c)  // (all loads in flight)
+      w[c] = c < slices ? *reinterpret_cast<const float2*>(cluster.map_shared_rank(sums, c) + row * S::LD + r) : make_float2(0.f, 0.f);
+    float2 v = w[0];
+#pragma unroll
+    for (int c = 1; c < 8; ++c) {
+      v.x += w[c].x;
+      v.y += w[c].y;
     }
     *reinterpret_cast<uint32_t*>(h + (int64_t)(tile.row + row) * rp + r) = both<T>(v.x, v.y);  // (ranks up to rp: zeros)
   }
@@ -494,7 +554,7 @@ shrink_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, T* h, const
 
 constexpr int kColPitch = kTileCols * 2 + 16;  // bytes of a tile row of B or y
 template <typename T>
-__global__ void __launch_bounds__(kPackThreads)
+__global__ void __launch_bounds__(kPackThreads, 4)
 expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const T* h, const int rp) {
   extern __shared__ __align__(16) unsigned char smem[];  // h [64][rp], then two stages of B [rp][128] and y [64][128]
   // (What is read before the wait is nothing that the shrinking kernel writes: see expand_step_kernel.)
@@ -534,22 +594,35 @@ expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const T* h,
       continue;
     }
     const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)tile.adapter * p.b_stride_i;
-    const int col = (threadIdx.x & 15) * 8;
+    // a thread's pieces of a unit: one column, every so many rows of B and of the warp's own 16 of y
+    constexpr int BROWS = kPackThreads / kColPieces, YROWS = 32 / kColPieces, YN = 16 / YROWS;
+    const int col = (threadIdx.x % kColPieces) * 8, b_row = threadIdx.x / kColPieces, y_row = warp * 16 + lane / kColPieces;
+    const T* b_at = b + (int64_t)b_row * p.b_stride_r + c0 + col;
+    const T* y_at = y + (int64_t)y_row * p.y_stride + c0 + col;
+    T* out_at = out + (int64_t)y_row * p.out_stride + c0 + col;
+    const int64_t b_skip = BROWS * p.b_stride_r, y_skip = YROWS * p.y_stride, out_skip = YROWS * p.out_stride;
+    uint32_t y_on = 0;
+#pragma unroll
+    for (int i = 0; i < YN; ++i) y_on |= (uint32_t)(y_row + i * YROWS < tile.rows) << i;
     auto request = [&](int step) {
       if (step < steps) {
-        const int c = c0 + step * kTileCols;
-        const uint32_t bd = ring + (step & 1) * stage_bytes, yd = bd + b_bytes;
-        const bool in = c + col < c1;
-        for (int row = threadIdx.x >> 4; row < rp; row += kPackThreads / 16) {
-          const bool on = in && row < p.rank;
-          copy16(bd + row * kColPitch + col * 2, b + (on ? (int64_t)row * p.b_stride_r + c + col : 0), on);
-        }
+        const uint32_t bd = ring + (step & 1) * stage_bytes + b_row * kColPitch + col * 2;
+        const uint32_t yd = ring + (step & 1) * stage_bytes + b_bytes + y_row * kColPitch + col * 2;
+        const bool in = c0 + step * kTileCols + col < c1;
+        const T* from = y_at;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {  // the warp's own 16 rows
-          const int row = warp * 16 + 2 * i + (lane >> 4);
-          const bool on = in && row < tile.rows;
-          copy16(yd + row * kColPitch + col * 2, y + (on ? (int64_t)row * p.y_stride + c + col : 0), on);
+        for (int i = 0; i < YN; ++i, from += y_skip) {
+          const bool on = in && ((y_on >> i) & 1);
+          copy16(yd + i * YROWS * kColPitch, on ? from : y, on);
         }
+        y_at += kTileCols;
+        from = b_at;
+#pragma unroll 4
+        for (int i = 0; i < rp / BROWS; ++i, from += b_skip) {
+          const bool on = in && b_row + i * BROWS < p.rank;
+          copy16(bd + i * BROWS * kColPitch, on ? from : b, on);
+        }
+        b_at += kTileCols;
       }
       copies_commit();
     };
@@ -567,40 +640,48 @@ expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const T* h,
       copies_wait<1>();
       __syncthreads();
       const uint32_t bd = ring + (step & 1) * stage_bytes;
-      unsigned char* yt = smem + kTileRows * h_pitch + (step & 1) * stage_bytes + b_bytes;
+      const uint32_t yt = bd + b_bytes;
       float acc[kTileCols / 8][4];
 #pragma unroll
       for (int j = 0; j < kTileCols / 8; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
+      const uint32_t ha = hd + (warp * 16 + (lane & 15)) * h_pitch + (lane >> 4) * 16;
+      const uint32_t ba = bd + (lane & 15) * kColPitch + (lane >> 4) * 16;
+#pragma unroll 2
       for (int k = 0; k < rp / 16; ++k) {
-        uint32_t hr[4];
-        ldmatrix4(hr, hd + (warp * 16 + (lane & 15)) * h_pitch + (lane >> 4) * 16 + k * 32);
-        const uint32_t ba = bd + (16 * k + (lane & 15)) * kColPitch + (lane >> 4) * 16;
+        uint32_t hr[4], w[kTileCols / 16][4];
+        ldmatrix4(hr, ha + k * 32);
+#pragma unroll
+        for (int j = 0; j < kTileCols / 16; ++j) ldmatrix4_trans(w[j], ba + k * 16 * kColPitch + j * 32);
 #pragma unroll
         for (int j = 0; j < kTileCols / 16; ++j) {
-          uint32_t w[4];
-          ldmatrix4_trans(w, ba + j * 32);
-          mma<T>(acc[2 * j], hr, w[0], w[1]);
-          mma<T>(acc[2 * j + 1], hr, w[2], w[3]);
+          mma<T>(acc[2 * j], hr, w[j][0], w[j][1]);
+          mma<T>(acc[2 * j + 1], hr, w[j][2], w[j][3]);
         }
       }
+      // y as the accumulators hold their values, 16 rows of 16 columns at a time, and back
+      const uint32_t ya = yt + (warp * 16 + (lane & 15)) * kColPitch + (lane >> 4) * 16;
 #pragma unroll
-      for (int j = 0; j < kTileCols / 8; ++j)
+      for (int j = 0; j < kTileCols / 16; ++j) {
+        uint32_t v[4];  // rows 0-7 and 8-15 of columns 0-7, then of columns 8-15
+        ldmatrix4(v, ya + j * 32);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          uint32_t* at = reinterpret_cast<uint32_t*>(yt + (warp * 16 + g + 8 * e) * kColPitch + (8 * j + 2 * c4) * 2);
-          const float2 v = two<T>(*at);
-          *at = both<T>(fmaf(scale, acc[j][2 * e], v.x), fmaf(scale, acc[j][2 * e + 1], v.y));
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = two<T>(v[e]);
+          const float* d = acc[2 * j + (e >> 1)] + 2 * (e & 1);
+          v[e] = both<T>(fmaf(scale, d[0], f.x), fmaf(scale, d[1], f.y));
         }
+        stmatrix4(ya + j * 32, v);
+      }
       __syncwarp();  // the warp's rows are its own
-      const int c = c0 + step * kTileCols + col;
+      const uint32_t from = yt + y_row * kColPitch + col * 2;
+      T* to = out_at;
+      const bool in = c0 + step * kTileCols + col < c1;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int row = warp * 16 + 2 * i + (lane >> 4);
-        if (c < c1 && row < tile.rows)
-          *reinterpret_cast<uint4*>(out + (int64_t)row * p.out_stride + c) = *reinterpret_cast<const uint4*>(yt + row * kColPitch + col * 2);
-      }
+      for (int i = 0; i < YN; ++i, to += out_skip)
+        if (in && ((y_on >> i) & 1)) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(smem + (from - hd) + i * YROWS * kColPitch);
+      out_at += kTileCols;
       __syncthreads();  // the stage may be filled again
     }
     copies_wait<0>();
@@ -666,15 +747,15 @@ cudaError_t allow_smem(K kernel, bool (&ready)[kMaxDevices], size_t bytes) {
 
 template <typename T, int RP>
 cudaError_t launch_shrink(const WsvdAdapterAddParams& p, T* h, cudaStream_t s) {
+  using S = Shrink<RP>;
   static bool ready[kMaxDevices];
-  constexpr size_t ring = (size_t)Shrink<RP>::STAGES * Shrink<RP>::STAGE, sums = (size_t)kTileRows * (RP + 4) * sizeof(float);
-  constexpr size_t smem = ring > sums ? ring : sums;
+  constexpr size_t ring = (size_t)S::STAGES * S::STAGE, sums = (size_t)kTileRows * S::LD * sizeof(float), smem = ring > sums ? ring : sums;
   const cudaError_t e = allow_smem(shrink_packed_kernel<T, RP>, ready, smem);
   if (e != cudaSuccess) return e;
   // slices: enough CTAs for every SM to have three, none shorter than 256 inputs
   int slices = 1;
   while (slices < 8 && (int64_t)(p.rows / kTileRows + 1) * slices < 148 * 3 && p.n_in / (2 * slices) >= 256) slices *= 2;
-  const int slice = ((p.n_in + slices - 1) / slices + kTileK - 1) / kTileK * kTileK;
+  const int slice = ((p.n_in + slices - 1) / slices + S::K - 1) / S::K * S::K;
   return launch_overlapped(shrink_packed_kernel<T, RP>, dim3(packed_tiles(p), slices), kPackThreads, smem, s, slices, p, h, slice, rank_16(p));
 }
 

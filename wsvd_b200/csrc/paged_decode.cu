@@ -213,7 +213,7 @@ struct Cfg {
   using T = T_;                                                         // q and out
   using M = typename std::conditional<I8_, __half, T_>::type;           // the products' operands
   static constexpr bool I8 = I8_;
-  static constexpr int D = D_, NT = NT_, HEADS = 8 * NT_;               // query heads of an item, at most
+  static constexpr int D = D_, NT = NT_;                                // NT: eights of query heads of an item
   static constexpr int ROW = D * (I8 ? 1 : 2), PIECES = ROW / 16;       // bytes and 16-byte pieces of a cached row
   // conflict-free ldmatrix: the pieces of a row changed about by the row's number, or rows of an odd number of pieces
   static constexpr bool SWZ = PIECES == 8 || PIECES == 16 || PIECES == 32;
