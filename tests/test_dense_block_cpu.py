@@ -36,6 +36,52 @@ def _adapters(**kw):
     return lambda: ops.adapter_add(a.pop("y"), a.pop("x"), a.pop("a"), a.pop("b"), a.pop("adapter"), **a)
 
 
+def _bind_args(op, kw):
+    """The arguments of csrc/bind.cpp's function for a call of `op`, in its order."""
+    g = torch.Generator().manual_seed(1)
+    table, T = pages(2, 8, 4, g)
+    st = kw.get("infer_state") or state([1, 2], table)
+    meta = [st.b_seq_len, st.b_req_idx, st.req_manager.req_to_token_indexs]
+    if op == "append":
+        d = dict(k=torch.zeros(2, 2, 16, dtype=H16), v=torch.zeros(2, 2, 16, dtype=H16), cache_k=torch.zeros(T, 2, 16, dtype=H16),
+                 cache_v=torch.zeros(T, 2, 16, dtype=H16), inv_freq=torch.ones(8))
+        d.update(kw)
+        return [d["k"], d["v"], *meta, *(d.get(n) for n in ("cache_k", "cache_v", "inv_freq", "cache_k_scale", "cache_v_scale", "q", "q_out",
+                                                           "cu_new", "pos_offset")), 0]
+    if op == "paged":
+        d = dict(q=torch.zeros(2, 4, 16, dtype=H16), cache_k=torch.zeros(T, 2, 16, dtype=H16), cache_v=torch.zeros(T, 2, 16, dtype=H16))
+        d.update(kw)
+        return [d["q"], *meta, *(d.get(n) for n in ("cache_k", "cache_v", "k_scale", "v_scale", "out", "workspace")), False,
+                d.get("window", 0), 0.0]
+    d = dict(y=torch.zeros(3, 24, dtype=H16), x=torch.zeros(3, 16, dtype=H16), a=torch.zeros(2, 16, 4, dtype=H16),
+             b=torch.zeros(2, 4, 24, dtype=H16), adapter=torch.zeros(3, dtype=torch.int32))
+    d.update(kw)
+    return [d.get(n) for n in ("y", "x", "a", "b", "adapter", "scale", "cu_new", "out", "workspace")]
+
+
+def _fits(op, **kw):
+    return getattr(_lib.bind(), op + "_fits")(*_bind_args(op, kw))
+
+
+def test_ordinary_calls_fit_and_no_cpu_tensor_is_launched_on():
+    g = torch.Generator().manual_seed(1)
+    i8 = dict(cache_k=_i8(20, 2, 16), cache_v=_i8(20, 2, 16))
+    sc = torch.zeros(20, 2, dtype=H16)
+    q = torch.zeros(2, 4, 16, dtype=H16)
+    for kw in ({}, dict(q=q), dict(q=q, q_out=q), dict(cu_new=torch.zeros(3, dtype=torch.int32)), dict(pos_offset=torch.zeros(2, dtype=torch.int32)),
+               dict(cache_k_scale=sc, cache_v_scale=sc, **i8), dict(inv_freq=torch.ones(0))):
+        assert _fits("append", **kw), kw
+        assert _lib.bind().append(*_bind_args("append", kw)) is None
+    for kw in ({}, dict(out=q), dict(window=5), dict(k_scale=sc, v_scale=sc, **i8), dict(workspace=torch.zeros(4))):
+        assert _fits("paged", **kw), kw
+        assert _lib.bind().paged(*_bind_args("paged", kw)) is None
+    for kw in ({}, dict(scale=torch.ones(2)), dict(adapter=torch.zeros(2, dtype=torch.int32), cu_new=torch.zeros(3, dtype=torch.int32))):
+        assert _fits("adapter", **kw), kw
+        assert _lib.bind().adapter(*_bind_args("adapter", kw)) is None
+    y = torch.zeros(3, 24, dtype=H16)
+    assert _fits("adapter", y=y, out=y)
+
+
 def _i8(*shape):
     return torch.zeros(*shape, dtype=torch.int8)
 
@@ -74,14 +120,17 @@ def test_a_valid_call_without_a_gpu_is_refused_for_the_device_alone(call):
     (dict(k=torch.zeros(2, 2, 16, dtype=H16, requires_grad=True)), ValueError, "no backward"),
 ])
 def test_append_refusals(kw, exc, match):
+    assert "rope_layout" in kw or not _fits("append", **kw)
     with pytest.raises(exc, match=match):
         _append(**kw)()
 
 
 def test_append_refuses_a_shifted_view_as_q_out():
     buf = torch.zeros(2, 4, 32, dtype=H16)
+    kw = dict(q=buf[..., :16], q_out=buf.view(-1)[:128].view(2, 4, 16))
+    assert not _fits("append", **kw)
     with pytest.raises(ValueError, match="another view"):
-        _append(q=buf[..., :16], q_out=buf.view(-1)[:128].view(2, 4, 16))()
+        _append(**kw)()
 
 
 @pytest.mark.parametrize("kw,exc,match", [
@@ -98,6 +147,7 @@ def test_append_refuses_a_shifted_view_as_q_out():
     (dict(q=torch.zeros(2, 4, 16, dtype=H16, requires_grad=True)), ValueError, "no backward"),
 ])
 def test_paged_decode_refusals(kw, exc, match):
+    assert not _fits("paged", **kw)
     with pytest.raises(exc, match=match):
         _paged(**kw)()
 
@@ -119,14 +169,16 @@ def test_paged_decode_refusals(kw, exc, match):
     (dict(b=torch.zeros(2, 4, 24, dtype=H16, requires_grad=True)), ValueError, "no backward"),
 ])
 def test_adapter_refusals(kw, exc, match):
+    assert not _fits("adapter", **kw)
     with pytest.raises(exc, match=match):
         _adapters(**kw)()
 
 
 def test_adapter_refuses_a_shifted_view_as_out():
     y = torch.zeros(3, 24, dtype=H16)
+    assert not _fits("adapter", y=y, out=y.as_strided((3, 24), (1, 1)))
     with pytest.raises(ValueError, match="another view"):
-        _adapters(y=y, out=y.view(-1).as_strided((3, 24), (1, 1)))()
+        _adapters(y=y, out=y.as_strided((3, 24), (1, 1)))()
 
 
 # ---- the C entries: a status before any CUDA call

@@ -584,3 +584,43 @@ def test_ops_on_another_stream():
         other.synchronize()
         assert torch.equal(got, want) and torch.equal(got_y, want_y)
         del noise
+
+
+def test_the_long_way_round_gives_the_same():
+    """An allocator of the caller's, a stream of the caller's: not csrc/bind.cpp's ordinary call."""
+    g = torch.Generator().manual_seed(24)
+    table, T = pages(3, 90, 16, g)
+    st = gpu(state([90, 7, 0], table))
+    q, k, v = randn(g, 3, 8, 128).cuda(), randn(g, T, 2, 128).cuda(), randn(g, T, 2, 128).cuda()
+    mine = lambda shape, dtype, device: torch.empty(shape, dtype=dtype, device=device)  # noqa: E731
+    out, lse = ops.paged_decode(q, st, k, v, return_lse=True, window=50)
+    out2, lse2 = ops.paged_decode(q, st, k, v, return_lse=True, window=50, alloc_tensor_func=mine)
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+    x, y, a, b = randn(g, 9, 64).cuda(), randn(g, 9, 64).cuda(), randn(g, 2, 64, 8).cuda(), randn(g, 2, 8, 64).cuda()
+    ad = torch.tensor([0, 1, -1, 1, 0, 0, 1, 1, 0], dtype=torch.int32).cuda()
+    assert torch.equal(ops.adapter_add(y, x, a, b, ad), ops.adapter_add(y, x, a, b, ad, alloc_tensor_func=mine))
+    new = state([3, 0, 50], table)
+    inv = torch.rand(64, generator=g).cuda()
+    kk, vv = randn(g, 3, 2, 128).cuda(), randn(g, 3, 2, 128).cuda()
+    caches = [(k.clone(), v.clone()) for _ in range(2)]
+    here = torch.cuda.current_stream()
+    got = [ops.kv_rope_append(kk, vv, gpu(new), *c, inv, q=q, **kw) for c, kw in zip(caches, ({}, dict(stream=here)))]
+    assert torch.equal(got[0], got[1]) and all(torch.equal(a, b) for a, b in zip(*caches))
+
+
+@pytest.mark.parametrize("call", ["append", "paged", "adapter"])
+def test_refusals_on_the_gpu_launch_nothing(call):
+    g = torch.Generator().manual_seed(25)
+    table, T = pages(2, 8, 4, g)
+    st = gpu(state([1, 2], table))
+    z = lambda *s: torch.zeros(*s, dtype=F16, device="cuda")  # noqa: E731
+    with pytest.raises(ValueError, match="must be a CUDA tensor|expected cuda"):
+        if call == "append":
+            ops.kv_rope_append(z(2, 2, 16), z(2, 2, 16), st, z(T, 2, 16), z(T, 2, 16), torch.ones(8))
+        elif call == "paged":
+            ops.paged_decode(z(2, 4, 16), st, z(T, 2, 16).cpu(), z(T, 2, 16))
+        else:
+            ops.adapter_add(z(2, 8), z(2, 8), z(1, 8, 4), z(1, 4, 8), torch.zeros(2, dtype=torch.int32))
+    if call == "paged":
+        with pytest.raises(Exception, match="workspace"):
+            ops.paged_decode(z(2, 4, 128), st, z(T, 2, 128), z(T, 2, 128), workspace=torch.zeros(4, device="cuda"))

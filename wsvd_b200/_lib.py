@@ -17,6 +17,7 @@ _ROOT = os.path.dirname(_PKG)
 _CSRC = os.path.join(_PKG, "csrc")
 _INCLUDE = os.path.join(_ROOT, "include")
 LIB_PATH = os.path.join(_PKG, "libwsvd_b200.so")
+BIND_PATH = os.path.join(_PKG, "_bind.so")  # csrc/bind.cpp: calls of the dense block's operators straight from torch tensors
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -36,15 +37,38 @@ def _deps():
     return sources() + hdr + [os.path.join(_INCLUDE, "wsvd_b200.h")]
 
 
-def _stale() -> bool:
-    if not os.path.exists(LIB_PATH):
+def _bind_deps():
+    return [os.path.join(_CSRC, "bind.cpp"), os.path.join(_INCLUDE, "wsvd_b200.h")]
+
+
+def _older(path, deps) -> bool:
+    if not os.path.exists(path):
         return True
-    t = os.path.getmtime(LIB_PATH)
-    return any(os.path.getmtime(f) > t for f in _deps())
+    t = os.path.getmtime(path)
+    return any(os.path.getmtime(f) > t for f in deps)
+
+
+def _stale() -> bool:
+    return _older(LIB_PATH, _deps()) or _older(BIND_PATH, _bind_deps())
+
+
+def _bind_command(out):
+    """The compiler call for csrc/bind.cpp: a Python module on torch's headers and libraries."""
+    import importlib.util
+    import sysconfig
+
+    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    cuda = os.environ.get("CUDA_HOME") or "/usr/local/cuda"
+    include = [_INCLUDE, os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    libs = os.path.join(torch, "lib")
+    return [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{d}" for d in include),
+            os.path.join(_CSRC, "bind.cpp"), "-o", out, f"-L{libs}", f"-Wl,-rpath,{libs}", "-ltorch_python", "-ltorch_cpu", "-lc10",
+            "-lc10_cuda"]
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile every .cu under csrc/ into one shared object for sm_100a.
+    """Compile every .cu under csrc/ into one shared object for sm_100a, and csrc/bind.cpp into a Python module.
 
     Safe when several processes start at once (one rank per GPU under torchrun): the
     staleness check, the compile and the rename happen under an inter-process file lock, the
@@ -63,17 +87,23 @@ def build(force: bool = False, verbose: bool = False) -> str:
                 nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
                 if not os.path.exists(nvcc):
                     raise RuntimeError("nvcc not found: cannot build libwsvd_b200.so")
-                tmp = f"{LIB_PATH}.{os.getpid()}.tmp"
+                tmp, tmp_bind = (f"{p}.{os.getpid()}.tmp" for p in (LIB_PATH, BIND_PATH))
                 cmd = [nvcc, *NVCC_FLAGS, "-I", _INCLUDE, "-I", _CSRC, *sources(), "-o", tmp, "-lcuda"]
                 if verbose:
                     cmd.insert(1, "-Xptxas=-v")
+                bind = subprocess.Popen(_bind_command(tmp_bind), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
                 res = subprocess.run(cmd, capture_output=True, text=True)
-                if res.returncode != 0:
-                    if os.path.exists(tmp):
-                        os.remove(tmp)
-                    raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+                said = bind.communicate()[0]
+                if res.returncode != 0 or bind.returncode != 0:
+                    for f in (tmp, tmp_bind):
+                        if os.path.exists(f):
+                            os.remove(f)
+                    if res.returncode != 0:
+                        raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+                    raise RuntimeError("the C++ compiler failed on csrc/bind.cpp:\n" + said)
                 if verbose:
                     print(res.stderr)
+                os.replace(tmp_bind, BIND_PATH)
                 os.replace(tmp, LIB_PATH)
             finally:
                 fcntl.flock(lockfile, fcntl.LOCK_UN)
@@ -291,6 +321,28 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = handle
     return _lib
+
+
+_bind = None
+
+
+def bind():
+    """The module of csrc/bind.cpp, connected to the library's entries; builds both first where they are missing or stale."""
+    global _bind
+    if _bind is None:
+        import importlib.util
+
+        import torch  # noqa: F401  (the module's libraries)
+
+        handle = lib()
+        spec = importlib.util.spec_from_file_location("wsvd_b200._bind", BIND_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        module.connect(*(ctypes.cast(getattr(handle, f"wsvd_{n}"), ctypes.c_void_p).value for n in
+                         ("kv_rope_append", "paged_decode_workspace_bytes", "paged_decode", "adapter_add_workspace_bytes",
+                          "adapter_add")))
+        _bind = module
+    return _bind
 
 
 class WsvdError(RuntimeError):

@@ -462,8 +462,25 @@ _pack_paged = _lib.packer(_lib.PagedDecodeParams)
 _pack_adapter = _lib.packer(_lib.AdapterAddParams)
 
 
-# The checks below, one by one with their messages, take 12 us of a call that takes 8 without them.  So each op first asks
-# in one expression whether everything is as it should be, and goes through them only if it is not.
+# An ordinary call (the current stream, torch's allocator, arguments as they should be) goes through csrc/bind.cpp, which
+# answers None to any other: the checks below say what is wrong with it, or it is made the long way.  (A single token's append
+# takes the GPU 3 us; with its arguments looked at in Python the call took 14, so it takes 6.)
+
+_fast = None
+
+
+def _ordinary():
+    global _fast
+    if _fast is None:
+        _fast = _lib.bind()
+    return _fast
+
+
+def _done(answer, name):
+    """bind.cpp's answer, where it is one."""
+    if answer.__class__ is int:
+        check(answer, name)
+    return answer
 
 def _tensor(name, t, dtypes, ndim, inner_contiguous=True):
     """As `_cuda_tensor`, the device left to `_on_one_gpu`."""
@@ -520,19 +537,10 @@ def _dense_cache(cache_k, cache_v, k_scale, v_scale, dtype, Hkv, D):
         raise TypeError("only int8 caches have scales")
 
 
-def _scales_fit(k_scale, v_scale, shape, index):
-    """Whether these are the scales of an int8 cache of this shape."""
-    return (k_scale.dtype is torch.float16 and v_scale.dtype is torch.float16 and k_scale.shape == shape[:2]
-            and v_scale.shape == shape[:2] and k_scale.get_device() == index and v_scale.get_device() == index)
-
-
 def _new(alloc_tensor_func, like, shape, dtype, stream):
     """A buffer of the op's own.  On a stream of the caller's its memory must not go back to the current stream's pool while
     that one still works on it."""
-    if alloc_tensor_func is torch.empty:  # (half of its time)
-        t = like.new_empty(shape) if dtype is like.dtype else like.new_empty(shape, dtype=dtype)
-    else:
-        t = alloc_tensor_func(shape, dtype=dtype, device=like.device)
+    t = alloc_tensor_func(shape, dtype=dtype, device=like.device)
     if stream is not None:
         t.record_stream(stream)
     return t
@@ -611,53 +619,30 @@ def kv_rope_append(k, v, infer_state, cache_k, cache_v, inv_freq, *, cache_k_sca
     zeros there.  A row without a place in the table or the cache is skipped and reported by `kernel_status`.
     The reference's dense caches are made by its test script (efficiency/test_timing_layer.py)."""
     lens, idx, table = infer_state.b_seq_len, infer_state.b_req_idx, infer_state.req_manager.req_to_token_indexs
-    try:
-        N, Hkv, D = shape = k.shape
-        k0, k1, k2 = k.stride()
-        v0, v1, v2 = v.stride()
-        ck0, ck1, ck2 = cache_k.stride()
-        cv0, cv1, cv2 = cache_v.stride()
-        table0, table1 = table.stride()
-        dtype, held, index = k.dtype, cache_k.dtype, k.get_device()
-        B = N if cu_new is None else cu_new.shape[0] - 1
-        rot = 2 * inv_freq.shape[0]
-        store = cache_k.shape
-        fine = (
-            index >= 0 and v.get_device() == index and cache_k.get_device() == index and cache_v.get_device() == index
-            and inv_freq.get_device() == index and lens.get_device() == index and idx.get_device() == index
-            and table.get_device() == index and dtype in _HALVES and v.dtype is dtype and cache_v.dtype is held
-            and (held is dtype and cache_k_scale is None and cache_v_scale is None
-                 or held is torch.int8 and _scales_fit(cache_k_scale, cache_v_scale, store, index))
-            and v.shape == shape and store[1:] == shape[1:] and cache_v.shape == store and k2 == v2 == ck2 == cv2 == table1 == 1
-            and D % 2 == 0 and 2 <= D <= 256 and rot <= D and Hkv > 0 and inv_freq.dtype is torch.float32
-            and lens.dtype is torch.int32 and idx.dtype is torch.int32 and table.dtype is torch.int32
-            and lens.shape == (B,) and idx.shape == (B,) and rope_layout in ROPE and q_out is None and inv_freq.stride() == (1,)
-            and lens.stride() == (1,) and idx.stride() == (1,)
-            and (q is None or q.shape[0] == N and q.shape[2] == D and q.dtype is dtype and q.get_device() == index and q.stride(2) == 1)
-            and (cu_new is None or cu_new.dtype is torch.int32 and cu_new.get_device() == index and cu_new.stride() == (1,))
-            and (pos_offset is None or pos_offset.dtype is torch.int32 and pos_offset.shape == (B,)
-                 and pos_offset.get_device() == index and pos_offset.stride() == (1,))
-            and not (torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or cache_k.requires_grad or
-                                                  cache_v.requires_grad or q is not None and q.requires_grad)))
-    except (AttributeError, TypeError, ValueError, IndexError):
-        fine = False
-    if not fine:
-        _check_append(k, v, lens, idx, table, cache_k, cache_v, inv_freq, cache_k_scale, cache_v_scale, q, q_out, cu_new, pos_offset,
-                      rope_layout)
+    if stream is None and rope_layout in ROPE:
+        done = _ordinary().append(k, v, lens, idx, table, cache_k, cache_v, inv_freq, cache_k_scale, cache_v_scale, q, q_out, cu_new,
+                                  pos_offset, ROPE[rope_layout])
+        if done is not None:
+            return None if _done(done, "wsvd_kv_rope_append") is True else done
+    _check_append(k, v, lens, idx, table, cache_k, cache_v, inv_freq, cache_k_scale, cache_v_scale, q, q_out, cu_new, pos_offset,
+                  rope_layout)
+    N, Hkv, D = k.shape
+    dtype, held, index = k.dtype, cache_k.dtype, k.get_device()
+    B = N if cu_new is None else cu_new.shape[0] - 1
     own = q is not None and q_out is None
     if own:
         q_out = _new(torch.empty, q, q.shape, dtype, stream)
     code, i8 = _CODE[dtype], held is torch.int8
     args = _pack_append(
-        k.data_ptr(), k0, k1, v.data_ptr(), v0, v1,
+        k.data_ptr(), *k.stride()[:2], v.data_ptr(), *v.stride()[:2],
         *((0, 0, 0, 0, 0, 0) if q is None else (q.data_ptr(), *q.stride()[:2], q_out.data_ptr(), *q_out.stride()[:2])),
-        cache_k.data_ptr(), ck0, ck1, cache_v.data_ptr(), cv0, cv1,
+        cache_k.data_ptr(), *cache_k.stride()[:2], cache_v.data_ptr(), *cache_v.stride()[:2],
         *((cache_k_scale.data_ptr(), *cache_k_scale.stride(), cache_v_scale.data_ptr(), *cache_v_scale.stride()) if i8 else
           (0, 0, 0, 0, 0, 0)),
-        inv_freq.data_ptr(), table.data_ptr(), table0, idx.data_ptr(), lens.data_ptr(),
-        0 if cu_new is None else cu_new.data_ptr(), 0 if pos_offset is None else pos_offset.data_ptr(), store[0],
-        N, B, 0 if q is None else q.shape[1], Hkv, D, rot, table.shape[1], table.shape[0], code, I8 if i8 else code,
-        ROPE[rope_layout], own)
+        inv_freq.data_ptr(), table.data_ptr(), table.stride(0), idx.data_ptr(), lens.data_ptr(),
+        0 if cu_new is None else cu_new.data_ptr(), 0 if pos_offset is None else pos_offset.data_ptr(), cache_k.shape[0],
+        N, B, 0 if q is None else q.shape[1], Hkv, D, 2 * inv_freq.shape[0], table.shape[1], table.shape[0], code,
+        I8 if i8 else code, ROPE[rope_layout], own)
     _run("wsvd_kv_rope_append", index, stream, args)
     return q_out
 
@@ -709,31 +694,14 @@ def paged_decode(q, infer_state, cache_k, cache_v, k_scale=None, v_scale=None, *
     run at the same time need one each.  (`dense_decode` is the reference's f16 baseline.)"""
     lens, idx, table = infer_state.b_seq_len, infer_state.b_req_idx, infer_state.req_manager.req_to_token_indexs
     window = int(window)
-    try:
-        B, Hq, D = shape = q.shape
-        T, Hkv, _ = store = cache_k.shape
-        q0, q1, q2 = q.stride()
-        k0, k1, k2 = cache_k.stride()
-        v0, v1, v2 = cache_v.stride()
-        table0, table1 = table.stride()
-        dtype, held, index = q.dtype, cache_k.dtype, q.get_device()
-        fine = (
-            index >= 0 and cache_k.get_device() == index and cache_v.get_device() == index and lens.get_device() == index
-            and idx.get_device() == index and table.get_device() == index and dtype in _HALVES and cache_v.dtype is held
-            and (held is dtype and k_scale is None and v_scale is None
-                 or held is torch.int8 and _scales_fit(k_scale, v_scale, store, index))
-            and store[2] == D and cache_v.shape == store and q2 == k2 == v2 == table1 == 1 and 1 <= D <= 256
-            and Hkv > 0 and Hq > 0 and Hq % Hkv == 0 and lens.dtype is torch.int32 and idx.dtype is torch.int32
-            and table.dtype is torch.int32 and lens.shape == (B,) and idx.shape == (B,) and lens.stride() == (1,)
-            and idx.stride() == (1,) and window >= 0
-            and (out is None or out.shape == shape and out.dtype is dtype and out.get_device() == index and out.stride(2) == 1)
-            and (workspace is None or workspace.get_device() == index and workspace.is_contiguous())
-            and not (torch.is_grad_enabled() and (q.requires_grad or cache_k.requires_grad or cache_v.requires_grad or
-                                                  out is not None and out.requires_grad)))
-    except (AttributeError, TypeError, ValueError, IndexError):
-        fine = False
-    if not fine:
-        _check_paged(q, lens, idx, table, cache_k, cache_v, k_scale, v_scale, out, window, workspace)
+    if stream is None and alloc_tensor_func is torch.empty:
+        done = _ordinary().paged(q, lens, idx, table, cache_k, cache_v, k_scale, v_scale, out, workspace, return_lse, window,
+                                 float(sm_scale))
+        if done is not None:
+            return _done(done, "wsvd_paged_decode")
+    _check_paged(q, lens, idx, table, cache_k, cache_v, k_scale, v_scale, out, window, workspace)
+    B, Hq, D = shape = q.shape
+    Hkv, dtype, held, index = cache_k.shape[1], q.dtype, cache_k.dtype, q.get_device()
     if out is None:
         out = _new(alloc_tensor_func, q, shape, dtype, stream)
     lse = _new(alloc_tensor_func, q, (B, Hq), torch.float32, stream) if return_lse else None
@@ -743,13 +711,12 @@ def paged_decode(q, infer_state, cache_k, cache_v, k_scale=None, v_scale=None, *
     else:
         have = workspace.numel() * workspace.element_size()
     code, i8 = _CODE[dtype], held is torch.int8
-    out0, out1, _ = out.stride()
     args = _pack_paged(
-        q.data_ptr(), q0, q1, cache_k.data_ptr(), k0, k1, cache_v.data_ptr(), v0, v1,
+        q.data_ptr(), *q.stride()[:2], cache_k.data_ptr(), *cache_k.stride()[:2], cache_v.data_ptr(), *cache_v.stride()[:2],
         *((k_scale.data_ptr(), *k_scale.stride(), v_scale.data_ptr(), *v_scale.stride()) if i8 else (0, 0, 0, 0, 0, 0)),
-        table.data_ptr(), table0, idx.data_ptr(), lens.data_ptr(), out.data_ptr(), out0, out1,
-        0 if lse is None else lse.data_ptr(), T, B, Hq, Hkv, D, table.shape[1], table.shape[0], code, I8 if i8 else code,
-        min(window, 2 ** 31 - 1), float(sm_scale))
+        table.data_ptr(), table.stride(0), idx.data_ptr(), lens.data_ptr(), out.data_ptr(), *out.stride()[:2],
+        0 if lse is None else lse.data_ptr(), cache_k.shape[0], B, Hq, Hkv, D, table.shape[1], table.shape[0], code,
+        I8 if i8 else code, min(window, 2 ** 31 - 1), float(sm_scale))
     _run("wsvd_paged_decode", index, stream, args, workspace.data_ptr(), have)
     return (out, lse) if return_lse else out
 
@@ -817,31 +784,14 @@ def adapter_add(y, x, a, b, adapter, *, scale=None, cu_new=None, out=None, works
     the op's own has y's there.  An adapter that does not exist adds nothing and is reported by `kernel_status`.
     `workspace`: an optional CUDA buffer of `adapter_add_workspace_bytes` bytes; calls that may run at the same time need one
     each."""
-    try:
-        N, n_in = x.shape
-        count, _, rank = a.shape
-        n_out, B = y.shape[1], adapter.shape[0]
-        x0, x1 = x.stride()
-        y0, y1 = y.stride()
-        a0, a1, a2 = a.stride()
-        b0, b1, b2 = b.stride()
-        dtype, index = x.dtype, x.get_device()
-        fine = (
-            index >= 0 and y.get_device() == index and a.get_device() == index and b.get_device() == index
-            and adapter.get_device() == index and dtype in _HALVES and y.dtype is dtype and a.dtype is dtype
-            and b.dtype is dtype and adapter.dtype is torch.int32 and adapter.stride() == (1,) and y.shape == (N, n_out)
-            and a.shape[1] == n_in and b.shape == (count, rank, n_out) and 1 <= rank <= 256 and n_in > 0 and n_out > 0
-            and x1 == y1 == a2 == b2 == 1
-            and (scale is None or scale.dtype is torch.float32 and scale.shape == (count,) and scale.get_device() == index
-                 and scale.stride() == (1,))
-            and (B == N if cu_new is None else cu_new.dtype is torch.int32 and cu_new.shape == (B + 1,)
-                 and cu_new.get_device() == index and cu_new.stride() == (1,))
-            and (out is None or out is y) and (workspace is None or workspace.get_device() == index and workspace.is_contiguous())
-            and not (torch.is_grad_enabled() and (x.requires_grad or y.requires_grad or a.requires_grad or b.requires_grad)))
-    except (AttributeError, TypeError, ValueError, IndexError):
-        fine = False
-    if not fine:
-        _check_adapters(y, x, a, b, adapter, scale, cu_new, out, workspace)
+    if stream is None and alloc_tensor_func is torch.empty:
+        done = _ordinary().adapter(y, x, a, b, adapter, scale, cu_new, out, workspace)
+        if done is not None:
+            return _done(done, "wsvd_adapter_add")
+    _check_adapters(y, x, a, b, adapter, scale, cu_new, out, workspace)
+    N, n_in = x.shape
+    count, _, rank = a.shape
+    n_out, B, dtype, index = y.shape[1], adapter.shape[0], x.dtype, x.get_device()
     own = out is None
     if own:
         out = _new(alloc_tensor_func, y, (N, n_out), dtype, stream)
@@ -851,9 +801,9 @@ def adapter_add(y, x, a, b, adapter, *, scale=None, cu_new=None, out=None, works
     else:
         have = workspace.numel() * workspace.element_size()
     args = _pack_adapter(
-        y.data_ptr(), y0, x.data_ptr(), x0, a.data_ptr(), a0, a1, b.data_ptr(), b0, b1, out.data_ptr(), out.stride(0),
-        adapter.data_ptr(), 0 if scale is None else scale.data_ptr(), 0 if cu_new is None else cu_new.data_ptr(), N, B, n_in, n_out,
-        rank, count, _CODE[dtype], own)
+        y.data_ptr(), y.stride(0), x.data_ptr(), x.stride(0), a.data_ptr(), *a.stride()[:2], b.data_ptr(), *b.stride()[:2],
+        out.data_ptr(), out.stride(0), adapter.data_ptr(), 0 if scale is None else scale.data_ptr(),
+        0 if cu_new is None else cu_new.data_ptr(), N, B, n_in, n_out, rank, count, _CODE[dtype], own)
     _run("wsvd_adapter_add", index, stream, args, workspace.data_ptr(), have)
     return out
 
