@@ -56,52 +56,55 @@ __global__ void __launch_bounds__(256) expand_any_kernel(const __grid_constant__
 
 // ---- one row per request (a decode step): products on the CUDA cores, weights read once per four rows that share them
 //
-// Bound by the adapters' bytes.  Every row of the batch has its blocks; those of a row that is the first, fifth, ... of its
+// Bound by the adapters' bytes, and by latency: a block asks for its weights as soon as it knows its row's adapter, while it
+// finds out who shares it.  Every row of the batch has its blocks; those of a row that is the first, fifth, ... of its
 // adapter in the batch do the work for it and the next three, so that an adapter comes from memory once and from L2 once
 // per four rows, whatever the order of the requests.  The input's length is cut into slices over the blocks; the slices'
 // sums are added in a fixed order by the expanding blocks, which have asked for their weights before (they are launched
 // while the shrinking ones still run).
 constexpr int kStepRows = 4, kStepThreads = 128, kStepCols = 8 * kStepThreads, kMaxSlices = 64, kMaxSlice = 2048;
+constexpr int kStepLoads = 8;  // weights that a thread of the shrinking kernel asks for at once
 
-// The rows (at most four) that the blocks of row n work for: rows[0] = n; 0 where another row's blocks do, or there is no
-// adapter.  The first warp looks the batch over; all threads get the answer.
+// The rows (at most four) that the blocks of row n, with adapter `mine`, work for: rows[0] = n; count 0 where another row's
+// blocks do, or there is no adapter.  The first warp looks the batch over; all threads get the answer.
 struct Rows {
-  int count, adapter;
+  int count;
   int row[kStepRows];
 };
-__device__ __forceinline__ void rows_of(const WsvdAdapterAddParams& p, int n, Rows* sm) {
+__device__ __forceinline__ void rows_of(const WsvdAdapterAddParams& p, int n, int mine, Rows* sm) {
   if (threadIdx.x < 32) {
-    const int lane = threadIdx.x, mine = adapter_of(p, n);
-    int before = 0, count = 0, row[kStepRows] = {n, n, n, n};
-    if (mine >= 0) {
-      count = 1;
-      for (int j0 = 0; j0 < p.batch && count < kStepRows; j0 += 128) {
-        int a[4];
+    const int lane = threadIdx.x;
+    int before = 0, count = 1, r1 = n, r2 = n, r3 = n;
+    for (int j0 = 0; j0 < p.batch && count < kStepRows; j0 += 128) {
+      int a[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = j0 + 32 * i + lane;
-          a[i] = j < p.batch ? p.adapter[j] : -1;
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int j = j0 + 32 * i + lane;
+        a[i] = j < p.batch ? p.adapter[j] : -1;
+      }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int j = j0 + 32 * i;
-          unsigned same = __ballot_sync(0xffffffffu, a[i] == mine);
-          const unsigned up_to = n >= j + 31 ? 0xffffffffu : n < j ? 0u : (2u << (n - j)) - 1u;  // rows up to n
-          before += __popc(same & up_to);
-          same &= ~up_to;
-          while (same != 0 && count < kStepRows) {
-            row[count++] = j + __ffs(same) - 1;
-            same &= same - 1;
-          }
+      for (int i = 0; i < 4; ++i) {
+        const int j = j0 + 32 * i;
+        unsigned same = __ballot_sync(0xffffffffu, a[i] == mine);
+        const unsigned up_to = n >= j + 31 ? 0xffffffffu : n < j ? 0u : (2u << (n - j)) - 1u;  // rows up to n
+        before += __popc(same & up_to);
+        same &= ~up_to;
+        while (same != 0 && count < kStepRows) {
+          const int row = j + __ffs(same) - 1;
+          if (count == 1) r1 = row;
+          else if (count == 2) r2 = row;
+          else r3 = row;
+          ++count;
+          same &= same - 1;
         }
       }
-      if ((before - 1) % kStepRows != 0) count = 0;  // (`before` counts row n itself)
     }
     if (lane == 0) {
-      sm->count = count;
-      sm->adapter = mine;
-#pragma unroll
-      for (int i = 0; i < kStepRows; ++i) sm->row[i] = row[i];
+      sm->count = mine < 0 || (before - 1) % kStepRows != 0 ? 0 : count;  // (`before` counts row n itself)
+      sm->row[0] = n;
+      sm->row[1] = r1;
+      sm->row[2] = r2;
+      sm->row[3] = r3;
     }
   }
   __syncthreads();
@@ -130,20 +133,16 @@ __device__ __forceinline__ uint32_t both<__nv_bfloat16>(float x, float y) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// h[slice][row][r]: the sum over the slice's inputs.  A thread has four neighbouring ranks and every `lanes`-th input.
+// acc[row][4 ranks] += x w over the `n` loaded inputs; x of the slice's input i of row j is xs[i R + j]
 template <typename T, int R>
-__device__ __forceinline__ void step_products(const T* a, int64_t stride, int k0, int k1, int lanes, int kl, const float* xs, float (&acc)[kStepRows][4]) {
+__device__ __forceinline__ void step_products(const uint2 (&w)[kStepLoads], const float* xs, int lanes, int n, float (&acc)[kStepRows][4]) {
 #pragma unroll
-  for (int i = 0; i < R; ++i)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
-#pragma unroll 8
-  for (int k = k0 + kl; k < k1; k += lanes) {
-    const uint2 w = __ldg(reinterpret_cast<const uint2*>(a + (int64_t)k * stride));
-    const float2 lo = two<T>(w.x), hi = two<T>(w.y);
+  for (int l = 0; l < kStepLoads; ++l) {
+    if (l >= n) break;
+    const float2 lo = two<T>(w[l].x), hi = two<T>(w[l].y);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const float x = xs[(k - k0) * R + i];
+      const float x = xs[l * lanes * R + i];
       acc[i][0] = fmaf(x, lo.x, acc[i][0]);
       acc[i][1] = fmaf(x, lo.y, acc[i][1]);
       acc[i][2] = fmaf(x, hi.x, acc[i][2]);
@@ -152,6 +151,7 @@ __device__ __forceinline__ void step_products(const T* a, int64_t stride, int k0
   }
 }
 
+// h[slice][row][r]: the sum over the slice's inputs.  A thread has four neighbouring ranks and every `lanes`-th input.
 template <typename T>
 __global__ void __launch_bounds__(kStepThreads)
 shrink_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, float* h, const int slice) {
@@ -159,22 +159,43 @@ shrink_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, float* h, con
   __shared__ Rows rows;
   before_this();
   let_next_in();
-  rows_of(p, blockIdx.x, &rows);
-  const int count = rows.count, quads = p.rank / 4, lanes = kStepThreads / quads;
+  const int n = blockIdx.x, mine = adapter_of(p, n);
+  const int quads = p.rank / 4, lanes = kStepThreads / quads, kl = threadIdx.x / quads, quad = threadIdx.x - kl * quads;
+  const int k0 = blockIdx.y * slice, k1 = min(p.n_in, k0 + slice);
+  const T* a = reinterpret_cast<const T*>(p.a) + (mine >= 0 ? (int64_t)mine * p.a_stride_i : 0) + (int64_t)(k0 + kl) * p.a_stride_k + 4 * quad;
+  const int64_t skip = (int64_t)lanes * p.a_stride_k;
+  int left = mine >= 0 && kl < lanes && k0 + kl < k1 ? (k1 - k0 - kl + lanes - 1) / lanes : 0;  // this thread's inputs
+  uint2 w[kStepLoads];
+  auto load = [&]() {
+#pragma unroll
+    for (int l = 0; l < kStepLoads; ++l)
+      if (l < left) w[l] = __ldg(reinterpret_cast<const uint2*>(a + l * skip));
+  };
+  load();
+  rows_of(p, n, mine, &rows);
+  const int count = rows.count;
   if (count == 0) return;
   const int R = count == 1 ? 1 : count == 2 ? 2 : 4;
-  const int k0 = blockIdx.y * slice, k1 = min(p.n_in, k0 + slice), kl = threadIdx.x / quads, quad = threadIdx.x - kl * quads;
   for (int i = 0; i < R; ++i) {
     const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)rows.row[i] * p.x_stride;  // (a row that is not there: row n again)
+#pragma unroll 4
     for (int k = k0 + threadIdx.x; k < k1; k += kStepThreads) xs[(k - k0) * R + i] = wide(x[k]);
   }
   __syncthreads();
   float acc[kStepRows][4];
-  const T* a = reinterpret_cast<const T*>(p.a) + (int64_t)rows.adapter * p.a_stride_i + 4 * quad;
-  if (kl < lanes) {
-    if (R == 1) step_products<T, 1>(a, p.a_stride_k, k0, k1, lanes, kl, xs, acc);
-    else if (R == 2) step_products<T, 2>(a, p.a_stride_k, k0, k1, lanes, kl, xs, acc);
-    else step_products<T, 4>(a, p.a_stride_k, k0, k1, lanes, kl, xs, acc);
+#pragma unroll
+  for (int i = 0; i < kStepRows; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+  const float* x = xs + kl * R;
+  while (left > 0) {
+    if (R == 1) step_products<T, 1>(w, x, lanes, left, acc);
+    else if (R == 2) step_products<T, 2>(w, x, lanes, left, acc);
+    else step_products<T, 4>(w, x, lanes, left, acc);
+    left -= kStepLoads;
+    a += kStepLoads * skip;
+    x += kStepLoads * lanes * R;
+    load();
   }
   __syncthreads();
   if (kl < lanes) {
@@ -187,49 +208,62 @@ shrink_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, float* h, con
   for (int j = threadIdx.x; j < count * p.rank; j += kStepThreads) {
     const int i = j / p.rank, r = j - i * p.rank;
     float s = 0.f;
+#pragma unroll 4
     for (int l = 0; l < lanes; ++l) s += xs[(l * R + i) * p.rank + r];
     h[((int64_t)blockIdx.y * p.rows + rows.row[i]) * p.rank + r] = s;
   }
 }
 
 // out[row][8 columns a thread] of up to four rows
+constexpr int kStepAhead = 8;  // ranks whose weights are asked for before the shrinking kernel has ended
 template <typename T>
 __global__ void __launch_bounds__(kStepThreads)
 expand_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* h, const int slices) {
-  extern __shared__ __align__(16) float hs[];  // [rank][rows]
+  extern __shared__ __align__(16) float hs[];  // [rank][rows], then a sum a thread
   __shared__ Rows rows;
   // What is read before the wait is nothing that the shrinking kernel writes, and that one has waited for what is in front
   // of it before it let this one in.  (Without adapters it does not run.)
   if (p.n_adapters == 0) before_this();
-  rows_of(p, blockIdx.x, &rows);
-  const int col = (blockIdx.y * kStepThreads + threadIdx.x) * 8, count = rows.count;
+  const int n = blockIdx.x, mine = adapter_of(p, n), col = (blockIdx.y * kStepThreads + threadIdx.x) * 8;
   const bool on = col < p.n_out;
-  if (rows.adapter < 0) {  // no adapter: y goes through
+  if (mine < 0) {  // no adapter: y goes through
     before_this();
-    const int n = blockIdx.x;
     if (on)
       *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + (int64_t)n * p.out_stride + col) =
           *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.y) + (int64_t)n * p.y_stride + col);
     return;
   }
-  if (count == 0) {
-    before_this();  // (no block ends before the shrinking kernel has)
-    return;
-  }
-  const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)rows.adapter * p.b_stride_i + (on ? col : 0);
-  if (on && (threadIdx.x & 7) == 0)
-    for (int r = 0; r < p.rank; ++r) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(b + (int64_t)r * p.b_stride_r));
-  before_this();
-  for (int j = threadIdx.x; j < kStepRows * p.rank; j += kStepThreads) {
-    const int i = j / p.rank, r = j - i * p.rank;
+  const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)mine * p.b_stride_i + (on ? col : 0);
+  uint4 ahead[kStepAhead];
+#pragma unroll
+  for (int r = 0; r < kStepAhead; ++r)
+    if (r < p.rank) ahead[r] = __ldg(reinterpret_cast<const uint4*>(b + (int64_t)r * p.b_stride_r));
+  if (on && (threadIdx.x & 7) == 0)  // (a line a thread)
+    for (int r = kStepAhead; r < p.rank; ++r) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(b + (int64_t)r * p.b_stride_r));
+  rows_of(p, n, mine, &rows);
+  const int count = rows.count;
+  before_this();  // (also where another row's blocks do the work: no block ends before the shrinking kernel has)
+  if (count == 0) return;
+  const float scale = p.scale != nullptr ? p.scale[mine] : 1.f;
+  // h: the slices' sums, dealt out to as many threads as there are, then theirs, always in the same order
+  const int sums = count * p.rank, shares = sums < kStepThreads ? kStepThreads / sums : 1;
+  for (int j = threadIdx.x; j < sums * shares; j += kStepThreads) {
+    const int share = j / sums, i = (j - share * sums) / p.rank, r = j - share * sums - i * p.rank;
+    const float* at = h + (int64_t)rows.row[i] * p.rank + r;
+    const int64_t skip = (int64_t)p.rows * p.rank;
     float s = 0.f;
-    if (i < count) {
-      const float* at = h + (int64_t)rows.row[i] * p.rank + r;
 #pragma unroll 8
-      for (int l = 0; l < slices; ++l) s += at[(int64_t)l * p.rows * p.rank];
-      if (p.scale != nullptr) s *= p.scale[rows.adapter];
+    for (int l = share; l < slices; l += shares) s += at[l * skip];
+    (shares == 1 ? hs[r * kStepRows + i] : hs[kStepRows * p.rank + j]) = shares == 1 ? s * scale : s;
+  }
+  if (shares > 1) {
+    __syncthreads();
+    for (int j = threadIdx.x; j < sums; j += kStepThreads) {
+      float s = 0.f;
+      for (int l = 0; l < shares; ++l) s += hs[kStepRows * p.rank + l * sums + j];
+      const int i = j / p.rank;
+      hs[(j - i * p.rank) * kStepRows + i] = s * scale;
     }
-    hs[r * kStepRows + i] = s;
   }
   __syncthreads();
   if (!on) return;
@@ -238,11 +272,9 @@ expand_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* 
   for (int i = 0; i < kStepRows; ++i)
 #pragma unroll
     for (int e = 0; e < 8; ++e) acc[i][e] = 0.f;
-  auto add = [&](auto rows_at_once) {
+  auto all = [&](auto rows_at_once) {
     constexpr int R = decltype(rows_at_once)::value;
-#pragma unroll 8
-    for (int r = 0; r < p.rank; ++r) {
-      const uint4 w = __ldg(reinterpret_cast<const uint4*>(b + (int64_t)r * p.b_stride_r));
+    auto add = [&](int r, const uint4& w) {
       const float4 f = *reinterpret_cast<const float4*>(hs + r * kStepRows);
       const float x[4] = {f.x, f.y, f.z, f.w};
       const uint32_t v[4] = {w.x, w.y, w.z, w.w};
@@ -255,11 +287,16 @@ expand_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* 
           acc[i][2 * e + 1] = fmaf(x[i], t.y, acc[i][2 * e + 1]);
         }
       }
-    }
+    };
+#pragma unroll
+    for (int r = 0; r < kStepAhead; ++r)
+      if (r < p.rank) add(r, ahead[r]);
+#pragma unroll 8
+    for (int r = kStepAhead; r < p.rank; ++r) add(r, __ldg(reinterpret_cast<const uint4*>(b + (int64_t)r * p.b_stride_r)));
   };
-  if (count == 1) add(std::integral_constant<int, 1>{});
-  else if (count == 2) add(std::integral_constant<int, 2>{});
-  else add(std::integral_constant<int, 4>{});
+  if (count == 1) all(std::integral_constant<int, 1>{});
+  else if (count == 2) all(std::integral_constant<int, 2>{});
+  else all(std::integral_constant<int, 4>{});
 #pragma unroll
   for (int i = 0; i < kStepRows; ++i) {
     if (i >= count) continue;
@@ -707,16 +744,13 @@ int rank_padded(int rank) {
 }
 int packed_tiles(const WsvdAdapterAddParams& p) { return p.rows / kTileRows + p.batch + 1; }
 int rank_16(const WsvdAdapterAddParams& p) { return (p.rank + 15) / 16 * 16; }
-// Steps: inputs of a slice, enough blocks for every SM to have several, slices of 64 to kMaxSlice inputs (of four rows in f32:
-// what fits shared memory).
+// Steps: inputs of a slice.  A thread of the shrinking kernel asks for kStepLoads inputs at once, and a slice is so many for each
+// of the block's lanes (64 rows, rank 32, 5120 inputs: 40 slices 24.9 us, 20 slices of 16 loads 26.2 us), but there are no
+// more than kMaxSlices, and none is longer than kMaxSlice (four rows of it in f32: what fits shared memory).
 int slice_of(const WsvdAdapterAddParams& p) {
-  const int64_t blocks = p.rows > 0 ? p.rows : 1;
-  int64_t slices = (148 * 8 + blocks - 1) / blocks;
-  const int64_t least = (p.n_in + kMaxSlice - 1) / kMaxSlice, most = (p.n_in + 63) / 64;
-  if (slices < least) slices = least;
-  if (slices > most) slices = most;
-  if (slices > kMaxSlices) slices = kMaxSlices;
-  return (int)(((p.n_in + slices - 1) / slices + 63) / 64 * 64);
+  const int lanes = kStepThreads / (p.rank < 4 ? 1 : p.rank / 4 > kStepThreads ? kStepThreads : p.rank / 4);
+  const int slice = lanes * kStepLoads, least = (p.n_in + kMaxSlices - 1) / kMaxSlices;
+  return slice < least ? least : slice > kMaxSlice ? kMaxSlice : slice;
 }
 int slices_of(const WsvdAdapterAddParams& p) { return (p.n_in + slice_of(p) - 1) / slice_of(p); }
 
@@ -730,7 +764,7 @@ cudaError_t launch_step(const WsvdAdapterAddParams& p, float* h, cudaStream_t s)
                                                         s, 1, p, h, slice);
   if (e != cudaSuccess) return e;
   return launch_overlapped(expand_step_kernel<T>, dim3(p.rows, (p.n_out + kStepCols - 1) / kStepCols), kStepThreads,
-                           (size_t)kStepRows * p.rank * sizeof(float), s, 1, p, (const float*)h, slices);
+                           ((size_t)kStepRows * p.rank + kStepThreads) * sizeof(float), s, 1, p, (const float*)h, slices);
 }
 
 // more than 48 KB of dynamic shared memory has to be asked for, once per kernel and device
