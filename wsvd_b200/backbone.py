@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import Dict, List, Optional, Tuple
 
 import torch
 
@@ -55,6 +55,19 @@ def rope_half(q: torch.Tensor, pos: torch.Tensor, theta: float) -> torch.Tensor:
     qf = q.float()
     a, b = qf[..., : D // 2], qf[..., D // 2:]
     return torch.cat([a * cos - b * sin, b * cos + a * sin], dim=-1).to(q.dtype)
+
+
+@dataclass
+class Adapters:
+    """Low-rank adapters of the requests of a batch, beside the shared projections of a step.
+
+    index [batch] int32: the adapter of each sequence (-1: none); layers: one dict per decoder layer, from the name of a
+    projection ("qkv": the joined query and K/V down-projections, "o", "up_gate", "down") to its factors (a [n, in, rank],
+    b [n, rank, out]); scale [n] f32: optional factor of each adapter."""
+
+    index: torch.Tensor
+    layers: List[Dict[str, Tuple[torch.Tensor, torch.Tensor]]]
+    scale: Optional[torch.Tensor] = None
 
 
 class _Layer:
@@ -171,10 +184,27 @@ class LatentDecoder:
         dist.all_gather_into_tensor(self.gathered, o, group=self.group)
         return self.gathered.permute(1, 0, 2, 3).reshape(self.batch, sp.heads * sp.head_dim)
 
+    @staticmethod
+    def _adapted(y, x, adapters, layer, name):
+        """y = x @ W with the batch's adapters of this projection added in place (ops.adapter_add)."""
+        factors = adapters.layers[layer].get(name) if adapters is not None else None
+        if factors is None:
+            return y
+        return ops.adapter_add(y, x, *factors, adapters.index, scale=adapters.scale, out=y)
+
     @torch.no_grad()
-    def step(self, x: torch.Tensor) -> torch.Tensor:
+    def step(self, x: torch.Tensor, adapters: Optional[Adapters] = None) -> torch.Tensor:
         """x [B, hidden] f16 -> [B, hidden]; appends one token per sequence to every layer's cache
-        at position `context` (the caller advances the lengths with `advance()`)."""
+        at position `context` (the caller advances the lengths with `advance()`).  `adapters`: low-rank
+        adapters of the batch's requests (on one GPU, with the fused element-wise kernels)."""
+        if adapters is not None:
+            if self.world > 1 or not self.fused_elementwise:
+                raise ValueError("adapters need one GPU and fused_elementwise=True")
+            if len(adapters.layers) != len(self.layers):
+                raise ValueError(f"adapters must have one dict per layer ({len(self.layers)}), got {len(adapters.layers)}")
+            for names in adapters.layers:
+                if not set(names) <= {"qkv", "o", "up_gate", "down"}:
+                    raise ValueError(f"unknown projections among {sorted(names)}: expected qkv, o, up_gate, down")
         sp = self.spec
         B, Hl = self.batch, self.local_heads
         if self.workspace is None:
@@ -195,9 +225,9 @@ class LatentDecoder:
         if self.world > 1:
             import torch.distributed as dist
         xn = ops.rms_norm(x) if fe else None  # later layers get theirs from the residual add of the FFN
-        for L in self.layers:
+        for i, L in enumerate(self.layers):
             if fe:
-                qkv = xn @ L.Wqkv  # [B, Hl*D | Hl*Rk | Hl*Rv]: the three outputs are column slices
+                qkv = self._adapted(xn @ L.Wqkv, xn, adapters, i, "qkv")  # [B, Hl*D | Hl*Rk | Hl*Rv]: the three outputs are column slices
                 nq, nk = Hl * sp.head_dim, Hl * sp.rank_k
                 q = ops.rope_half_(qkv[:, :nq].unflatten(1, (Hl, sp.head_dim)), pos, self.inv_freq)
                 xk = qkv[:, nq:nq + nk].unflatten(1, (Hl, sp.rank_k))
@@ -209,14 +239,15 @@ class LatentDecoder:
                 xv = (xn @ L.A_v).view(B, Hl, sp.rank_v)
             ops.latent_quant_append(xk, xv, self.before, L.lk, L.ks, L.lv, L.vs)
             o = self._attend(L, q)
-            a = o @ L.Wo
+            a = self._adapted(o @ L.Wo, o, adapters, i, "o")
             if self.o_proj == "row":
                 dist.all_reduce(a, group=self.group)
             if fe:
                 x, h = ops.add_rms_norm(x, a)  # residual add + the FFN's normalisation
-                ug = h @ L.Wug
+                ug = self._adapted(h @ L.Wug, h, adapters, i, "up_gate")
                 nf = L.Wup.shape[1]
-                f = ops.silu_mul(ug[:, :nf], ug[:, nf:]) @ L.Wdown
+                g = ops.silu_mul(ug[:, :nf], ug[:, nf:])
+                f = self._adapted(g @ L.Wdown, g, adapters, i, "down")
             else:
                 x = x + a
                 h = _rms_norm(x)
@@ -229,8 +260,8 @@ class LatentDecoder:
                 x = x + f
         return x
 
-    def capture(self, x: torch.Tensor):
-        """Capture `step(x)` followed by the length update in a CUDA graph.  The split plan is
+    def capture(self, x: torch.Tensor, adapters: Optional[Adapters] = None):
+        """Capture `step(x, adapters)` followed by the length update in a CUDA graph.  The split plan is
         made for the cache capacity, so one graph serves every later step.  With several ranks
         the head gather has to be the fused one with its epoch on the device
         (`PeerGather(device_epoch=True)`); the FFN's NCCL all-reduce is captured as it is.  Returns (graph, output tensor); replay
@@ -241,13 +272,13 @@ class LatentDecoder:
         side = torch.cuda.Stream(device=self.device)
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):  # warm-up: workspace, position table, cuBLAS handles
-            self.step(x)
+            self.step(x, adapters)
             self._advance_device()
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize(self.device)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            y = self.step(x)
+            y = self.step(x, adapters)
             self._advance_device(host=False)  # recorded, not run: the caller counts replays in self.context
         return graph, y
 
