@@ -356,6 +356,54 @@ def test_paged_scores_of_lowest_value_and_nan(D):
     assert torch.isnan(got[2]).all()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_paged_short_sequences_of_bytes_keep_the_scores(dtype):
+    """Sequences of one to three tokens, whose weights average nothing out: lse of one token is its score.  With the query as 24
+    bits the products are exact, so that a score is off by the query's half step, 2^-23 of its row's largest power of two, and
+    four roundings of f32.  lse is then r + log2(sum) of a reference r that may lie up to 16 (a factor 2^16) below the score: a
+    logarithm of 8 to 16 has steps of 2^-20, and so has the difference that went into the exponential (a half step, 2^-21); the
+    exponential and the sum are off by 2^-22 more.  In all 2^-20 + 2^-21 + 2^-22 < 2^-19 in base 2, which the first run of this test
+    (0.0447, off by 2^-21) showed to be missing from the bound."""
+    g = torch.Generator().manual_seed(31)
+    table, T = pages(64, 4, 2, g)
+    st = state([1] * 64, table)
+    q = randn(g, 64, 4, 128, dtype=dtype)
+    k, v = (torch.randint(-127, 128, (T, 2, 128), generator=g, dtype=torch.int8) for _ in range(2))
+    ks, vs = ((torch.rand(T, 2, generator=g) * 0.02 + 0.001).half() for _ in range(2))
+    _, lse = ops.paged_decode(q.cuda(), gpu(st), *(t.cuda() for t in (k, v, ks, vs)), return_lse=True)
+    lse = lse.cpu().double()
+    for b in range(64):
+        s = int(table[b, 0])
+        for h in range(4):
+            kk = k[s, h // 2].double() * ks[s, h // 2].double()
+            qq = q[b, h].double()
+            z = float(kk @ qq) / math.sqrt(128)
+            tol = (2.0 ** -23 * float(qq.abs().max()) * float(kk.abs().sum())) / math.sqrt(128) + 8 * 2.0 ** -24 * abs(z) + 2.0 ** -19 * math.log(2)
+            assert abs(float(lse[b, h]) - z) <= tol, (b, h, float(lse[b, h]) - z, tol)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("D", [128, 40])
+def test_paged_queries_that_are_not_numbers_stay_in_their_heads(D, i8, bad):
+    g = torch.Generator().manual_seed(32)
+    lens = [20, 700]
+    table, T = pages(2, 700, 4, g)
+    st = state(lens, table)
+    q = randn(g, 2, 8, D)
+    k, v = (torch.randint(-127, 128, (T, 2, D), generator=g, dtype=torch.int8) for _ in range(2)) if i8 else (randn(g, T, 2, D) for _ in range(2))
+    scales = [(torch.rand(T, 2, generator=g) * 0.02 + 0.001).half().cuda() for _ in range(2)] if i8 else []
+    args = (gpu(st), k.cuda(), v.cuda(), *scales)
+    want = ops.paged_decode(q.cuda(), *args).cpu()
+    q[0, 1, 3] = q[1, 6, D - 1] = bad
+    got, lse = ops.paged_decode(q.cuda(), *args, return_lse=True)
+    got, lse = got.cpu(), lse.cpu()
+    hit = torch.zeros(2, 8, dtype=torch.bool)
+    hit[0, 1] = hit[1, 6] = True
+    assert torch.equal(got[~hit], want[~hit]) and torch.isfinite(lse[~hit]).all()
+    assert torch.isnan(got[hit]).all()
+
+
 def test_paged_runs_are_bitwise_equal_and_take_a_workspace():
     g = torch.Generator().manual_seed(16)
     table, T = pages(3, 3000, 16, g)

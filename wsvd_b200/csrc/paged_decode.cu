@@ -119,9 +119,13 @@ __global__ void __launch_bounds__(kAnyWarps * 32) paged_decode_any_kernel(const 
 // as partial sums, which paged_merge_kernel joins in a fixed order.
 //
 // Weights go into the product as two 16-bit terms (17 bits of bf16, 22 of f16): the one rounding that is left is the
-// result's.  int8 rows become f16 exactly (a byte under the exponent of 1024); their queries are scaled by a power of two to
-// [1, 2) at the largest, which is exact, so that bf16 ones of any size fit f16; the running maximum is that of score times v
-// scale, so that the weights with the v scale in them stay at or below one.
+// result's.  int8 keys meet their queries as bytes: a query row is taken to 24 bits below its largest value (a power of two
+// times it, so that bf16 ones of any size fit) and split into three bytes, whose products with the keys' are exact; bf16
+// rows of more than FINE tokens do without the third, a rounding of the query at 2^-16 of its row's largest value, 20 times
+// below the steps of bf16 itself and averaged over the weights of the tokens (8 sequences of up to 32768: 69 us, with the third byte
+// 77); f16 rows, whose own steps are no larger than that, keep it.  int8
+// values become f16 exactly (a byte under the exponent of 1024); the running maximum is that of score times v scale, so
+// that the weights with the v scale in them stay at or below one.
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 // bounds of the shares, for the workspace: CTAs of a GPU of so many SMs, CTAs of an item
@@ -222,7 +226,7 @@ struct Cfg {
   static constexpr int SLOT_BYTES = TOK * PITCH;                        // a ring slot: K or V rows of a step
   static constexpr int RING = kWarps * 4 * SLOT_BYTES;
   // CTAs of an SM that registers have to leave room for
-  static constexpr int CTAS = NT == 2 ? 2 : D <= 128 ? 3 : I8 ? 3 : 2;
+  static constexpr int CTAS = NT == 2 ? 2 : D <= 128 ? 3 : 2;
   // where a row's piece is, from the row's first byte (rows start on their own size where pieces change places)
   static __device__ __forceinline__ uint32_t at(int row, int piece) {
     return row * PITCH + (SWZ ? (piece ^ (row & 7)) * 16 : piece * 16);
@@ -233,6 +237,7 @@ struct Cfg {
   // The reference of the weights is a past maximum until one is 2^SLACK above it: sums are rescaled once or twice instead of
   // at every new maximum.  f16 weights are lifted so far that they use all of f16's range above one: 2^7 2^8 = 2^15, and
   // what is left of them below it is 2^-31 of the reference.
+  static constexpr int FINE = 512;
   static constexpr float SLACK = 8.f, LIFT = std::is_same<M, __half>::value ? 7.f : 0.f;
 };
 
@@ -446,7 +451,8 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
     request_v(my_ring + 3 * C::SLOT_BYTES);
 
     const float c = (p.sm_scale != 0.f ? p.sm_scale : rsqrtf((float)D)) * kLog2e;
-    uint32_t q[NT][D / 16][2];
+    uint32_t q[NT][D / 16][2], q_low[NT][C::I8 ? D / 32 : 1][2];
+    bool fine = false;
     float cq[NT][2], m[NT][2], l[NT][2], acc[D / 16][NT][4];
     const int steps = (int)(hi - lo);
     for (int step = 0; step < steps; ++step) {
@@ -459,8 +465,9 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
       if (now.flags & 1) {
         const Run run = ring_run[warp][step % META];
         const int in = run.it % chunks * hpi, h0 = run.hk * group + in, heads = min(hpi, group - in);
+        fine = std::is_same_v<T, __half> || run.tokens <= C::FINE;
         // queries as B operand: lane (head g, dims 2 c4, 2 c4 + 1 and + 8 of every 16; bytes: dims 4 c4 .. + 3 and + 16 of
-        // every 32, high bytes in the even entries, low ones in the odd)
+        // every 32, high bytes in the even entries, middle ones in the odd, low ones in q_low)
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
           const bool on = 8 * j + g < heads;
@@ -486,25 +493,29 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
             finite = (__ballot_sync(0xffffffffu, finite) >> (4 * g) & 15) == 15;
             // (the exponent of the largest; below 2^-100 all is as good as 0)
             const int e = amax > 0.f && finite ? max(-100, (__float_as_int(amax) >> 23) - 127) : 0;
-            const float up = power_of_two(14 - e);
+            const float up = power_of_two(22 - e);
 #pragma unroll
             for (int k = 0; k < D / 16; k += 2)
 #pragma unroll
               for (int t = 0; t < 2; ++t) {
                 const float2 f0 = unpack2<T>(q[j][k][t]), f1 = unpack2<T>(q[j][k + 1][t]);
-                const int v[4] = {__float2int_rn(f0.x * up), __float2int_rn(f0.y * up),
-                                  __float2int_rn(f1.x * up), __float2int_rn(f1.y * up)};
-                uint32_t high = 0, low = 0;
+                int v[4] = {__float2int_rn(f0.x * up), __float2int_rn(f0.y * up), __float2int_rn(f1.x * up), __float2int_rn(f1.y * up)};
+                if (!fine)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) v[i] = (v[i] + 128) & ~255;
+                uint32_t high = 0, mid = 0, low = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  high |= ((uint32_t)(v[i] >> 8) & 255u) << (8 * i);
+                  high |= ((uint32_t)(v[i] >> 16) & 255u) << (8 * i);
+                  mid |= ((uint32_t)(v[i] >> 8) & 255u) << (8 * i);
                   low |= ((uint32_t)v[i] & 255u) << (8 * i);
                 }
                 q[j][k][t] = high;
-                q[j][k + 1][t] = low;
+                q[j][k + 1][t] = mid;
+                q_low[j][k / 2][t] = low;
               }
             // the factor of head 8 j + g; this lane's columns are heads 2 c4 and 2 c4 + 1
-            const float f = finite ? c * power_of_two(e - 14) : NAN;
+            const float f = finite ? c * power_of_two(e - 22) : NAN;
             cq[j][0] = __shfl_sync(0xffffffffu, f, 8 * c4);
             cq[j][1] = __shfl_sync(0xffffffffu, f, 8 * c4 + 4);
           }
@@ -541,9 +552,22 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
 #pragma unroll
             for (int i = 0; i < 4; ++i) z[u][j][i] = SUMS == 1 ? part[u][j][0][i] : part[u][j][0][i] + part[u][j][SUMS - 1][i];
       } else {
-        int32_t high[C::SUBS][NT][4], low[C::SUBS][NT][4];
+        int32_t high[C::SUBS][NT][4], mid[C::SUBS][NT][4], low[C::SUBS][NT][4];
 #pragma unroll
-        for (int i = 0; i < C::SUBS * NT * 4; ++i) (&high[0][0][0])[i] = (&low[0][0][0])[i] = 0;
+        for (int i = 0; i < C::SUBS * NT * 4; ++i) (&high[0][0][0])[i] = (&mid[0][0][0])[i] = (&low[0][0][0])[i] = 0;
+        const auto third_byte = [&] {
+#pragma unroll
+          for (int k = 0; k < D / 16; k += 2)
+#pragma unroll
+            for (int u = 0; u < C::SUBS; ++u) {
+              uint32_t a[4];
+              ldmatrix4(a, C::skip(k_base + u * 16 * C::PITCH, k));
+#pragma unroll
+              for (int j = 0; j < NT; ++j) mma_s8_u8(low[u][j], a, q_low[j][k / 2][0], q_low[j][k / 2][1]);
+            }
+        };
+        // (before the others where registers are short: rows of 256, 128 us if it comes after, 103 so; rows of 128 69 and 78)
+        if (D > 128 && fine) third_byte();
 #pragma unroll
         for (int k = 0; k < D / 16; k += 2)
 #pragma unroll
@@ -553,15 +577,17 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
               mma_s8_s8(high[u][j], a, q[j][k][0], q[j][k][1]);
-              mma_s8_u8(low[u][j], a, q[j][k + 1][0], q[j][k + 1][1]);
+              mma_s8_u8(mid[u][j], a, q[j][k + 1][0], q[j][k + 1][1]);
             }
           }
+        if (D <= 128 && fine) third_byte();
 #pragma unroll
         for (int u = 0; u < C::SUBS; ++u)
 #pragma unroll
           for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) z[u][j][i] = (float)(high[u][j][i] * 256 + low[u][j][i]);  // (below 2^30)
+            for (int i = 0; i < 4; ++i)  // (each sum is below 2^23)
+              z[u][j][i] = fmaf((float)high[u][j][i], 65536.f, (float)(mid[u][j][i] * 256 + low[u][j][i]));
       }
 
       __syncwarp();
