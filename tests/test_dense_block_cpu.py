@@ -271,3 +271,41 @@ def test_the_oracle_leaves_out_what_does_not_exist():
     assert (out[2] == 0).all() and (lse[2] == -float("inf")).all()
     stored, turned = append64(k[:3], v[:3], q, state([1, 6, 0], table, idx=[0, 1, 5]), None, torch.ones(4), None, "half", T)
     assert not stored and len(turned) == 3
+
+
+def _bytes(T=None):
+    table, T = pages(2, 8, 4, torch.Generator().manual_seed(1))
+    store, scale = torch.zeros(T, 2, 16, dtype=torch.int8), torch.ones(T, 2, dtype=H16)
+    return dict(cache_k=store, cache_v=store.clone()), scale
+
+
+def test_gradients_of_the_small_arguments_are_refused_too():
+    caches, scale = _bytes()
+    wanted = scale.clone().requires_grad_()
+    calls = [("append", _append, dict(inv_freq=torch.ones(8, requires_grad=True))),
+             ("append", _append, dict(**caches, cache_k_scale=wanted, cache_v_scale=scale)),
+             ("paged", _paged, dict(**caches, k_scale=scale, v_scale=wanted)),
+             ("adapter", _adapters, dict(scale=torch.ones(2, requires_grad=True)))]
+    for op, call, kw in calls:
+        assert not getattr(_lib.bind(), op + "_fits")(*_bind_args(op, kw))
+        with pytest.raises(ValueError, match="no backward"):
+            call(**kw)()
+
+
+def test_outputs_whose_elements_share_memory_are_refused():
+    caches, scale = _bytes()
+    T = scale.shape[0]
+    calls = [("append", _append, dict(q=torch.zeros(2, 4, 16, dtype=H16), q_out=torch.zeros(1, 4, 16, dtype=H16).expand(2, 4, 16))),
+             ("append", _append, dict(cache_k=torch.zeros(T, 1, 16, dtype=H16).expand(T, 2, 16))),
+             ("append", _append, dict(**caches, cache_k_scale=scale, cache_v_scale=scale[:1].expand(T, 2))),
+             ("paged", _paged, dict(out=torch.zeros(2, 1, 16, dtype=H16).expand(2, 4, 16))),
+             ("adapter", _adapters, dict(out=torch.zeros(1, 24, dtype=H16).expand(3, 24))),
+             ("adapter", _adapters, dict(out=torch.zeros(72, dtype=H16).as_strided((3, 24), (16, 1))))]
+    for op, call, kw in calls:
+        assert not getattr(_lib.bind(), op + "_fits")(*_bind_args(op, kw))
+        with pytest.raises(ValueError, match="share memory"):
+            call(**kw)()
+    # heads outside, tokens inside, and K beside V in one buffer are as good as any order
+    both = torch.zeros(T, 2, 2, 16, dtype=H16)
+    for kw in (dict(cache_k=both[:, 0], cache_v=both[:, 1]), dict(cache_k=torch.zeros(2, T, 16, dtype=H16).transpose(0, 1))):
+        assert getattr(_lib.bind(), "append_fits")(*_bind_args("append", kw))

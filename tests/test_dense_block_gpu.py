@@ -486,6 +486,21 @@ def test_adapters_that_do_not_exist():
             assert ops.kernel_status() == 7
 
 
+@pytest.mark.parametrize("n_in", [64, 61])
+def test_adapters_rows_in_front_of_the_first_request(n_in):
+    """cu_new that begins behind row 0: those rows are padding like the ones behind."""
+    g = torch.Generator().manual_seed(33)
+    x, y = randn(g, 200, n_in), randn(g, 200, 48)
+    a, b = randn(g, 2, n_in, 8, scale=0.1).cuda(), randn(g, 2, 8, 48).cuda()
+    args = dict(cu_new=torch.tensor([70, 150, 151], dtype=torch.int32).cuda())
+    ad = torch.tensor([1, 0], dtype=torch.int32).cuda()
+    got = ops.adapter_add(y.cuda(), x.cuda(), a, b, ad, **args).cpu()
+    assert torch.equal(got[:70], y[:70]) and torch.equal(got[151:], y[151:])
+    mine = torch.full((200, 48), 7.0, dtype=F16, device="cuda")
+    kept = ops.adapter_add(y.cuda(), x.cuda(), a, b, ad, out=mine, **args).cpu()
+    assert (kept[:70] == 7).all() and (kept[151:] == 7).all() and torch.equal(kept[70:151], got[70:151])
+
+
 @pytest.mark.parametrize("n_in", [256, 33])
 def test_adapters_with_infinities_stay_in_their_rows(n_in):
     g = torch.Generator().manual_seed(5)
@@ -612,6 +627,69 @@ def test_two_graphs_and_an_eager_call_share_nothing():
         assert torch.equal(eager, runs[0][2])
         for _, out, want, *_ in runs:
             assert torch.equal(out, want)
+
+
+def test_calls_of_nothing_and_next_to_nothing():
+    """No rows, no sequences, no positions, no adapters, a table without columns."""
+    none = lambda *shape, dtype=F16: torch.zeros(*shape, dtype=dtype, device="cuda")  # noqa: E731
+    empty = gpu(state([], torch.zeros(0, 0, dtype=torch.int32)))
+    cache = none(0, 2, 64)
+    assert ops.paged_decode(none(0, 4, 64), empty, cache, cache).shape == (0, 4, 64)
+    assert ops.kv_rope_append(none(0, 2, 64), none(0, 2, 64), empty, none(8, 2, 64), none(8, 2, 64), none(32, dtype=torch.float32),
+                              q=none(0, 4, 64)).shape == (0, 4, 64)
+    for D in (64, 40):
+        for width, slots in ((0, 8), (4, 0)):
+            st = gpu(state([3, 0], torch.zeros(2, width, dtype=torch.int32)))
+            ck, cv = none(slots, 2, D), none(slots, 2, D)
+            out, lse = ops.paged_decode(randn(torch.Generator().manual_seed(1), 2, 4, D).cuda(), st, ck, cv, return_lse=True)
+            assert (out == 0).all() and (lse == -math.inf).all()
+            assert ops.kernel_status() in (5, 7)
+            ops.kv_rope_append(none(2, 2, D), none(2, 2, D), st, ck, cv, none(D // 2, dtype=torch.float32))
+            assert (ck == 0).all() and ops.kernel_status() in (5, 7)
+    y = randn(torch.Generator().manual_seed(2), 5, 48).cuda()
+    for n_in in (64, 61):
+        for cu in (None, torch.tensor([0, 2, 2, 4, 4, 4], dtype=torch.int32).cuda()):
+            got = ops.adapter_add(y, none(5, n_in), none(0, n_in, 8), none(0, 8, 48), torch.full((5,), -1, dtype=torch.int32, device="cuda"), cu_new=cu)
+            assert torch.equal(got, y)
+            assert ops.adapter_add(none(0, 48), none(0, n_in), none(2, n_in, 8), none(2, 8, 48), none(0, dtype=torch.int32),
+                                   cu_new=None if cu is None else none(1, dtype=torch.int32)).shape == (0, 48)
+
+
+@pytest.mark.parametrize("D", [64, 40])
+def test_paged_batches_of_tens_of_thousands(D):
+    """One token each: out is its value row (weight one, a rounding of a sum of one term)."""
+    g = torch.Generator().manual_seed(34)
+    B = 40000
+    q, k, v = randn(g, B, 2, D), randn(g, B, 1, D), randn(g, B, 1, D)
+    table = torch.randperm(B, generator=g).to(torch.int32)[:, None].contiguous()
+    got = ops.paged_decode(q.cuda(), gpu(state([1] * B, table)), k.cuda(), v.cuda()).cpu()
+    want = v[table[:, 0].long()].expand(B, 2, D)
+    assert ((got.double() - want.double()).abs() <= (2.0 ** -11 + 2.0 ** -17) * want.double().abs() + 2.0 ** -24).all()
+
+
+def test_two_streams_at_once():
+    """Calls that run side by side have workspaces of their own."""
+    g = torch.Generator().manual_seed(35)
+    lens = [9000, 20, 4000]
+    table, T = pages(3, 9000, 16, g)
+    st = gpu(state(lens, table))
+    k, v = randn(g, T, 2, 128).cuda(), randn(g, T, 2, 128).cuda()
+    qs = [randn(g, 3, 8, 128).cuda() for _ in range(2)]
+    x, y = randn(g, 3, 512).cuda(), randn(g, 3, 256).cuda()
+    a, b = randn(g, 2, 512, 16, scale=0.05).cuda(), randn(g, 2, 16, 256).cuda()
+    ads = [torch.tensor(t, dtype=torch.int32).cuda() for t in ([0, 1, 0], [1, -1, 1])]
+    want = [(ops.paged_decode(q, st, k, v), ops.adapter_add(y, x, a, b, ad)) for q, ad in zip(qs, ads)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((ops.paged_decode(qs[i], st, k, v), ops.adapter_add(y, x, a, b, ads[i])))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o, z in got[i]:
+            assert torch.equal(o, want[i][0]) and torch.equal(z, want[i][1])
 
 
 def test_ops_on_another_stream():

@@ -322,8 +322,8 @@ expand_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* 
 // in shared memory, 16-byte stores.
 constexpr int kTileRows = 64, kTileCols = 64, kPackThreads = 128, kColPieces = kTileCols / 8;
 
-// The row tiles of the batch, numbered through the requests in order; what is behind the last one counts as one more request
-// without an adapter where it is copied.  Every thread knows the tiles [before, before + mine) of its requests.
+// The row tiles of the batch, numbered through the requests in order; what is behind the last one and in front of the first
+// counts as two more requests without an adapter where it is copied.  Every thread knows the tiles [before, before + mine) of its requests.
 struct RowTile {
   int row, rows, adapter;  // rows 0: there is no such tile; adapter -1: none
 };
@@ -331,15 +331,16 @@ struct RowTiles {
   const WsvdAdapterAddParams& p;
   int b0, b1, before, mine, total;
 
-  // rows [*from, result) of request b, inside [0, rows) whatever cu_new says
+  // rows [*from, result) of request b, inside [0, rows) whatever cu_new says; behind the last request (copied rows) what is behind
+  // its rows, then what is in front of the first's
   __device__ __forceinline__ int span(int b, int* from) const {
-    *from = min(max(p.cu_new[b], 0), p.rows);
-    return b < p.batch ? max(*from, min(p.cu_new[b + 1], p.rows)) : p.rows;
+    *from = b > p.batch ? 0 : min(max(p.cu_new[b], 0), p.rows);
+    return b == p.batch ? p.rows : max(*from, min(p.cu_new[b > p.batch ? 0 : b + 1], p.rows));
   }
   __device__ __forceinline__ RowTiles(const WsvdAdapterAddParams& params) : p(params) {
     __shared__ int sums[kPackThreads / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int requests = p.batch + (p.copy_tail ? 1 : 0), per = (requests + kPackThreads - 1) / kPackThreads;
+    const int requests = p.batch + (p.copy_tail ? 2 : 0), per = (requests + kPackThreads - 1) / kPackThreads;
     b0 = min(requests, (int)threadIdx.x * per);
     b1 = min(requests, b0 + per);
     mine = 0;
@@ -742,7 +743,7 @@ int rank_padded(int rank) {
   while (r < rank) r *= 2;
   return r;
 }
-int packed_tiles(const WsvdAdapterAddParams& p) { return p.rows / kTileRows + p.batch + 1; }
+int packed_tiles(const WsvdAdapterAddParams& p) { return p.rows / kTileRows + p.batch + 2; }
 int rank_16(const WsvdAdapterAddParams& p) { return (p.rank + 15) / 16 * 16; }
 // Steps: inputs of a slice.  A thread of the shrinking kernel asks for kStepLoads inputs at once, and a slice is so many for each
 // of the block's lanes (64 rows, rank 32, 5120 inputs: 40 slices 24.9 us, 20 slices of 16 loads 26.2 us), but there are no
@@ -864,7 +865,7 @@ int wsvd_adapter_add(const WsvdAdapterAddParams* p, void* workspace, size_t work
   if (!p->cu_new && p->rows != p->batch) return WSVD_ERR_BAD_SHAPE;
   if ((p->n_out + 255) / 256 > 65535) return WSVD_ERR_TOO_LARGE;
   if (p->rows == 0) return WSVD_OK;
-  if (!p->y || !p->x || !p->out || !p->adapter) return WSVD_ERR_NULL_POINTER;
+  if (!p->y || !p->x || !p->out || (p->batch > 0 && !p->adapter)) return WSVD_ERR_NULL_POINTER;
   if (p->n_adapters > 0 && (!p->a || !p->b)) return WSVD_ERR_NULL_POINTER;
   if (!workspace) return WSVD_ERR_NULL_POINTER;
   if (workspace_bytes < wsvd_adapter_add_workspace_bytes(p)) return WSVD_ERR_WORKSPACE_TOO_SMALL;

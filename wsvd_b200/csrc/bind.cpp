@@ -55,6 +55,22 @@ bool differentiated(std::initializer_list<const Tensor*> ts) {
     if (t && t->requires_grad()) return true;
   return false;
 }
+// an output's elements have a place in memory each
+bool apart(const Tensor* t) {
+  if (!t || t->numel() == 0) return true;
+  int64_t order[3], dims = t->dim(), reach = 1;
+  for (int64_t i = 0; i < dims; ++i) {
+    int64_t j = i;
+    for (; j > 0 && t->stride(order[j - 1]) > t->stride(i); --j) order[j] = order[j - 1];
+    order[j] = i;
+  }
+  for (int64_t i = 0; i < dims; ++i) {
+    const int64_t size = t->size(order[i]), stride = t->stride(order[i]);
+    if (size > 1 && stride < reach) return false;
+    reach += stride * (size - 1);
+  }
+  return true;
+}
 int code(at::ScalarType t) { return t == at::kChar ? WSVD_I8 : t == at::kHalf ? WSVD_F16 : WSVD_BF16; }
 bool half(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 void* at_of(const Tensor* t) { return t ? t->data_ptr() : nullptr; }
@@ -99,7 +115,7 @@ struct Append {
            (q ? rows(q, 3, type, device) && q->size(0) == N && q->size(2) == D : !q_out) &&
            (!q_out || (rows(q_out, 3, type, device) && same_shape(*q, *q_out) &&
                        (q_out->data_ptr() != q->data_ptr() || q_out->strides() == q->strides()))) &&
-           !differentiated({k, v, q, q_out, ck, cv});
+           apart(q_out) && apart(ck) && apart(cv) && apart(ks) && apart(vs) && !differentiated({k, v, q, q_out, ck, cv, ks, vs, inv});
   }
 };
 
@@ -180,7 +196,7 @@ struct Paged {
     return rows(q, 3, type, device) && D >= 1 && D <= 256 && K > 0 && H > 0 && H % K == 0 && window >= 0 &&
            cache_fits(ck, cv, ks, vs, type, K, D, device) && metadata_fits(lens, idx, table, q->size(0), device) &&
            (!out || (rows(out, 3, type, device) && same_shape(*out, *q))) &&
-           (!workspace || (workspace->device() == device && workspace->is_contiguous())) && !differentiated({q, ck, cv, out});
+           (!workspace || (workspace->device() == device && workspace->is_contiguous())) && apart(out) && !differentiated({q, ck, cv, ks, vs, out});
   }
 };
 
@@ -256,7 +272,7 @@ struct Adapters {
            (cu ? vector(cu, B + 1, at::kInt, device) : B == N) &&
            (!out || (rows(out, 2, type, device) && same_shape(*out, *y) &&
                      (out->data_ptr() != y->data_ptr() || out->strides() == y->strides()))) &&
-           (!workspace || (workspace->device() == device && workspace->is_contiguous())) && !differentiated({x, y, a, b, out});
+           (!workspace || (workspace->device() == device && workspace->is_contiguous())) && apart(out) && !differentiated({x, y, a, b, scale, out});
   }
 };
 

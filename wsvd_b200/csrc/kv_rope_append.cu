@@ -381,15 +381,18 @@ extern "C" int wsvd_kv_rope_append(const WsvdKvRopeAppendParams* p, void* stream
   if (p->rope_layout != WSVD_ROPE_HALF && p->rope_layout != WSVD_ROPE_INTERLEAVED) return WSVD_ERR_BAD_DTYPE;
   if (!p->cu_new && p->rows != p->batch) return WSVD_ERR_BAD_SHAPE;
   if (p->rows == 0) return WSVD_OK;
-  if (!p->k || !p->v || !p->cache_k || !p->cache_v || !p->req_to_token || !p->b_req_idx || !p->b_seq_len)
-    return WSVD_ERR_NULL_POINTER;
+  if (!p->k || !p->v || (p->batch > 0 && (!p->b_req_idx || !p->b_seq_len))) return WSVD_ERR_NULL_POINTER;
+  const bool places = p->n_token_slots > 0 && p->n_req > 0 && p->max_len > 0;  // (else no row is stored)
+  if (places && (!p->cache_k || !p->cache_v || !p->req_to_token)) return WSVD_ERR_NULL_POINTER;
   if (p->rot_dim > 0 && !p->inv_freq) return WSVD_ERR_NULL_POINTER;
   if (p->n_q_heads > 0 && (!p->q || !p->q_out)) return WSVD_ERR_NULL_POINTER;
-  if (i8 && (!p->k_scale || !p->v_scale)) return WSVD_ERR_BAD_DTYPE;
+  if (i8 && places && (!p->k_scale || !p->v_scale)) return WSVD_ERR_BAD_DTYPE;
   if ((int64_t)p->rows * ((int64_t)p->n_q_heads + 2 * (int64_t)p->n_kv_heads) > (int64_t)1 << 32) return WSVD_ERR_TOO_LARGE;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const cudaError_t e = p->dtype == WSVD_F16 ? (i8 ? wsvd::launch_append<__half, true>(*p, s) : wsvd::launch_append<__half, false>(*p, s))
-                        : i8                 ? wsvd::launch_append<__nv_bfloat16, true>(*p, s)
-                                             : wsvd::launch_append<__nv_bfloat16, false>(*p, s);
+  WsvdKvRopeAppendParams call = *p;
+  if (!places) call.max_len = 0;
+  const cudaError_t e = p->dtype == WSVD_F16 ? (i8 ? wsvd::launch_append<__half, true>(call, s) : wsvd::launch_append<__half, false>(call, s))
+                        : i8                 ? wsvd::launch_append<__nv_bfloat16, true>(call, s)
+                                             : wsvd::launch_append<__nv_bfloat16, false>(call, s);
   return e == cudaSuccess ? WSVD_OK : wsvd::record_cuda_error(e);
 }

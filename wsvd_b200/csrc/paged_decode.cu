@@ -954,23 +954,27 @@ int wsvd_paged_decode(const WsvdPagedDecodeParams* p, void* workspace, size_t wo
   if (!i8 && p->cache_dtype != p->dtype) return WSVD_ERR_BAD_DTYPE;
   if (p->batch > 65535 || p->n_q_heads > 65535) return WSVD_ERR_TOO_LARGE;
   if (p->batch == 0) return WSVD_OK;
-  if (!p->q || !p->k || !p->v || !p->out || !p->req_to_token || !p->b_req_idx || !p->b_seq_len) return WSVD_ERR_NULL_POINTER;
-  if (i8 && (!p->k_scale || !p->v_scale)) return WSVD_ERR_BAD_DTYPE;
+  if (!p->q || !p->out || !p->b_req_idx || !p->b_seq_len) return WSVD_ERR_NULL_POINTER;
+  const bool places = p->n_token_slots > 0 && p->n_req > 0 && p->max_len > 0;  // (else no sequence has positions)
+  if (places && (!p->k || !p->v || !p->req_to_token)) return WSVD_ERR_NULL_POINTER;
+  if (i8 && places && (!p->k_scale || !p->v_scale)) return WSVD_ERR_BAD_DTYPE;
   const size_t need = wsvd_paged_decode_workspace_bytes(p);
   if (need > 0 && !workspace) return WSVD_ERR_NULL_POINTER;
   if (workspace_bytes < need) return WSVD_ERR_WORKSPACE_TOO_SMALL;
   if (need > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15) != 0) return WSVD_ERR_BAD_STRIDE;
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  WsvdPagedDecodeParams call = *p;
+  if (!places) call.max_len = 0;
   cudaError_t e;
-  if (wsvd::fits_tensor_cores(*p)) {
-    if (p->dtype == WSVD_F16)
-      e = i8 ? wsvd::launch_tensor_cores<__half, true>(*p, workspace, s) : wsvd::launch_tensor_cores<__half, false>(*p, workspace, s);
+  if (wsvd::fits_tensor_cores(call)) {
+    if (call.dtype == WSVD_F16)
+      e = i8 ? wsvd::launch_tensor_cores<__half, true>(call, workspace, s) : wsvd::launch_tensor_cores<__half, false>(call, workspace, s);
     else
-      e = i8 ? wsvd::launch_tensor_cores<__nv_bfloat16, true>(*p, workspace, s)
-             : wsvd::launch_tensor_cores<__nv_bfloat16, false>(*p, workspace, s);
+      e = i8 ? wsvd::launch_tensor_cores<__nv_bfloat16, true>(call, workspace, s)
+             : wsvd::launch_tensor_cores<__nv_bfloat16, false>(call, workspace, s);
   } else {
-    if (p->dtype == WSVD_F16) i8 ? wsvd::launch_any<__half, int8_t>(*p, s) : wsvd::launch_any<__half, __half>(*p, s);
-    else i8 ? wsvd::launch_any<__nv_bfloat16, int8_t>(*p, s) : wsvd::launch_any<__nv_bfloat16, __nv_bfloat16>(*p, s);
+    if (call.dtype == WSVD_F16) i8 ? wsvd::launch_any<__half, int8_t>(call, s) : wsvd::launch_any<__half, __half>(call, s);
+    else i8 ? wsvd::launch_any<__nv_bfloat16, int8_t>(call, s) : wsvd::launch_any<__nv_bfloat16, __nv_bfloat16>(call, s);
     e = cudaGetLastError();
   }
   return e == cudaSuccess ? WSVD_OK : wsvd::record_cuda_error(e);

@@ -494,6 +494,16 @@ def _tensor(name, t, dtypes, ndim, inner_contiguous=True):
         raise ValueError(f"{name}: innermost dimension must be contiguous")
 
 
+def _apart(name, t):
+    """An output's elements have a place in memory each."""
+    reach = 1
+    for stride, size in sorted(zip(t.stride(), t.shape)):
+        if size > 1 and t.numel() > 0:
+            if stride < reach:
+                raise ValueError(f"{name}: elements share memory (shape {tuple(t.shape)}, strides {t.stride()})")
+            reach += stride * (size - 1)
+
+
 def _on_one_gpu(**tensors):
     index = None
     for name, t in tensors.items():
@@ -593,9 +603,13 @@ def _check_append(k, v, lens, idx, table, cache_k, cache_v, inv_freq, cache_k_sc
                 raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
             if q_out.data_ptr() == q.data_ptr() and q_out.stride() != q.stride() and q.numel() > 0:
                 raise ValueError("q_out may be q itself, not another view of its storage")
+            _apart("q_out", q_out)
     elif q_out is not None:
         raise ValueError("q_out without q")
-    _no_gradient("kv_rope_append", k, v, q, q_out, cache_k, cache_v)
+    for name, t in (("cache_k", cache_k), ("cache_v", cache_v), ("cache_k_scale", cache_k_scale), ("cache_v_scale", cache_v_scale)):
+        if t is not None:
+            _apart(name, t)
+    _no_gradient("kv_rope_append", k, v, q, q_out, cache_k, cache_v, cache_k_scale, cache_v_scale, inv_freq)
     _on_one_gpu(k=k, v=v, q=q, q_out=q_out, cache_k=cache_k, cache_v=cache_v, cache_k_scale=cache_k_scale,
                 cache_v_scale=cache_v_scale, inv_freq=inv_freq, b_seq_len=lens, b_req_idx=idx, req_to_token_indexs=table,
                 cu_new=cu_new, pos_offset=pos_offset)
@@ -616,7 +630,8 @@ def kv_rope_append(k, v, infer_state, cache_k, cache_v, inv_freq, *, cache_k_sca
     `latent_quant_append`, on the rotated f32 row).  `q_out` may be q.
 
     Rows behind cu_new[B] are padding: nothing of them is stored, a `q_out` of the caller's keeps its rows, the op's own has
-    zeros there.  A row without a place in the table or the cache is skipped and reported by `kernel_status`.
+    zeros there.  A row without a place in the table or the cache is skipped and reported by `kernel_status`.  No two rows may
+    name the same slot.
     The reference's dense caches are made by its test script (efficiency/test_timing_layer.py)."""
     lens, idx, table = infer_state.b_seq_len, infer_state.b_req_idx, infer_state.req_manager.req_to_token_indexs
     if stream is None and rope_layout in ROPE:
@@ -670,11 +685,12 @@ def _check_paged(q, lens, idx, table, cache_k, cache_v, k_scale, v_scale, out, w
         _tensor("out", out, (q.dtype,), 3)
         if out.shape != q.shape:
             raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+        _apart("out", out)
     if window < 0:
         raise ValueError("window must not be negative")
     if workspace is not None and not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    _no_gradient("paged_decode", q, cache_k, cache_v, out)
+    _no_gradient("paged_decode", q, cache_k, cache_v, k_scale, v_scale, out)
     _on_one_gpu(q=q, cache_k=cache_k, cache_v=cache_v, k_scale=k_scale, v_scale=v_scale, b_seq_len=lens, b_req_idx=idx,
                 req_to_token_indexs=table, out=out, workspace=workspace)
 
@@ -766,9 +782,10 @@ def _check_adapters(y, x, a, b, adapter, scale, cu_new, out, workspace):
             raise ValueError(f"out must be {tuple(y.shape)}, got {tuple(out.shape)}")
         if out.data_ptr() == y.data_ptr() and out.stride() != y.stride() and y.numel() > 0:
             raise ValueError("out may be y itself, not another view of its storage")
+        _apart("out", out)
     if workspace is not None and not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    _no_gradient("adapter_add", y, x, a, b, out)
+    _no_gradient("adapter_add", y, x, a, b, scale, out)
     _on_one_gpu(x=x, y=y, a=a, b=b, adapter=adapter, scale=scale, cu_new=cu_new, out=out, workspace=workspace)
 
 
@@ -780,7 +797,7 @@ def adapter_add(y, x, a, b, adapter, *, scale=None, cu_new=None, out=None, works
     x [N, n_in], y [N, n_out] (the projection's result), a [n_adapters, n_in, rank], b [n_adapters, rank, n_out], all f16 or all
     bf16 (rows at any stride: y and out may be column slices); adapter [B] int32; scale [n_adapters] f32, None means
     1.  Rows are packed by request, `cu_new` [B + 1] int32 as in `kv_rope_append` (None: one row per request).  Returns
-    out; `out=y` adds in place.  x a is summed in f32.  Rows behind cu_new[B] are padding: a caller's `out` keeps its rows,
+    out; `out=y` adds in place.  x a is summed in f32 (and, of packed rows, rounded to their type).  Rows behind cu_new[B] are padding: a caller's `out` keeps its rows,
     the op's own has y's there.  An adapter that does not exist adds nothing and is reported by `kernel_status`.
     `workspace`: an optional CUDA buffer of `adapter_add_workspace_bytes` bytes; calls that may run at the same time need one
     each."""
