@@ -317,9 +317,11 @@ expand_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* 
 // Bound by x, y and out.  Shrink: a warp has 16 rows and all ranks, tiles of 64 inputs come by 16-byte asynchronous copies;
 // the input's length is cut into slices over the CTAs of a cluster, so that every SM has work, and their sums meet in
 // shared memory in a fixed order (left to the expanding CTAs in f32 they cost those 12 us).  h is rounded once to the 16-bit
-// type (a step of it is 2^-9 of the adapter's share of the result, which is rounded to that type itself).  Expand: equal shares of (tile, 128 columns) over the CTAs that the GPU
-// holds at once; a CTA keeps its tile's h, B's columns come from L2 and y's from memory a step ahead, y + product in place
-// in shared memory, 16-byte stores.
+// type (a step of it is 2^-9 of the adapter's share of the result, which is rounded to that type itself).  Expand: tiles of 128
+// rows, equal shares of (tile, 64 columns) over the CTAs that the GPU holds at once; a warp has 32 rows and, up to 64 ranks, keeps
+// their h in registers (what is in shared memory twice is what bounds it: 64-row tiles 97 us, 128 rows 92, with h in registers 89;
+// 256 threads, or a third stage and a CTA less on the SM, 100 and 104).  B's columns come from L2 and y's from memory a unit ahead,
+// y + product in place in shared memory, 16-byte stores.  6000 rows of 4096 to 11008, rank 64: 89 us, 4.6 TB/s of x, y and out.
 constexpr int kTileRows = 64, kTileCols = 64, kPackThreads = 128, kColPieces = kTileCols / 8;
 
 // The row tiles of the batch, numbered through the requests in order; what is behind the last one and in front of the first
@@ -327,6 +329,7 @@ constexpr int kTileRows = 64, kTileCols = 64, kPackThreads = 128, kColPieces = k
 struct RowTile {
   int row, rows, adapter;  // rows 0: there is no such tile; adapter -1: none
 };
+template <int ROWS>
 struct RowTiles {
   const WsvdAdapterAddParams& p;
   int b0, b1, before, mine, total;
@@ -347,7 +350,7 @@ struct RowTiles {
     for (int b = b0; b < b1; ++b) {
       int from;
       const int to = span(b, &from);
-      mine += (to - from + kTileRows - 1) / kTileRows;
+      mine += (to - from + ROWS - 1) / ROWS;
     }
     int incl = mine;
 #pragma unroll
@@ -373,15 +376,15 @@ struct RowTiles {
       int first = before;
       for (int b = b0; b < b1; ++b) {
         int from;
-        const int to = span(b, &from), n = (to - from + kTileRows - 1) / kTileRows;
+        const int to = span(b, &from), n = (to - from + ROWS - 1) / ROWS;
         if (t < first + n) {
-          const int row = from + (t - first) * kTileRows;
+          const int row = from + (t - first) * ROWS;
           int i = b < p.batch ? p.adapter[b] : -1;
           if (i < -1 || i >= p.n_adapters) {
             atomicMax(&g_status, kOutsideStorage);
             i = -1;
           }
-          tile = RowTile{row, min(kTileRows, to - row), i};
+          tile = RowTile{row, min(ROWS, to - row), i};
           break;
         }
         first += n;
@@ -446,7 +449,7 @@ shrink_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, T* h, const
   extern __shared__ __align__(16) unsigned char smem[];
   before_this();
   let_next_in();
-  const RowTiles tiles(p);
+  const RowTiles<kTileRows> tiles(p);
   if ((int)blockIdx.x >= tiles.total) return;
   const RowTile tile = tiles.find(blockIdx.x);
   if (tile.adapter < 0) return;
@@ -590,22 +593,24 @@ shrink_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, T* h, const
   cluster.sync();  // (nobody's shared memory goes while another reads it)
 }
 
+constexpr int kWideRows = 128, kWarpRows = kWideRows / (kPackThreads / 32), kMt = kWarpRows / 16;
 constexpr int kColPitch = kTileCols * 2 + 16;  // bytes of a tile row of B or y
-template <typename T>
-__global__ void __launch_bounds__(kPackThreads, 4)
+// HK: how many 16 ranks of h a warp keeps in registers (0: it reads them from shared memory again for every unit).
+template <typename T, int HK>
+__global__ void __launch_bounds__(kPackThreads, 3)
 expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const T* h, const int rp) {
   extern __shared__ __align__(16) unsigned char smem[];  // h [64][rp], then two stages of B [rp][128] and y [64][128]
   // (What is read before the wait is nothing that the shrinking kernel writes: see expand_step_kernel.)
   if (p.n_adapters == 0) before_this();
-  const RowTiles tiles(p);
+  const RowTiles<kWideRows> tiles(p);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c4 = lane & 3;
   const int blocks = (p.n_out + kTileCols - 1) / kTileCols;
   const int64_t units = (int64_t)tiles.total * blocks;
   const int shares = (int)min((int64_t)gridDim.x, units);
   int64_t unit = (int)blockIdx.x < shares ? share_begin(blockIdx.x, units, shares) : 0;
   const int64_t end = (int)blockIdx.x < shares ? share_begin(blockIdx.x + 1, units, shares) : 0;
-  const int h_pitch = rp * 2 + 16, b_bytes = rp * kColPitch, stage_bytes = b_bytes + kTileRows * kColPitch;
-  const uint32_t hd = smem_addr(smem), ring = hd + kTileRows * h_pitch;
+  const int h_pitch = rp * 2 + 16, b_bytes = rp * kColPitch, stage_bytes = b_bytes + kWideRows * kColPitch;
+  const uint32_t hd = smem_addr(smem), ring = hd + kWideRows * h_pitch;
   bool waited = p.n_adapters == 0;
   auto wait_once = [&]() {
     if (!waited) before_this();
@@ -633,8 +638,8 @@ expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const T* h,
     }
     const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)tile.adapter * p.b_stride_i;
     // a thread's pieces of a unit: one column, every so many rows of B and of the warp's own 16 of y
-    constexpr int BROWS = kPackThreads / kColPieces, YROWS = 32 / kColPieces, YN = 16 / YROWS;
-    const int col = (threadIdx.x % kColPieces) * 8, b_row = threadIdx.x / kColPieces, y_row = warp * 16 + lane / kColPieces;
+    constexpr int BROWS = kPackThreads / kColPieces, YROWS = 32 / kColPieces, YN = kWarpRows / YROWS;
+    const int col = (threadIdx.x % kColPieces) * 8, b_row = threadIdx.x / kColPieces, y_row = warp * kWarpRows + lane / kColPieces;
     const T* b_at = b + (int64_t)b_row * p.b_stride_r + c0 + col;
     const T* y_at = y + (int64_t)y_row * p.y_stride + c0 + col;
     T* out_at = out + (int64_t)y_row * p.out_stride + c0 + col;
@@ -667,50 +672,71 @@ expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const T* h,
     request(0);
     wait_once();
     const float scale = p.scale != nullptr ? p.scale[tile.adapter] : 1.f;
-    for (int i = threadIdx.x; i < kTileRows * (rp / 8); i += kPackThreads) {
+    for (int i = threadIdx.x; i < kWideRows * (rp / 8); i += kPackThreads) {
       const int row = i / (rp / 8), r = (i % (rp / 8)) * 8;
       const bool on = row < tile.rows;
       copy16(hd + row * h_pitch + r * 2, h + (on ? (int64_t)(tile.row + row) * rp + r : 0), on);
     }
     copies_commit();
+    const uint32_t ha = hd + (warp * kWarpRows + (lane & 15)) * h_pitch + (lane >> 4) * 16;
+    uint32_t hr[HK > 0 ? HK : 1][kMt][4];
     for (int step = 0; step < steps; ++step) {
       request(step + 1);
       copies_wait<1>();
       __syncthreads();
+      if (HK > 0 && step == 0) {
+#pragma unroll
+        for (int k = 0; k < HK; ++k)
+#pragma unroll
+          for (int i = 0; i < kMt; ++i) {
+            if (k < rp / 16) ldmatrix4(hr[k][i], ha + i * 16 * h_pitch + k * 32);
+            else hr[k][i][0] = hr[k][i][1] = hr[k][i][2] = hr[k][i][3] = 0;
+          }
+      }
       const uint32_t bd = ring + (step & 1) * stage_bytes;
       const uint32_t yt = bd + b_bytes;
-      float acc[kTileCols / 8][4];
+      float acc[kMt][kTileCols / 8][4];
 #pragma unroll
-      for (int j = 0; j < kTileCols / 8; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
-      const uint32_t ha = hd + (warp * 16 + (lane & 15)) * h_pitch + (lane >> 4) * 16;
+      for (int i = 0; i < kMt * kTileCols / 8 * 4; ++i) (&acc[0][0][0])[i] = 0.f;
       const uint32_t ba = bd + (lane & 15) * kColPitch + (lane >> 4) * 16;
-#pragma unroll 2
-      for (int k = 0; k < rp / 16; ++k) {
-        uint32_t hr[4], w[kTileCols / 16][4];
-        ldmatrix4(hr, ha + k * 32);
+      auto products = [&](int k, const uint32_t (&h16)[kMt][4]) {
+        uint32_t w[kTileCols / 16][4];
 #pragma unroll
         for (int j = 0; j < kTileCols / 16; ++j) ldmatrix4_trans(w[j], ba + k * 16 * kColPitch + j * 32);
 #pragma unroll
-        for (int j = 0; j < kTileCols / 16; ++j) {
-          mma<T>(acc[2 * j], hr, w[j][0], w[j][1]);
-          mma<T>(acc[2 * j + 1], hr, w[j][2], w[j][3]);
+        for (int j = 0; j < kTileCols / 16; ++j)
+#pragma unroll
+          for (int i = 0; i < kMt; ++i) {
+            mma<T>(acc[i][2 * j], h16[i], w[j][0], w[j][1]);
+            mma<T>(acc[i][2 * j + 1], h16[i], w[j][2], w[j][3]);
+          }
+      };
+      if constexpr (HK > 0) {
+#pragma unroll
+        for (int k = 0; k < HK; ++k)
+          if (k < rp / 16) products(k, hr[k]);
+      } else {
+#pragma unroll 2
+        for (int k = 0; k < rp / 16; ++k) {
+#pragma unroll
+          for (int i = 0; i < kMt; ++i) ldmatrix4(hr[0][i], ha + i * 16 * h_pitch + k * 32);
+          products(k, hr[0]);
         }
       }
       // y as the accumulators hold their values, 16 rows of 16 columns at a time, and back
-      const uint32_t ya = yt + (warp * 16 + (lane & 15)) * kColPitch + (lane >> 4) * 16;
+      const uint32_t ya = yt + (warp * kWarpRows + (lane & 15)) * kColPitch + (lane >> 4) * 16;
 #pragma unroll
-      for (int j = 0; j < kTileCols / 16; ++j) {
+      for (int ij = 0; ij < kMt * kTileCols / 16; ++ij) {
+        const int i = ij / (kTileCols / 16), j = ij % (kTileCols / 16);
         uint32_t v[4];  // rows 0-7 and 8-15 of columns 0-7, then of columns 8-15
-        ldmatrix4(v, ya + j * 32);
+        ldmatrix4(v, ya + i * 16 * kColPitch + j * 32);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 f = two<T>(v[e]);
-          const float* d = acc[2 * j + (e >> 1)] + 2 * (e & 1);
+          const float* d = acc[i][2 * j + (e >> 1)] + 2 * (e & 1);
           v[e] = both<T>(fmaf(scale, d[0], f.x), fmaf(scale, d[1], f.y));
         }
-        stmatrix4(ya + j * 32, v);
+        stmatrix4(ya + i * 16 * kColPitch + j * 32, v);
       }
       __syncwarp();  // the warp's rows are its own
       const uint32_t from = yt + y_row * kColPitch + col * 2;
@@ -794,6 +820,30 @@ cudaError_t launch_shrink(const WsvdAdapterAddParams& p, T* h, cudaStream_t s) {
   return launch_overlapped(shrink_packed_kernel<T, RP>, dim3(packed_tiles(p), slices), kPackThreads, smem, s, slices, p, h, slice, rank_16(p));
 }
 
+template <typename T, int HK>
+cudaError_t launch_expand(const WsvdAdapterAddParams& p, const T* h, cudaStream_t s) {
+  static bool ready[kMaxDevices];
+  const int rp = rank_16(p);
+  auto bytes = [](int r) { return (size_t)kWideRows * (r * 2 + 16) + 2 * ((size_t)r * kColPitch + kWideRows * kColPitch); };
+  cudaError_t e = allow_smem(expand_packed_kernel<T, HK>, ready, bytes(256));
+  if (e != cudaSuccess) return e;
+  // CTAs that the GPU holds at once, asked once per device and rank (what is written twice is the same)
+  int device = 0;
+  e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  static int resident[kMaxDevices][17];
+  int& fits = resident[device][rp / 16];
+  if (fits == 0) {
+    int per_sm = 0, sms = 0;
+    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, expand_packed_kernel<T, HK>, kPackThreads, bytes(rp));
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e != cudaSuccess) return e;
+    fits = per_sm * sms > 0 ? per_sm * sms : 1;
+  }
+  const int64_t units = (int64_t)packed_tiles(p) * ((p.n_out + kTileCols - 1) / kTileCols);
+  return launch_overlapped(expand_packed_kernel<T, HK>, dim3((unsigned)(units < fits ? units : fits)), kPackThreads, bytes(rp), s, 1, p, h, rp);
+}
+
 template <typename T>
 cudaError_t launch_packed(const WsvdAdapterAddParams& p, T* h, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
@@ -807,26 +857,7 @@ cudaError_t launch_packed(const WsvdAdapterAddParams& p, T* h, cudaStream_t s) {
     }
     if (e != cudaSuccess) return e;
   }
-  static bool ready[kMaxDevices];
-  const int rp = rank_16(p);
-  auto bytes = [](int r) { return (size_t)kTileRows * (r * 2 + 16) + 2 * ((size_t)r * kColPitch + kTileRows * kColPitch); };
-  e = allow_smem(expand_packed_kernel<T>, ready, bytes(256));
-  if (e != cudaSuccess) return e;
-  // CTAs that the GPU holds at once, asked once per device and rank (what is written twice is the same)
-  int device = 0;
-  e = cudaGetDevice(&device);
-  if (e != cudaSuccess) return e;
-  static int resident[kMaxDevices][17];
-  int& fits = resident[device][rp / 16];
-  if (fits == 0) {
-    int per_sm = 0, sms = 0;
-    e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, expand_packed_kernel<T>, kPackThreads, bytes(rp));
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    if (e != cudaSuccess) return e;
-    fits = per_sm * sms > 0 ? per_sm * sms : 1;
-  }
-  const int64_t units = (int64_t)packed_tiles(p) * ((p.n_out + kTileCols - 1) / kTileCols);
-  return launch_overlapped(expand_packed_kernel<T>, dim3((unsigned)(units < fits ? units : fits)), kPackThreads, bytes(rp), s, 1, p, (const T*)h, rp);
+  return p.rank <= 64 ? launch_expand<T, 4>(p, h, s) : launch_expand<T, 0>(p, h, s);
 }
 
 template <typename T>
