@@ -61,7 +61,9 @@ __global__ void __launch_bounds__(256) expand_any_kernel(const __grid_constant__
 // adapter in the batch do the work for it and the next three, so that an adapter comes from memory once and from L2 once
 // per four rows, whatever the order of the requests.  The input's length is cut into slices over the blocks; the slices'
 // sums are added in a fixed order by the expanding blocks, which have asked for their weights before (they are launched
-// while the shrinking ones still run).
+// while the shrinking ones still run).  Measured, a call: four rows of 4096 to 4096, rank 16: 8 us (two launches and their chains of
+// loads); 64 rows of 5120 to 15360, rank 32, 48 adapters: 24 us, 2.0 TB/s of weights: the slices' sums, half of the second
+// kernel, wait for the slowest slice.
 constexpr int kStepRows = 4, kStepThreads = 128, kStepCols = 8 * kStepThreads, kMaxSlices = 64, kMaxSlice = 2048;
 constexpr int kStepLoads = 8;  // weights that a thread of the shrinking kernel asks for at once
 
@@ -312,7 +314,7 @@ expand_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* 
   }
 }
 
-// ---- packed rows (prompts): products on the tensor cores, tiles of 64 rows of one request
+// ---- packed rows (prompts): products on the tensor cores, tiles of one request's rows (64 to shrink, 128 to expand)
 //
 // Bound by x, y and out.  Shrink: a warp has 16 rows and all ranks, tiles of 64 inputs come by 16-byte asynchronous copies;
 // the input's length is cut into slices over the CTAs of a cluster, so that every SM has work, and their sums meet in
@@ -321,7 +323,8 @@ expand_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* 
 // rows, equal shares of (tile, 64 columns) over the CTAs that the GPU holds at once; a warp has 32 rows and, up to 64 ranks, keeps
 // their h in registers (what is in shared memory twice is what bounds it: 64-row tiles 97 us, 128 rows 92, with h in registers 89;
 // 256 threads, or a third stage and a CTA less on the SM, 100 and 104).  B's columns come from L2 and y's from memory a unit ahead,
-// y + product in place in shared memory, 16-byte stores.  6000 rows of 4096 to 11008, rank 64: 89 us, 4.6 TB/s of x, y and out.
+// y + product in place in shared memory, 16-byte stores.  7095 rows of 4096 to 11008, rank 64: 89 us, 4.2 TB/s of
+// x, y and out (96 where the card is at its power limit).
 constexpr int kTileRows = 64, kTileCols = 64, kPackThreads = 128, kColPieces = kTileCols / 8;
 
 // The row tiles of the batch, numbered through the requests in order; what is behind the last one and in front of the first
@@ -599,7 +602,7 @@ constexpr int kColPitch = kTileCols * 2 + 16;  // bytes of a tile row of B or y
 template <typename T, int HK>
 __global__ void __launch_bounds__(kPackThreads, 3)
 expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const T* h, const int rp) {
-  extern __shared__ __align__(16) unsigned char smem[];  // h [64][rp], then two stages of B [rp][128] and y [64][128]
+  extern __shared__ __align__(16) unsigned char smem[];  // h [128][rp], then two stages of B [rp][64] and y [128][64]
   // (What is read before the wait is nothing that the shrinking kernel writes: see expand_step_kernel.)
   if (p.n_adapters == 0) before_this();
   const RowTiles<kWideRows> tiles(p);

@@ -8,6 +8,10 @@
 // The angle of a far position needs more than f32: at position 10^5 the f32 product is off by up to 0.004 radians, a bf16
 // rounding step.  It is taken in f64 (the product of an int32 and an f32 is exact there but for its last two bits), reduced
 // to [-pi, pi] with a two-term 2 pi, and only then handed to sincosf in f32.
+//
+// Memory bound: 14856 rows of prompts, 40 heads of 128, f16: 139 us, 6.57 TB/s read and written (a plain copy has that rate); into
+// bytes, 5665 rows of 8 KV heads and 32 queries: 33 us, 3.9 TB/s (a row's maximum has to be there before its first byte).  A step of up to 64 rows: 3 us, the
+// chain length -> page -> row.
 #include "dense_ops.cuh"
 
 namespace wsvd {
@@ -143,7 +147,8 @@ __global__ void __launch_bounds__(128) kv_append_any_kernel(const __grid_constan
 // computed once for all heads.  What a row's place is (up to four dependent loads) and the angles are worked out while the
 // block's vectors are on their way.
 constexpr int kVecThreads = 256;
-// from here on four units a thread (a block's set-up is paid for more data), below it one (more SMs at work)
+// From here on four units a thread (a block's set-up is paid for more data), below it one (more SMs at work).  (14856 rows of 40 heads:
+// 139 us with four, 178 with one; the kernel alone for 64 rows of 32 + 2 x 8 heads 4.7 and 3.2, for one row 4.1 and 3.1.)
 constexpr int64_t kManyUnits = 148 * 4 * kVecThreads * 4;
 
 struct Divisor {  // n / d for n < 2^31

@@ -118,6 +118,11 @@ __global__ void __launch_bounds__(kAnyWarps * 32) paged_decode_any_kernel(const 
 // (common.cuh), so that ragged batches load every SM alike; what several CTAs hold of one (sequence, head) they leave
 // as partial sums, which paged_merge_kernel joins in a fixed order.
 //
+// Measured, a call: 16 sequences of 4096, 40 heads of 128, f16: 212 us, 6.3 TB/s of cache (a plain copy: 6.56); 32 of 300 to 8192,
+// 32 heads on 8, bf16: 86 us, 5.7 TB/s; 48 in a window of 4096, heads of 64: 63 us, 5.3 TB/s; bytes, 8 of up to 32768: 69 to 75 us, 5.1
+// to 4.7 TB/s (bound by instructions: six matrix products a 16 tokens and 32 dims, values converted one by one); one of 2048: 14 us,
+// of which the page table, the rows and the merge wait for one another 10 (at other batches 4 us are the ends of the call).
+//
 // Weights go into the product as two 16-bit terms (17 bits of bf16, 22 of f16): the one rounding that is left is the
 // result's.  int8 keys meet their queries as bytes: a query row is taken to 24 bits below its largest value (a power of two
 // times it, so that bf16 ones of any size fit) and split into three bytes, whose products with the keys' are exact; bf16
@@ -128,7 +133,8 @@ __global__ void __launch_bounds__(kAnyWarps * 32) paged_decode_any_kernel(const 
 // that the weights with the v scale in them stay at or below one.
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-// bounds of the shares, for the workspace: CTAs of a GPU of so many SMs, CTAs of an item
+// bounds of the shares, for the workspace: CTAs of a GPU of so many SMs, CTAs of an item (one sequence of 60000 with one KV head:
+// 24 us with at most 128, 48 with all of the GPU's, whose partials one block has to join)
 constexpr int kMaxSms = 160, kMaxCtas = 4, kMaxParts = 128;
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -896,7 +902,8 @@ cudaError_t launch_fast(const WsvdPagedDecodeParams& p, const Items& it, const P
   if (grid < 1) grid = 1;
   e = launch_overlapped(paged_decode_kernel<C>, dim3((unsigned)grid), kThreads, (size_t)C::RING, s, 1, p, part, it);
   if (e != cudaSuccess || reach <= C::TOK) return e;  // (one warp an item and head: no partials)
-  // (an item has about grid / items + 1 CTAs: one round of loads for four warps, else many warps)
+  // An item has about grid / items + 1 CTAs: one round of loads for four warps, else many warps.  (48 sequences in a window: 62 us with
+  // four, 72 with sixteen; one sequence of 60000 with one KV head: 29 and 24.)
   const dim3 heads(p.n_q_heads, p.batch);
   if (grid * (kWarps / it.hw) <= 14 * items)
     return launch_overlapped(paged_merge_kernel<typename C::T, C::D, 4>, heads, 4 * 32, 0, s, 1, p, part, it);
