@@ -273,7 +273,7 @@ int wsvd_latent_quant_append_i8(const WsvdQuantAppendParams* p, void* stream);
  *
  * Rows behind cu_new[batch] are padding: nothing of them is stored (q_out: left as it was, or zeroed with clear_tail).  A row
  * whose position is outside [0, max_len) is skipped (status 5), one whose request or slot does not exist too
- * (status 7); its query is rotated all the same.  Two rows that name one slot leave either's values, head by head.
+ * (status 7); its query is rotated all the same.  No two rows may name one slot (what it then holds is not defined).
  * head_dim <= 256 and even, rot_dim even and <= head_dim.  No counterpart in the reference, whose dense caches are made
  * by its test script (efficiency/test_timing_layer.py).
  */
@@ -338,8 +338,10 @@ int wsvd_paged_decode(const WsvdPagedDecodeParams* p, void* workspace, size_t wo
  *   out[n] = y[n] + scale[i] (x[n] A_i) B_i,   i = adapter[request of row n]  (-1: out[n] = y[n])
  * y, out [rows, n_out], x [rows, n_in], A [n_adapters, n_in, rank], B [n_adapters, rank, n_out], all f16 or all bf16,
  * innermost stride 1; adapter [batch] int32; scale (optional) f32 [n_adapters].  Rows are packed by request, cu_new as
- * above (NULL: one row per request).  x A is summed in f32.  out may be y (same stride), and must not overlap x.
- * Rows behind cu_new[batch] are padding: left as they were, or copied from y with copy_tail.  An adapter outside [-1, n_adapters) adds nothing (status 7).  rank <= 256.
+ * above (NULL: one row per request).  x A is summed in f32 (packed rows: then
+ * rounded to their type).  out may be y (same stride), and must not overlap x.
+ * Rows behind cu_new[batch] are padding: left as they were, or copied from y with copy_tail.  An adapter outside
+ * [-1, n_adapters) adds nothing (status 7).  rank <= 256.
  */
 typedef struct WsvdAdapterAddParams {
   const void* y;            int64_t y_stride;

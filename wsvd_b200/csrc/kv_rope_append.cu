@@ -10,8 +10,8 @@
 // to [-pi, pi] with a two-term 2 pi, and only then handed to sincosf in f32.
 //
 // Memory bound: 14856 rows of prompts, 40 heads of 128, f16: 139 us, 6.57 TB/s read and written (a plain copy has that rate); into
-// bytes, 5665 rows of 8 KV heads and 32 queries: 33 us, 3.9 TB/s (a row's maximum has to be there before its first byte).  A step of up to 64 rows: 3 us, the
-// chain length -> page -> row.
+// bytes, 5665 rows of 8 KV heads and 32 queries: 33 us, 3.9 TB/s (a row's maximum has to be there before its first byte).  A step
+// of up to 64 rows: 3 us, the chain length -> page -> row.
 #include "dense_ops.cuh"
 
 namespace wsvd {
