@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from tests.dense_block import (adapters64, append64, assert_held, assert_rotated, attend64, half_step, pages, rotate64, rows_of,
+from tests.dense_block import (F32, adapters64, append64, assert_held, assert_rotated, attend64, half_step, pages, rotate64, rows_of,
                                state)
 from wsvd_b200 import ops
 
@@ -380,6 +380,27 @@ def test_paged_short_sequences_of_bytes_keep_the_scores(dtype):
             z = float(kk @ qq) / math.sqrt(128)
             tol = (2.0 ** -23 * float(qq.abs().max()) * float(kk.abs().sum())) / math.sqrt(128) + 8 * 2.0 ** -24 * abs(z) + 2.0 ** -19 * math.log(2)
             assert abs(float(lse[b, h]) - z) <= tol, (b, h, float(lse[b, h]) - z, tol)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_paged_sums_of_bytes_at_their_largest(D):
+    """Every key -128 and queries whose lower two bytes are all but full: the integer sums are at the ends of their range.  Each
+    product is exact, the sum is off by f32's roundings; all tokens weigh the same, so that out is their mean value."""
+    g = torch.Generator().manual_seed(36)
+    n = 45
+    table, T = pages(1, n, 8, g)
+    st = state([n], table)
+    q = torch.full((1, 2, D), 65504 * 2.0 ** -22, dtype=F16)
+    q[0, :, 5] = 1.0
+    q[0, 1] *= -1
+    k = torch.full((T, 1, D), -128, dtype=torch.int8)
+    v = torch.randint(-128, 128, (T, 1, D), generator=g, dtype=torch.int8)
+    ks, vs = torch.full((T, 1), 0.5).half(), torch.full((T, 1), 0.25).half()
+    out, lse = ops.paged_decode(q.cuda(), gpu(st), *(t.cuda() for t in (k, v, ks, vs)), return_lse=True)
+    z = (q[0].double().sum(1) * -64 / math.sqrt(D) + math.log(n)).unsqueeze(0)
+    assert ((lse.cpu().double() - z).abs() <= 2.0 ** -19 * math.log(2) + 8 * F32 * z.abs()).all()
+    mean = v[table[0].long(), 0].double().mean(0) * 0.25
+    assert ((out.cpu().double() - mean).abs() <= 2.0 ** -11 * mean.abs() + 2.0 ** -16 * 32).all()
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])

@@ -240,10 +240,10 @@ struct Cfg {
   // the address of the piece `more` (even) behind the one at `addr`: at(row, piece) + ... for piece 0 or 1
   static __device__ __forceinline__ uint32_t skip(uint32_t addr, int more) { return SWZ ? addr ^ (more * 16) : addr + more * 16; }
   static constexpr uint32_t FULL = TOK == 32 ? 0xffffffffu : 0xffffu;
+  static constexpr int FINE = 512;  // tokens of a sequence up to which bf16 queries meet bytes as 24 bits
   // The reference of the weights is a past maximum until one is 2^SLACK above it: sums are rescaled once or twice instead of
   // at every new maximum.  f16 weights are lifted so far that they use all of f16's range above one: 2^7 2^8 = 2^15, and
   // what is left of them below it is 2^-31 of the reference.
-  static constexpr int FINE = 512;
   static constexpr float SLACK = 8.f, LIFT = std::is_same<M, __half>::value ? 7.f : 0.f;
 };
 
