@@ -339,7 +339,7 @@ int wsvd_paged_decode(const WsvdPagedDecodeParams* p, void* workspace, size_t wo
  * y, out [rows, n_out], x [rows, n_in], A [n_adapters, n_in, rank], B [n_adapters, rank, n_out], all f16 or all bf16,
  * innermost stride 1; adapter [batch] int32; scale (optional) f32 [n_adapters].  Rows are packed by request, cu_new as
  * above (NULL: one row per request).  x A is summed in f32 (packed rows: then
- * rounded to their type).  out may be y (same stride), and must not overlap x.
+ * rounded to their type's number of bits, with the range of f32).  out may be y (same stride), and must not overlap x.
  * Rows behind cu_new[batch] are padding: left as they were, or copied from y with copy_tail.  An adapter outside
  * [-1, n_adapters) adds nothing (status 7).  rank <= 256.
  */

@@ -319,8 +319,7 @@ expand_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* 
 // Bound by x, y and out.  Shrink: a warp has 16 rows and all ranks, tiles of 64 inputs come by 16-byte asynchronous copies;
 // the input's length is cut into slices over the CTAs of a cluster, so that every SM has work, and their sums meet in
 // shared memory in a fixed order (left to the expanding CTAs in f32 they cost those 12 us).  h is rounded once to the 16-bit
-// type (a step of it is 2^-9 of the adapter's share of the result, which is rounded to that type itself).  Expand: tiles of 128
-// rows, equal shares of (tile, 64 columns) over the CTAs that the GPU holds at once; a warp has 32 rows and, up to 64 ranks, keeps
+// type (PackedH, below).  Expand: tiles of 128 rows, equal shares of (tile, 64 columns) over the CTAs that the GPU holds at once; a warp has 32 rows and, up to 64 ranks, keeps
 // their h in registers (what is in shared memory twice is what bounds it: 64-row tiles 97 us, 128 rows 92, with h in registers 89;
 // 256 threads, or a third stage and a CTA less on the SM, 100 and 104).  B's columns come from L2 and y's from memory a unit ahead,
 // y + product in place in shared memory, 16-byte stores.  7095 rows of 4096 to 11008, rank 64: 89 us, 4.2 TB/s of
@@ -444,10 +443,22 @@ struct Shrink {
   static constexpr int STAGE = kTileRows * X_PITCH + K * A_PITCH;
   static constexpr int LD = RP + 4;  // of the warps' sums (four more words a row: no bank twice)
 };
-// h [rows][rp] in 16 bits: rp is the rank rounded up to 16.  The CTAs of a cluster (along y) have one tile and a slice each.
+// h of packed rows between the two kernels, rounded once to the rows' type.  x A has f32's range, which f16 has not: f16 rows are
+// stored times the power of two that brings their largest to 2^14 .. 2^15 (what is below it keeps all 11 bits down to 2^-28 of it).
+// Why 16 bits: the error against 64 bits is 2.15e-4 in f16 and 1.76e-3 in bf16 (an adapter's share of a third of y, rank 64), where the
+// result's own rounding is 2.08e-4 and 1.66e-3; a second 16-bit term takes that away for twice the products (7095 rows of
+// 4096 to 11008: rank 64 89 us and 106 with it, rank 128 146 and 186).
+template <typename T>
+struct PackedH {
+  T* rows;      // [rows][rp], rp: the rank rounded up to 16
+  float* back;  // [rows] the inverse of the row's factor, f16 only
+};
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+// The CTAs of a cluster (along y) have one tile and a slice each.
 template <typename T, int RP>
 __global__ void __launch_bounds__(kPackThreads)
-shrink_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, T* h, const int slice, const int rp) {
+shrink_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const PackedH<T> h, const int slice, const int rp) {
   using S = Shrink<RP>;
   extern __shared__ __align__(16) unsigned char smem[];
   before_this();
@@ -578,20 +589,45 @@ shrink_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, T* h, const
   const auto cluster = cooperative_groups::this_cluster();
   cluster.sync();
   const int slices = cluster.num_blocks(), part = kTileRows / slices, from = (int)cluster.block_rank() * part;
-  for (int i = threadIdx.x; i < part * (rp / 2); i += kPackThreads) {
-    const int row = from + i / (rp / 2), r = (i % (rp / 2)) * 2;
-    if (row >= tile.rows) continue;
-    float2 w[8];
+  // G lanes a row, PAIRS pairs of ranks a lane
+  constexpr int G = RP / 2 < 32 ? RP / 2 : 32, PAIRS = RP / 2 / G, ROWS = kPackThreads / G;
+  const int member = threadIdx.x % G;
+  for (int row0 = 0; row0 < part; row0 += ROWS) {
+    const int in_part = row0 + threadIdx.x / G, row = from + in_part;
+    const bool on = in_part < part && row < tile.rows;
+    float2 v[PAIRS];
+    float amax = 0.f;
 #pragma unroll
-    for (int c = 0; c < 8; ++c)  // (all loads in flight)
-      w[c] = c < slices ? *reinterpret_cast<const float2*>(cluster.map_shared_rank(sums, c) + row * S::LD + r) : make_float2(0.f, 0.f);
-    float2 v = w[0];
+    for (int j = 0; j < PAIRS; ++j) {
+      const int r = 2 * (member + j * G);
+      float2 w[8];
 #pragma unroll
-    for (int c = 1; c < 8; ++c) {
-      v.x += w[c].x;
-      v.y += w[c].y;
+      for (int c = 0; c < 8; ++c)  // (all loads in flight)
+        w[c] = on && r < rp && c < slices ? *reinterpret_cast<const float2*>(cluster.map_shared_rank(sums, c) + row * S::LD + r) : make_float2(0.f, 0.f);
+      v[j] = w[0];
+#pragma unroll
+      for (int c = 1; c < 8; ++c) {
+        v[j].x += w[c].x;
+        v[j].y += w[c].y;
+      }
+      if (isfinite(v[j].x)) amax = fmaxf(amax, fabsf(v[j].x));
+      if (isfinite(v[j].y)) amax = fmaxf(amax, fabsf(v[j].y));
     }
-    *reinterpret_cast<uint32_t*>(h + (int64_t)(tile.row + row) * rp + r) = both<T>(v.x, v.y);  // (ranks up to rp: zeros)
+    float up = 1.f;
+    if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+      for (int o = 1; o < G; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      // (a sum of products of f16 values is 0 or a multiple of 2^-48 below 2^63)
+      const int e = amax > 0.f ? (__float_as_int(amax) >> 23) - 127 - 14 : 0;
+      up = power_of_two(-e);
+      if (on && member == 0) h.back[tile.row + row] = power_of_two(e);
+    }
+#pragma unroll
+    for (int j = 0; j < PAIRS; ++j) {
+      const int r = 2 * (member + j * G);
+      if (on && r < rp)  // (ranks up to rp: zeros)
+        *reinterpret_cast<uint32_t*>(h.rows + (int64_t)(tile.row + row) * rp + r) = both<T>(v[j].x * up, v[j].y * up);
+    }
   }
   cluster.sync();  // (nobody's shared memory goes while another reads it)
 }
@@ -601,12 +637,12 @@ constexpr int kColPitch = kTileCols * 2 + 16;  // bytes of a tile row of B or y
 // HK: how many 16 ranks of h a warp keeps in registers (0: it reads them from shared memory again for every unit).
 template <typename T, int HK>
 __global__ void __launch_bounds__(kPackThreads, 3)
-expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const T* h, const int rp) {
+expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const PackedH<T> h, const int rp) {
   extern __shared__ __align__(16) unsigned char smem[];  // h [128][rp], then two stages of B [rp][64] and y [128][64]
   // (What is read before the wait is nothing that the shrinking kernel writes: see expand_step_kernel.)
   if (p.n_adapters == 0) before_this();
   const RowTiles<kWideRows> tiles(p);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c4 = lane & 3;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2;
   const int blocks = (p.n_out + kTileCols - 1) / kTileCols;
   const int64_t units = (int64_t)tiles.total * blocks;
   const int shares = (int)min((int64_t)gridDim.x, units);
@@ -678,9 +714,17 @@ expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const T* h,
     for (int i = threadIdx.x; i < kWideRows * (rp / 8); i += kPackThreads) {
       const int row = i / (rp / 8), r = (i % (rp / 8)) * 8;
       const bool on = row < tile.rows;
-      copy16(hd + row * h_pitch + r * 2, h + (on ? (int64_t)(tile.row + row) * rp + r : 0), on);
+      copy16(hd + row * h_pitch + r * 2, h.rows + (on ? (int64_t)(tile.row + row) * rp + r : 0), on);
     }
     copies_commit();
+    float back[kMt][2];  // of rows g and g + 8 of every 16: the adapter's scale, and of f16 rows what their factor takes back
+#pragma unroll
+    for (int i = 0; i < kMt; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = warp * kWarpRows + 16 * i + 8 * e + g;
+        back[i][e] = std::is_same<T, __half>::value && row < tile.rows ? scale * __ldcg(h.back + tile.row + row) : scale;
+      }
     const uint32_t ha = hd + (warp * kWarpRows + (lane & 15)) * h_pitch + (lane >> 4) * 16;
     uint32_t hr[HK > 0 ? HK : 1][kMt][4];
     for (int step = 0; step < steps; ++step) {
@@ -737,7 +781,7 @@ expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const T* h,
         for (int e = 0; e < 4; ++e) {
           const float2 f = two<T>(v[e]);
           const float* d = acc[i][2 * j + (e >> 1)] + 2 * (e & 1);
-          v[e] = both<T>(fmaf(scale, d[0], f.x), fmaf(scale, d[1], f.y));
+          v[e] = both<T>(fmaf(back[i][e & 1], d[0], f.x), fmaf(back[i][e & 1], d[1], f.y));
         }
         stmatrix4(ya + i * 16 * kColPitch + j * 32, v);
       }
@@ -810,7 +854,7 @@ cudaError_t allow_smem(K kernel, bool (&ready)[kMaxDevices], size_t bytes) {
 }
 
 template <typename T, int RP>
-cudaError_t launch_shrink(const WsvdAdapterAddParams& p, T* h, cudaStream_t s) {
+cudaError_t launch_shrink(const WsvdAdapterAddParams& p, const PackedH<T>& h, cudaStream_t s) {
   using S = Shrink<RP>;
   static bool ready[kMaxDevices];
   constexpr size_t ring = (size_t)S::STAGES * S::STAGE, sums = (size_t)kTileRows * S::LD * sizeof(float), smem = ring > sums ? ring : sums;
@@ -824,7 +868,7 @@ cudaError_t launch_shrink(const WsvdAdapterAddParams& p, T* h, cudaStream_t s) {
 }
 
 template <typename T, int HK>
-cudaError_t launch_expand(const WsvdAdapterAddParams& p, const T* h, cudaStream_t s) {
+cudaError_t launch_expand(const WsvdAdapterAddParams& p, const PackedH<T>& h, cudaStream_t s) {
   static bool ready[kMaxDevices];
   const int rp = rank_16(p);
   auto bytes = [](int r) { return (size_t)kWideRows * (r * 2 + 16) + 2 * ((size_t)r * kColPitch + kWideRows * kColPitch); };
@@ -848,8 +892,9 @@ cudaError_t launch_expand(const WsvdAdapterAddParams& p, const T* h, cudaStream_
 }
 
 template <typename T>
-cudaError_t launch_packed(const WsvdAdapterAddParams& p, T* h, cudaStream_t s) {
+cudaError_t launch_packed(const WsvdAdapterAddParams& p, void* workspace, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
+  const PackedH<T> h{reinterpret_cast<T*>(workspace), reinterpret_cast<float*>(reinterpret_cast<T*>(workspace) + (int64_t)p.rows * rank_16(p))};
   if (p.n_adapters > 0) {
     switch (rank_padded(p.rank)) {
       case 16: e = launch_shrink<T, 16>(p, h, s); break;
@@ -866,7 +911,7 @@ cudaError_t launch_packed(const WsvdAdapterAddParams& p, T* h, cudaStream_t s) {
 template <typename T>
 cudaError_t launch_adapters(const WsvdAdapterAddParams& p, void* workspace, cudaStream_t s) {
   float* h = reinterpret_cast<float*>(workspace);
-  if (whole_vectors(p)) return p.cu_new != nullptr ? launch_packed<T>(p, reinterpret_cast<T*>(workspace), s) : launch_step<T>(p, h, s);
+  if (whole_vectors(p)) return p.cu_new != nullptr ? launch_packed<T>(p, workspace, s) : launch_step<T>(p, h, s);
   shrink_any_kernel<T><<<p.rows, 128, 0, s>>>(p, h);
   expand_any_kernel<T><<<dim3(p.rows, (p.n_out + 255) / 256), 256, 0, s>>>(p, h);
   return cudaGetLastError();
@@ -886,7 +931,7 @@ extern "C" {
 
 size_t wsvd_adapter_add_workspace_bytes(const WsvdAdapterAddParams* p) {
   if (!p || p->rows <= 0 || p->rank <= 0 || p->n_in <= 0 || p->batch < 0) return 0;
-  // packed rows: h in f32 or, its rows padded, in 16 bits; one row per request: a sum per slice of the input
+  // packed rows: h in f32 or, its rows padded, in 16 bits with a factor a row (the padding only to 16: no more); one row per request: a sum per slice of the input
   if (p->cu_new) return (size_t)p->rows * (p->rank < 16 ? 16 : p->rank) * sizeof(float);
   return (size_t)wsvd::slices_of(*p) * p->rows * p->rank * sizeof(float);
 }
