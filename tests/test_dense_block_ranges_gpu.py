@@ -5,8 +5,8 @@ import math
 import pytest
 import torch
 
-from tests.dense_block import F32, adapters64, half_step
-from tests.test_dense_block_gpu import randn, status_is_clean  # noqa: F401  (the fixture)
+from tests.dense_block import F32, adapters64, attend64, half_step, pages, quantize, state
+from tests.test_dense_block_gpu import gpu, randn, status_is_clean  # noqa: F401  (the fixture)
 from wsvd_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -98,3 +98,69 @@ def test_sums_of_single_rows_are_f32(dtype, n_in, n_out):
     assert ((y.double() + rounded - want).abs() > bound).double().mean() > 0.2  # the bound tells a 16-bit x A apart
     got = _adapters(y, x, a, b, ad)
     assert ((got.double() - want).abs() <= bound).all(), ((got.double() - want).abs() - bound).max().item()
+
+
+# ------------------------------------------------------------------ attention: bf16 queries on bytes
+
+def _coarse(q):
+    """Rows of q (f64) as 16-bit whole numbers of steps below the power of two of their largest."""
+    step = 2.0 ** (torch.floor(torch.log2(q.abs().amax(-1, keepdim=True))) - 14)
+    return (q / step).round() * step
+
+
+def _long_bytes(g, lens, H, K, D, outlier, dtype=BF16):
+    """Queries [B, H, D] (outlier: the size of one value of each row, whose keys are 0), keys of which one is along the mean of its
+    queries, so that it has nearly all the weight; (q, state, k, v, ks, vs)."""
+    table, T = pages(len(lens), max(lens), 16, g)
+    st = state(lens, table)
+    q = torch.randn(len(lens), H, D, generator=g)
+    k, v = torch.randn(T, K, D, generator=g), torch.randn(T, K, D, generator=g)
+    for b, n in enumerate(lens):
+        heads = q[b].view(K, H // K, D)
+        k[int(table[b, n // 3])] = 3.0 * heads.mean(1) * (H // K) ** 0.5
+    if outlier:
+        q[..., 5] = outlier
+        k[..., 5] = 0
+    (k, ks), (v, vs) = quantize(k.double()), quantize(v.double())
+    return q.to(dtype), st, k, v, ks, vs
+
+
+def _check_long_bytes(q, st, k, v, ks, vs):
+    want, lse, bound, lse_bound = attend64(q, st, k, v, ks, vs, 0, 0.0)
+    # a weight in f16 (two terms, lifted by 2^7): the last step of f16 is 2^-24, so it is off by up to 2^-25 2^-7 of the largest weight,
+    # where its own bits end.  Next to a weight of one that meets a value of zero, the others of 2^-36 each are below that.
+    values = (v.double() * vs.double()[..., None]).abs().max()
+    bound = bound + st.b_seq_len.double()[:, None, None] * 2.0 ** -32 * values
+    got, got_lse = ops.paged_decode(q.cuda(), gpu(st), k.cuda(), v.cuda(), ks.cuda(), vs.cuda(), return_lse=True)
+    off, off_lse = (got.cpu().double() - want).abs() - bound, (got_lse.cpu().double() - lse).abs() - lse_bound
+    assert (off_lse <= 0).all(), off_lse.max().item()
+    assert (off <= 0).all(), off.max().item()
+    return lse, lse_bound
+
+
+@pytest.mark.parametrize("H,K,D", [(8, 2, 128), (8, 1, 128), (16, 1, 128), (4, 4, 64), (8, 2, 256), (6, 2, 96)])
+@pytest.mark.parametrize("outlier", [24.0, 192.0])
+def test_bf16_queries_with_an_outlier_keep_the_scores_of_bytes(H, K, D, outlier):
+    """One value that is large against the others': at 16 bits below it the others' scores would be lost."""
+    g = torch.Generator().manual_seed(H + D)
+    case = _long_bytes(g, [511, 512, 513, 3001], H, K, D, outlier)
+    q, st = case[:2]
+    lse, lse_bound = _check_long_bytes(*case)
+    if outlier > 100:  # planted in the oracle, a query of 16 bits is beyond the bound
+        planted = attend64(_coarse(q.double()), st, *case[2:], 0, 0.0)[1]
+        assert ((planted - lse).abs() > lse_bound).any()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,K,D", [(8, 2, 128), (8, 1, 64), (16, 1, 128), (4, 1, 256)])
+def test_queries_on_bytes_of_long_sequences(dtype, H, K, D):
+    g = torch.Generator().manual_seed(H * D)
+    _check_long_bytes(*_long_bytes(g, [513, 5000, 700], H, K, D, 0.0, dtype))
+
+
+def test_an_outlier_in_one_head_of_a_group():
+    g = torch.Generator().manual_seed(12)
+    q, st, k, v, ks, vs = _long_bytes(g, [1500], 4, 1, 128, 0.0)
+    q[0, 2, 5] = 200.0
+    k[..., 5] = 0
+    _check_long_bytes(q, st, k, v, ks, vs)

@@ -125,10 +125,9 @@ __global__ void __launch_bounds__(kAnyWarps * 32) paged_decode_any_kernel(const 
 //
 // Weights go into the product as two 16-bit terms (17 bits of bf16, 22 of f16): the one rounding that is left is the
 // result's.  int8 keys meet their queries as bytes: a query row is taken to 24 bits below its largest value (a power of two
-// times it, so that bf16 ones of any size fit) and split into three bytes, whose products with the keys' are exact; bf16
-// rows of more than FINE tokens do without the third, a rounding of the query at 2^-16 of its row's largest value, 20 times
-// below the steps of bf16 itself and averaged over the weights of the tokens (8 sequences of up to 32768: 69 us, with the third byte
-// 77); f16 rows, whose own steps are no larger than that, keep it.  int8
+// times it, so that bf16 ones of any size fit) and split into three bytes, whose products with the keys' are exact.  (Two bytes
+// are 4 to 10 % less time where heads are of 256, 1 % where they are of 128, and lose the small values of a row beside one large one: scores
+// off by up to 0.01 where it is 200 times the others.)  int8
 // values become f16 exactly (a byte under the exponent of 1024); the running maximum is that of score times v scale, so
 // that the weights with the v scale in them stay at or below one.
 
@@ -240,7 +239,6 @@ struct Cfg {
   // the address of the piece `more` (even) behind the one at `addr`: at(row, piece) + ... for piece 0 or 1
   static __device__ __forceinline__ uint32_t skip(uint32_t addr, int more) { return SWZ ? addr ^ (more * 16) : addr + more * 16; }
   static constexpr uint32_t FULL = TOK == 32 ? 0xffffffffu : 0xffffu;
-  static constexpr int FINE = 512;  // tokens of a sequence up to which bf16 queries meet bytes as 24 bits
   // The reference of the weights is a past maximum until one is 2^SLACK above it: sums are rescaled once or twice instead of
   // at every new maximum.  f16 weights are lifted so far that they use all of f16's range above one: 2^7 2^8 = 2^15, and
   // what is left of them below it is 2^-31 of the reference.
@@ -458,7 +456,6 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
 
     const float c = (p.sm_scale != 0.f ? p.sm_scale : rsqrtf((float)D)) * kLog2e;
     uint32_t q[NT][D / 16][2], q_low[NT][C::I8 ? D / 32 : 1][2];
-    bool fine = false;
     float cq[NT][2], m[NT][2], l[NT][2], acc[D / 16][NT][4];
     const int steps = (int)(hi - lo);
     for (int step = 0; step < steps; ++step) {
@@ -471,7 +468,6 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
       if (now.flags & 1) {
         const Run run = ring_run[warp][step % META];
         const int in = run.it % chunks * hpi, h0 = run.hk * group + in, heads = min(hpi, group - in);
-        fine = std::is_same_v<T, __half> || run.tokens <= C::FINE;
         // queries as B operand: lane (head g, dims 2 c4, 2 c4 + 1 and + 8 of every 16; bytes: dims 4 c4 .. + 3 and + 16 of
         // every 32, high bytes in the even entries, middle ones in the odd, low ones in q_low)
 #pragma unroll
@@ -505,10 +501,7 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
 #pragma unroll
               for (int t = 0; t < 2; ++t) {
                 const float2 f0 = unpack2<T>(q[j][k][t]), f1 = unpack2<T>(q[j][k + 1][t]);
-                int v[4] = {__float2int_rn(f0.x * up), __float2int_rn(f0.y * up), __float2int_rn(f1.x * up), __float2int_rn(f1.y * up)};
-                if (!fine)
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) v[i] = (v[i] + 128) & ~255;
+                const int v[4] = {__float2int_rn(f0.x * up), __float2int_rn(f0.y * up), __float2int_rn(f1.x * up), __float2int_rn(f1.y * up)};
                 uint32_t high = 0, mid = 0, low = 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -561,19 +554,17 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
         int32_t high[C::SUBS][NT][4], mid[C::SUBS][NT][4], low[C::SUBS][NT][4];
 #pragma unroll
         for (int i = 0; i < C::SUBS * NT * 4; ++i) (&high[0][0][0])[i] = (&mid[0][0][0])[i] = (&low[0][0][0])[i] = 0;
-        const auto third_byte = [&] {
+        // the low bytes in a loop of their own (8 sequences of up to 32768: 69 us; in the one below, where three sums wait for one load,
+        // 77), in front of the others (behind them the registers of rows of 256 do not reach)
 #pragma unroll
-          for (int k = 0; k < D / 16; k += 2)
+        for (int k = 0; k < D / 16; k += 2)
 #pragma unroll
-            for (int u = 0; u < C::SUBS; ++u) {
-              uint32_t a[4];
-              ldmatrix4(a, C::skip(k_base + u * 16 * C::PITCH, k));
+          for (int u = 0; u < C::SUBS; ++u) {
+            uint32_t a[4];
+            ldmatrix4(a, C::skip(k_base + u * 16 * C::PITCH, k));
 #pragma unroll
-              for (int j = 0; j < NT; ++j) mma_s8_u8(low[u][j], a, q_low[j][k / 2][0], q_low[j][k / 2][1]);
-            }
-        };
-        // (before the others where registers are short: rows of 256, 128 us if it comes after, 103 so; rows of 128 69 and 78)
-        if (D > 128 && fine) third_byte();
+            for (int j = 0; j < NT; ++j) mma_s8_u8(low[u][j], a, q_low[j][k / 2][0], q_low[j][k / 2][1]);
+          }
 #pragma unroll
         for (int k = 0; k < D / 16; k += 2)
 #pragma unroll
@@ -586,7 +577,6 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
               mma_s8_u8(mid[u][j], a, q[j][k + 1][0], q[j][k + 1][1]);
             }
           }
-        if (D <= 128 && fine) third_byte();
 #pragma unroll
         for (int u = 0; u < C::SUBS; ++u)
 #pragma unroll
