@@ -1,4 +1,6 @@
 """Adapters of the batch's requests in the decode step (backbone.LatentDecoder.step)."""
+import gc
+
 import pytest
 import torch
 
@@ -77,3 +79,34 @@ def test_a_captured_step_with_adapters_replays_like_the_eager_one():
     torch.cuda.synchronize()
     err = (out.float() - want.float()).abs().max().item()
     assert err <= 2e-2 * want.float().abs().max().item()  # (another split plan: the graph's is made for the capacity)
+
+
+@pytest.mark.gpu
+def test_a_captured_step_keeps_what_it_reads():
+    """Input and adapters made inline: nothing else holds them when the graph is replayed and their memory is asked for again."""
+    start = (torch.randn(3, 512, generator=torch.Generator().manual_seed(6)) * 0.5).half().cuda()
+
+    def adapters():
+        return Adapters(torch.tensor([0, 1, -1], dtype=torch.int32).cuda(), _layers(2, 16, list(WIDTHS), "cuda"),
+                        torch.tensor([0.5, 2.0]).cuda())
+
+    held = adapters()
+    model = _model()
+    graph, want = model.capture(start, held)
+    graph.replay()
+    want = want.clone()
+
+    model = _model()
+    mine = adapters()
+    graph, got = model.capture(start.clone(), mine)
+    mine.layers[0]["qkv"] = None  # the container is the caller's; the graph keeps the tensors
+    del model, mine
+    gc.collect()
+    sizes = [t.shape for names in held.layers for pair in names.values() for t in pair] + [start.shape]
+    junk = [torch.full(s, float("nan"), dtype=torch.float16, device="cuda") for s in sizes * 3]
+    ints = [torch.full((3,), 1, dtype=torch.int32, device="cuda") for _ in range(8)]
+    floats = [torch.full((2,), float("nan"), device="cuda") for _ in range(8)]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    del junk, ints, floats

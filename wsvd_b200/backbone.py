@@ -265,7 +265,9 @@ class LatentDecoder:
         made for the cache capacity, so one graph serves every later step.  With several ranks
         the head gather has to be the fused one with its epoch on the device
         (`PeerGather(device_epoch=True)`); the FFN's NCCL all-reduce is captured as it is.  Returns (graph, output tensor); replay
-        with graph.replay() after writing the new input into x."""
+        with graph.replay() after writing the new input into x.  The graph holds on to what it reads: the model, x and
+        the adapters' tensors as they are now.  Other adapters, indices or scales are written into those (what is put in
+        their place in `adapters` afterwards is not seen by a replay)."""
         assert self.world == 1 or self.o_proj == "row" or (self.pg is not None and self.pg.device_epoch)
         self.before.max_len_in_batch = self.capacity
         self.after.max_len_in_batch = self.capacity
@@ -277,6 +279,8 @@ class LatentDecoder:
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize(self.device)
         graph = torch.cuda.CUDAGraph()
+        # (replays read them at their addresses, whoever else has let go of them)
+        graph.reads = (self, x) if adapters is None else (self, x, adapters.index, adapters.scale, [dict(names) for names in adapters.layers])
         with torch.cuda.graph(graph):
             y = self.step(x, adapters)
             self._advance_device(host=False)  # recorded, not run: the caller counts replays in self.context
