@@ -269,7 +269,7 @@ int wsvd_latent_quant_append_i8(const WsvdQuantAppendParams* p, void* stream);
  *   go through.  WSVD_ROPE_HALF pairs (j, j + rot_dim / 2), WSVD_ROPE_INTERLEAVED (2 j, 2 j + 1).
  *   cache_k, cache_v [T, Hkv, D]: the rows' dtype, or int8 with f16 scales [T, Hkv] per (slot, head): the quantiser of
  *   wsvd_latent_quant_append_i8 on the rotated f32 row.
- *   q_out [rows, Hq, D] receives the rotated queries; it may be q itself (same strides).
+ *   q_out [rows, Hq, D] receives the rotated queries; it may be q itself (same strides), and must not overlap q, k or v otherwise.
  *
  * Rows behind cu_new[batch] are padding: nothing of them is stored (q_out: left as it was, or zeroed with clear_tail).  A row
  * whose position is outside [0, max_len) is skipped (status 5), one whose request or slot does not exist too
@@ -309,7 +309,7 @@ int wsvd_kv_rope_append(const WsvdKvRopeAppendParams* p, void* stream);
  * exp(sm_scale q . k_s).  A sequence without positions gives zeros and -inf.
  * What is stored in slots that no position of the call names is never read.  A page-table entry outside [0, T) is left out
  * as if it were masked, a request outside the table leaves its sequence empty (status 7); a length beyond max_len is
- * clamped to it (status 5).
+ * clamped to it (status 5).  out may be q itself (same strides), and must not overlap q or the caches otherwise.
  * wsvd_dense_decode_f16 is the reference's dense baseline (f16, each query head for itself); this is the serving form.
  */
 typedef struct WsvdPagedDecodeParams {
@@ -339,7 +339,7 @@ int wsvd_paged_decode(const WsvdPagedDecodeParams* p, void* workspace, size_t wo
  * y, out [rows, n_out], x [rows, n_in], A [n_adapters, n_in, rank], B [n_adapters, rank, n_out], all f16 or all bf16,
  * innermost stride 1; adapter [batch] int32; scale (optional) f32 [n_adapters].  Rows are packed by request, cu_new as
  * above (NULL: one row per request).  x A is summed in f32 (packed rows: then
- * rounded to their type's number of bits, with the range of f32).  out may be y (same stride), and must not overlap x.
+ * rounded to their type's number of bits, with the range of f32).  out may be y (same stride), and must not overlap y, x, A or B otherwise.
  * Rows behind cu_new[batch] are padding: left as they were, or copied from y with copy_tail.  An adapter outside
  * [-1, n_adapters) adds nothing (status 7).  rank <= 256.
  */

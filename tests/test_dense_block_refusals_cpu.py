@@ -1,0 +1,117 @@
+"""What the dense attention block's operators refuse beyond tests/test_dense_block_cpu.py: both ways of a call, without a GPU."""
+import random
+
+import pytest
+import torch
+
+from tests.dense_block import pages
+from tests.test_dense_block_cpu import H16, _adapters, _append, _bind_args, _paged
+from wsvd_b200 import _lib, ops
+
+CALLS = {"append": _append, "paged": _paged, "adapter": _adapters}
+
+
+def refused(op, match, exc=ValueError, **kw):
+    assert not getattr(_lib.bind(), op + "_fits")(*_bind_args(op, kw))
+    with pytest.raises(exc, match=match):
+        CALLS[op](**kw)()
+
+
+def accepted(op, **kw):
+    """Nothing but the device is wrong with the call."""
+    assert getattr(_lib.bind(), op + "_fits")(*_bind_args(op, kw))
+    with pytest.raises(ValueError, match="must be a CUDA tensor"):
+        CALLS[op](**kw)()
+
+
+# ------------------------------------------------------------------ outputs over inputs
+
+def test_a_shifted_output_is_refused():
+    """y = buf[:-1], out = buf[1:]: blocks would write rows of y that others have yet to read."""
+    rows = torch.zeros(4, 24, dtype=H16)
+    refused("adapter", "out may be y itself", y=rows[:-1], out=rows[1:])
+    refused("adapter", "out may be y itself", y=rows[1:], out=rows[:-1])
+    flat = torch.zeros(3 * 24 + 8, dtype=H16)
+    refused("adapter", "out may be y itself", y=flat[:72].view(3, 24), out=flat[8:].view(3, 24))
+    tokens = torch.zeros(3, 4, 16, dtype=H16)
+    refused("append", "q_out may be q itself", q=tokens[:-1], q_out=tokens[1:])
+    refused("append", "q_out may be q itself", q=tokens[:2], q_out=tokens[:2].flatten().view(4, 2, 16).transpose(0, 1))
+    refused("paged", "out may be q itself", q=tokens[1:], out=tokens[:-1])
+
+
+def test_an_output_over_another_input_is_refused():
+    qkv = torch.zeros(2, 8 * 16, dtype=H16)
+    q, k, v = (qkv[:, a:b].unflatten(1, (-1, 16)) for a, b in ((0, 64), (64, 96), (96, 128)))
+    refused("append", "must not overlap k", q=q, k=k, v=v, q_out=qkv[:, 64:].unflatten(1, (-1, 16)))
+    refused("append", "must not overlap v", q=torch.zeros_like(q), v=v, q_out=qkv[:, 64:].unflatten(1, (-1, 16)))
+    x = torch.zeros(3, 16 + 24, dtype=H16)
+    refused("adapter", "must not overlap x", x=x[:, :16], out=x[:, 15:39])
+    a = torch.zeros(2, 16, 4, dtype=H16)
+    refused("adapter", "must not overlap a", a=a, out=a.flatten()[:72].view(3, 24))
+    b = torch.zeros(2, 4, 24, dtype=H16)
+    refused("adapter", "must not overlap b", b=b, out=b[1, 1:])
+    table, T = pages(2, 8, 4, torch.Generator().manual_seed(1))
+    cache = torch.zeros(T, 2, 16, dtype=H16)
+    for name in ("cache_k", "cache_v"):
+        refused("paged", "must not overlap " + name, out=cache[2:6].view(2, 4, 16), **{name: cache})
+
+
+def test_outputs_beside_inputs_in_one_buffer_are_served():
+    """Disjoint columns, heads or halves of one buffer, and an input itself."""
+    qkv = torch.zeros(2, 12 * 16, dtype=H16)
+    cut = [qkv[:, a * 16:b * 16].unflatten(1, (-1, 16)) for a, b in ((0, 4), (4, 6), (6, 8), (8, 12))]
+    accepted("append", q=cut[0], k=cut[1], v=cut[2], q_out=cut[3])
+    accepted("append", q=cut[0], k=cut[1], v=cut[2], q_out=cut[0])
+    by_head = torch.zeros(2, 2, 3, 16, dtype=H16)  # q, k and v of a head side by side
+    q, k, v = by_head.unbind(2)
+    accepted("append", q=q, k=k, v=v, q_out=q)
+    outside = torch.zeros(8, 2, 16, dtype=H16).transpose(0, 1)  # heads outside
+    accepted("append", q=outside[:, :4], k=outside[:, 4:6], v=outside[:, 6:], q_out=outside[:, :4])
+    both = torch.zeros(3, 48, dtype=H16)
+    accepted("adapter", y=both[:, :24], out=both[:, 24:])
+    accepted("adapter", y=both[:, :24], out=both[:, :24])
+    every = torch.zeros(6, 24, dtype=H16)
+    accepted("adapter", y=every[::2], out=every[1::2])
+    accepted("adapter", y=every[:3], out=every[3:])
+    one = torch.zeros(1, 64, dtype=H16)  # one row: its stride is nobody's
+    accepted("adapter", x=torch.zeros(1, 16, dtype=H16), adapter=torch.zeros(1, dtype=torch.int32), y=one[:, :24], out=one.as_strided((1, 24), (24, 1)))
+    q = torch.zeros(2, 4, 16, dtype=H16)
+    accepted("paged", q=q, out=q)
+
+
+def test_views_of_one_buffer_meet_where_their_elements_do():
+    rng = random.Random(7)
+    buf = torch.zeros(4000, dtype=H16)
+    where = torch.arange(4000)
+    met = 0
+    for _ in range(1500):
+        views = []
+        pitch = [rng.choice([1, 2, 3, 8]), rng.choice([8, 24, 40, 41]), rng.choice([80, 200, 206])]
+        for _ in range(2):
+            if rng.random() < 0.15:
+                pitch = [rng.randint(0, 6), rng.randint(0, 50), rng.randint(0, 220)]
+            shape = [rng.randint(0 if rng.random() < 0.02 else 1, 5) for _ in range(3)]
+            views.append((shape, [pitch[2], pitch[1], pitch[0]], rng.randint(0, 300)))
+        a, b = (buf.as_strided(*v) for v in views)
+        want = bool(set(where.as_strided(*views[0]).flatten().tolist()) & set(where.as_strided(*views[1]).flatten().tolist()))
+        got = ops._meet(a, b)
+        assert got == want or (got and not want and views[0][1] != views[1][1]), views  # (long searches count as met)
+        assert ops._meet(b, a) == got
+        met += want
+    assert 200 < met < 1300
+
+
+def test_both_ways_of_a_call_refuse_the_same_views():
+    rng = random.Random(11)
+    buf = torch.zeros(600, dtype=H16)
+    seen = {True: 0, False: 0}
+    for _ in range(400):
+        pitch = rng.choice([24, 25, 32, 48, 56])
+        y = buf.as_strided((3, 24), (pitch, 1), rng.randint(0, 100))
+        out = buf.as_strided((3, 24), (pitch if rng.random() < 0.8 else 40, 1), rng.randint(0, 250))
+        fits = _lib.bind().adapter_fits(*_bind_args("adapter", dict(y=y, out=out)))
+        with pytest.raises(ValueError) as error:
+            _adapters(y=y, out=out)()
+        assert fits == ("CUDA tensor" in str(error.value)), (y.stride(), out.stride(), y.storage_offset(), out.storage_offset(), error.value)
+        seen[fits] += 1
+    assert min(seen.values()) > 50

@@ -14,6 +14,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+
 #include "wsvd_b200.h"
 
 namespace {
@@ -71,6 +73,55 @@ bool apart(const Tensor* t) {
   }
   return true;
 }
+// Whether two tensors have a byte of memory in common, as ops.py's _meet: apart = sum of i stride over a's dims - the same over b's.
+struct Terms {
+  int n = 0, budget = 256;
+  int64_t size, stride[6], first[6], last[6];
+  void add(const Tensor& t, bool minus) {
+    for (int64_t d = 0; d < t.dim(); ++d) {
+      const int64_t s = t.stride(d) * t.element_size(), most = t.size(d) - 1;
+      if (most < 1 || s == 0) continue;
+      int i = 0;
+      while (i < n && stride[i] > s) ++i;
+      if (i == n || stride[i] != s) {
+        for (int j = n++; j > i; --j) stride[j] = stride[j - 1], first[j] = first[j - 1], last[j] = last[j - 1];
+        stride[i] = s, first[i] = last[i] = 0;
+      }
+      (minus ? first[i] : last[i]) += minus ? -most : most;
+    }
+  }
+  static int64_t below(int64_t a, int64_t b) { return a / b - (a % b != 0 && a < 0); }  // b > 0
+  bool reach(int at, int64_t left) {
+    int64_t low = 0, high = 0;
+    for (int i = at; i < n; ++i) low += stride[i] * first[i], high += stride[i] * last[i];
+    if (left <= low - size || left >= high + size) return false;
+    if (at == n) return true;
+    const int64_t s = stride[at];
+    low -= s * first[at], high -= s * last[at];
+    const int64_t from = std::max(first[at], -below(high + size - 1 - left, s)), to = std::min(last[at], below(left - low + size - 1, s));
+    for (int64_t i = from; i <= to; ++i)
+      if (--budget < 0 || reach(at + 1, left - i * s)) return true;
+    return false;
+  }
+};
+bool meet(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  Terms t;
+  t.size = std::max(a.element_size(), b.element_size());
+  t.add(a, false);
+  t.add(b, true);
+  return t.reach(0, static_cast<const char*>(b.data_ptr()) - static_cast<const char*>(a.data_ptr()));
+}
+// an output may be the input `in_place` itself (one shape), and has no memory of any input otherwise
+bool no_overlap(const Tensor* out, const Tensor& in_place, std::initializer_list<const Tensor*> others) {
+  if (!out) return true;
+  bool same = out->data_ptr() == in_place.data_ptr();
+  for (int64_t d = 0; same && d < out->dim(); ++d) same = out->size(d) < 2 || out->stride(d) == in_place.stride(d);
+  if (!same && meet(*out, in_place)) return false;
+  for (const Tensor* t : others)
+    if (meet(*out, *t)) return false;
+  return true;
+}
 int code(at::ScalarType t) { return t == at::kChar ? WSVD_I8 : t == at::kHalf ? WSVD_F16 : WSVD_BF16; }
 bool half(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
 void* at_of(const Tensor* t) { return t ? t->data_ptr() : nullptr; }
@@ -113,8 +164,7 @@ struct Append {
            cache_fits(ck, cv, ks, vs, type, H, D, device) && metadata_fits(lens, idx, table, batch, device) &&
            (!cu || vector(cu, batch + 1, at::kInt, device)) && (!off || vector(off, batch, at::kInt, device)) &&
            (q ? rows(q, 3, type, device) && q->size(0) == N && q->size(2) == D : !q_out) &&
-           (!q_out || (rows(q_out, 3, type, device) && same_shape(*q, *q_out) &&
-                       (q_out->data_ptr() != q->data_ptr() || q_out->strides() == q->strides()))) &&
+           (!q_out || (rows(q_out, 3, type, device) && same_shape(*q, *q_out) && no_overlap(q_out, *q, {k, v}))) &&
            apart(q_out) && apart(ck) && apart(cv) && apart(ks) && apart(vs) && !differentiated({k, v, q, q_out, ck, cv, ks, vs, inv});
   }
 };
@@ -195,7 +245,7 @@ struct Paged {
     const int64_t H = q->size(1), D = q->size(2), K = ck->size(1);
     return rows(q, 3, type, device) && D >= 1 && D <= 256 && K > 0 && H > 0 && H % K == 0 && window >= 0 &&
            cache_fits(ck, cv, ks, vs, type, K, D, device) && metadata_fits(lens, idx, table, q->size(0), device) &&
-           (!out || (rows(out, 3, type, device) && same_shape(*out, *q))) &&
+           (!out || (rows(out, 3, type, device) && same_shape(*out, *q) && no_overlap(out, *q, {ck, cv}))) &&
            (!workspace || (workspace->device() == device && workspace->is_contiguous())) && apart(out) && !differentiated({q, ck, cv, ks, vs, out});
   }
 };
@@ -270,8 +320,7 @@ struct Adapters {
            a->size(1) == in && b->size(0) == count && b->size(1) == rank && b->size(2) == columns && rank >= 1 && rank <= 256 && in > 0 &&
            columns > 0 && vector(adapter, B, at::kInt, device) && (!scale || vector(scale, count, at::kFloat, device)) &&
            (cu ? vector(cu, B + 1, at::kInt, device) : B == N) &&
-           (!out || (rows(out, 2, type, device) && same_shape(*out, *y) &&
-                     (out->data_ptr() != y->data_ptr() || out->strides() == y->strides()))) &&
+           (!out || (rows(out, 2, type, device) && same_shape(*out, *y) && no_overlap(out, *y, {x, a, b}))) &&
            (!workspace || (workspace->device() == device && workspace->is_contiguous())) && apart(out) && !differentiated({x, y, a, b, scale, out});
   }
 };

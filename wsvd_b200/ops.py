@@ -504,6 +504,55 @@ def _apart(name, t):
             reach += stride * (size - 1)
 
 
+def _meet(a, b):
+    """Whether two tensors have a byte of memory in common.  (Exact for views of one layout, column slices of a joined
+    matrix or heads of a joined projection among them; strides of two layouts that would take long to look through count as yes.)"""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    size, apart = max(a.element_size(), b.element_size()), b.data_ptr() - a.data_ptr()
+    # apart = sum of i stride over a's dims - the same over b's, but for the last element's bytes
+    terms = {}
+    for t, sign in ((a, 1), (b, -1)):
+        for n, s in zip(t.shape, t.stride()):
+            if n > 1 and s > 0:
+                r = terms.setdefault(s * t.element_size(), [0, 0])
+                r[sign > 0] += sign * (n - 1)
+    terms = sorted(terms.items(), reverse=True)
+    budget = 256
+
+    def reach(at, left):
+        nonlocal budget
+        low = sum(s * r[0] for s, r in terms[at:])
+        high = sum(s * r[1] for s, r in terms[at:])
+        if not low - size < left < high + size:
+            return False
+        if at == len(terms):
+            return True
+        s, (first, last) = terms[at]
+        low, high = low - s * first, high - s * last
+        for i in range(max(first, -((high + size - 1 - left) // s)), min(last, (left - low + size - 1) // s) + 1):
+            budget -= 1
+            if budget < 0 or reach(at + 1, left - i * s):
+                return True
+        return False
+
+    return reach(0, apart)
+
+
+def _same_places(a, b):
+    """Two tensors of one shape whose elements are at the same addresses."""
+    return a.data_ptr() == b.data_ptr() and all(n < 2 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+
+
+def _no_overlap(name, out, in_place, t, **others):
+    """An output may be the input `in_place` itself, and has no memory of any input otherwise."""
+    if not _same_places(out, t) and _meet(out, t):
+        raise ValueError(f"{name} may be {in_place} itself, not another view of its storage")
+    for other, o in others.items():
+        if o is not None and _meet(out, o):
+            raise ValueError(f"{name} must not overlap {other}")
+
+
 def _on_one_gpu(**tensors):
     index = None
     for name, t in tensors.items():
@@ -601,8 +650,7 @@ def _check_append(k, v, lens, idx, table, cache_k, cache_v, inv_freq, cache_k_sc
             _tensor("q_out", q_out, (dtype,), 3)
             if q_out.shape != q.shape:
                 raise ValueError(f"q_out must be {tuple(q.shape)}, got {tuple(q_out.shape)}")
-            if q_out.data_ptr() == q.data_ptr() and q_out.stride() != q.stride() and q.numel() > 0:
-                raise ValueError("q_out may be q itself, not another view of its storage")
+            _no_overlap("q_out", q_out, "q", q, k=k, v=v)
             _apart("q_out", q_out)
     elif q_out is not None:
         raise ValueError("q_out without q")
@@ -627,11 +675,11 @@ def kv_rope_append(k, v, infer_state, cache_k, cache_v, inv_freq, *, cache_k_sca
     adds the new rows afterwards.  The first ``2 * len(inv_freq)`` dims are rotated by ``(position + pos_offset[b]) *
     inv_freq`` (`rope_layout` as in `latent_decode`), the others and v go through.
     cache_k, cache_v [T, Hkv, D] in the rows' dtype, or int8 with f16 scales [T, Hkv] (the quantiser of
-    `latent_quant_append`, on the rotated f32 row).  `q_out` may be q.
+    `latent_quant_append`, on the rotated f32 row).  `q_out` may be q, and shares no memory with q, k or v otherwise.
 
     Rows behind cu_new[B] are padding: nothing of them is stored, a `q_out` of the caller's keeps its rows, the op's own has
     zeros there.  A row without a place in the table or the cache is skipped and reported by `kernel_status`.  No two rows may
-    name the same slot.
+    name the same slot, and none may be read from memory that the call writes.
     The reference's dense caches are made by its test script (efficiency/test_timing_layer.py)."""
     lens, idx, table = infer_state.b_seq_len, infer_state.b_req_idx, infer_state.req_manager.req_to_token_indexs
     if stream is None and rope_layout in ROPE:
@@ -685,6 +733,7 @@ def _check_paged(q, lens, idx, table, cache_k, cache_v, k_scale, v_scale, out, w
         _tensor("out", out, (q.dtype,), 3)
         if out.shape != q.shape:
             raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+        _no_overlap("out", out, "q", q, cache_k=cache_k, cache_v=cache_v)
         _apart("out", out)
     if window < 0:
         raise ValueError("window must not be negative")
@@ -705,7 +754,8 @@ def paged_decode(q, infer_state, cache_k, cache_v, k_scale=None, v_scale=None, *
     Sequence b attends to the positions ``max(0, b_seq_len[b] - window) <= s < b_seq_len[b]`` (window 0: all), position s in
     token slot ``req_to_token_indexs[b_req_idx[b], s]``.  Query heads that share a KV head share its loads.  A
     sequence without positions gives zeros and -inf.  A page-table entry outside the cache is left out and
-    reported by `kernel_status`, a length is clamped to the table's width.  `sm_scale` 0 means 1/sqrt(D).
+    reported by `kernel_status`, a length is clamped to the table's width.  `sm_scale` 0 means 1/sqrt(D).  `out` may be q, and shares
+    no memory with q or the caches otherwise.
     `workspace`: an optional CUDA byte/float buffer of `paged_decode_workspace_bytes` bytes; calls that may
     run at the same time need one each.  (`dense_decode` is the reference's f16 baseline.)"""
     lens, idx, table = infer_state.b_seq_len, infer_state.b_req_idx, infer_state.req_manager.req_to_token_indexs
@@ -780,8 +830,7 @@ def _check_adapters(y, x, a, b, adapter, scale, cu_new, out, workspace):
         _tensor("out", out, one, 2)
         if out.shape != y.shape:
             raise ValueError(f"out must be {tuple(y.shape)}, got {tuple(out.shape)}")
-        if out.data_ptr() == y.data_ptr() and out.stride() != y.stride() and y.numel() > 0:
-            raise ValueError("out may be y itself, not another view of its storage")
+        _no_overlap("out", out, "y", y, x=x, a=a, b=b)
         _apart("out", out)
     if workspace is not None and not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
@@ -797,7 +846,7 @@ def adapter_add(y, x, a, b, adapter, *, scale=None, cu_new=None, out=None, works
     x [N, n_in], y [N, n_out] (the projection's result), a [n_adapters, n_in, rank], b [n_adapters, rank, n_out], all f16 or all
     bf16 (rows at any stride: y and out may be column slices); adapter [B] int32; scale [n_adapters] f32, None means
     1.  Rows are packed by request, `cu_new` [B + 1] int32 as in `kv_rope_append` (None: one row per request).  Returns
-    out; `out=y` adds in place.  x a is summed in f32 (and, of packed rows, rounded to their type's number
+    out; `out=y` adds in place (an `out` that has memory of y, x, a or b otherwise is refused).  x a is summed in f32 (and, of packed rows, rounded to their type's number
     of bits, with the range of f32).  Rows behind cu_new[B] are padding: a caller's `out` keeps its rows, the op's own has y's there.  An adapter that does not exist adds nothing and is reported by `kernel_status`.
     `workspace`: an optional CUDA buffer of `adapter_add_workspace_bytes` bytes; calls that may run at the same time need one
     each."""
