@@ -115,3 +115,26 @@ def test_both_ways_of_a_call_refuse_the_same_views():
         assert fits == ("CUDA tensor" in str(error.value)), (y.stride(), out.stride(), y.storage_offset(), out.storage_offset(), error.value)
         seen[fits] += 1
     assert min(seen.values()) > 50
+
+
+# ------------------------------------------------------------------ derivatives
+
+def test_forward_mode_tangents_are_refused_under_no_grad_too():
+    def dual(*shape, dtype=H16):
+        t = torch.zeros(*shape, dtype=dtype)
+        return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+    table, T = pages(2, 8, 4, torch.Generator().manual_seed(1))
+    store, scale = torch.zeros(T, 2, 16, dtype=torch.int8), torch.ones(T, 2, dtype=H16)
+    with torch.autograd.forward_ad.dual_level():
+        calls = [("append", dict(k=dual(2, 2, 16))), ("append", dict(v=dual(2, 2, 16))), ("append", dict(q=dual(2, 4, 16))),
+                 ("append", dict(inv_freq=dual(8, dtype=torch.float32))),
+                 ("paged", dict(q=dual(2, 4, 16))), ("paged", dict(cache_v=dual(T, 2, 16))),
+                 ("paged", dict(cache_k=store, cache_v=store, k_scale=scale, v_scale=dual(T, 2))),
+                 ("adapter", dict(x=dual(3, 16))), ("adapter", dict(y=dual(3, 24))), ("adapter", dict(a=dual(2, 16, 4))),
+                 ("adapter", dict(b=dual(2, 4, 24))), ("adapter", dict(scale=dual(2, dtype=torch.float32)))]
+        for op, kw in calls:
+            refused(op, "no forward-mode derivative", **kw)
+            with torch.no_grad():
+                refused(op, "no forward-mode derivative", **kw)
+        accepted("adapter", x=torch.autograd.forward_ad.unpack_dual(dual(3, 16)).primal)

@@ -51,10 +51,11 @@ bool scales(const Tensor* t, const Tensor& cache) {
   return t && t->layout() == at::kStrided && t->dim() == 2 && t->scalar_type() == at::kHalf && t->device() == cache.device() &&
          t->size(0) == cache.size(0) && t->size(1) == cache.size(1);
 }
+// a gradient is wanted of one of them, or one carries a tangent (which torch.no_grad() does not switch off)
 bool differentiated(std::initializer_list<const Tensor*> ts) {
-  if (!c10::GradMode::is_enabled()) return false;
+  const bool backward = c10::GradMode::is_enabled();
   for (const Tensor* t : ts)
-    if (t && t->requires_grad()) return true;
+    if (t && ((backward && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
   return false;
 }
 // an output's elements have a place in memory each

@@ -12,6 +12,7 @@ import functools
 from typing import Callable, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import LatentDecodeParams, check
@@ -567,8 +568,12 @@ def _on_one_gpu(**tensors):
 
 
 def _no_gradient(op, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    tensors = [t for t in tensors if t is not None]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ValueError(f"{op} has no backward: call it under torch.no_grad() or on detached tensors")
+    # (torch.no_grad() does not switch forward mode off)
+    if any(t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{op} has no forward-mode derivative: call it on the primal tensors")
 
 
 def _metadata(lens, idx, table, B):
