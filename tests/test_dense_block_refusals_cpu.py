@@ -4,7 +4,7 @@ import random
 import pytest
 import torch
 
-from tests.dense_block import pages
+from tests.dense_block import pages, state
 from tests.test_dense_block_cpu import H16, _adapters, _append, _bind_args, _paged
 from wsvd_b200 import _lib, ops
 
@@ -138,3 +138,26 @@ def test_forward_mode_tangents_are_refused_under_no_grad_too():
             with torch.no_grad():
                 refused(op, "no forward-mode derivative", **kw)
         accepted("adapter", x=torch.autograd.forward_ad.unpack_dual(dual(3, 16)).primal)
+
+
+# ------------------------------------------------------------------ sizes
+
+def test_sizes_beyond_32_bits_are_refused_not_cut():
+    """2^32 + 3 rows would be 3 (tensors of one element's memory)."""
+    many = 2 ** 32 + 3
+    cu = torch.zeros(3, dtype=torch.int32)
+    rows = torch.zeros(1, 2, 16, dtype=H16).expand(many, 2, 16)
+    refused("append", "rows of k", k=rows, v=rows, cu_new=cu)
+    none = torch.zeros(2, 0, 16, dtype=H16)
+    heads = torch.zeros(2, 1, 16, dtype=H16).expand(2, many, 16)
+    refused("append", "heads of q", q=heads)
+    refused("append", "heads of k", k=heads, v=heads, cache_k=heads, cache_v=heads)
+    refused("paged", "heads of q", q=torch.zeros(2, 1, 16, dtype=H16).expand(2, 2 ** 32 + 4, 16))
+    table = torch.zeros(1, 8, dtype=torch.int32).expand(many, 8)
+    refused("append", "rows of req_to_token_indexs", infer_state=state([1, 2], table))
+    refused("paged", "rows of req_to_token_indexs", infer_state=state([1, 2], table))
+    two = torch.zeros(2, dtype=torch.int32)
+    refused("adapter", "rows of x", x=torch.zeros(1, 16, dtype=H16).expand(many, 16), y=torch.zeros(1, 24, dtype=H16).expand(many, 24),
+            adapter=two, cu_new=cu)
+    refused("adapter", "adapters", a=torch.zeros(1, 16, 4, dtype=H16).expand(many, 16, 4), b=torch.zeros(1, 4, 24, dtype=H16).expand(many, 4, 24))
+    accepted("append", q=none)

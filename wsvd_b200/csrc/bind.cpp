@@ -51,6 +51,8 @@ bool scales(const Tensor* t, const Tensor& cache) {
   return t && t->layout() == at::kStrided && t->dim() == 2 && t->scalar_type() == at::kHalf && t->device() == cache.device() &&
          t->size(0) == cache.size(0) && t->size(1) == cache.size(1);
 }
+// sizes that the C entries take as 32-bit numbers
+bool countable(std::initializer_list<int64_t> sizes) { return std::max(sizes) <= INT32_MAX; }
 // a gradient is wanted of one of them, or one carries a tangent (which torch.no_grad() does not switch off)
 bool differentiated(std::initializer_list<const Tensor*> ts) {
   const bool backward = c10::GradMode::is_enabled();
@@ -139,7 +141,8 @@ bool cache_fits(const Tensor* k, const Tensor* v, const Tensor* ks, const Tensor
   return held == at::kChar ? scales(ks, *k) && scales(vs, *k) : !ks && !vs;
 }
 bool metadata_fits(const Tensor* lens, const Tensor* idx, const Tensor* table, int64_t batch, const at::Device& device) {
-  return vector(lens, batch, at::kInt, device) && vector(idx, batch, at::kInt, device) && rows(table, 2, at::kInt, device);
+  return vector(lens, batch, at::kInt, device) && vector(idx, batch, at::kInt, device) && rows(table, 2, at::kInt, device) &&
+         countable({batch, table->size(0), table->size(1)});
 }
 
 // ---- kv_rope_append(k, v, lens, idx, table, cache_k, cache_v, inv_freq, k_scale, v_scale, q, q_out, cu_new, pos_offset, layout)
@@ -160,7 +163,7 @@ struct Append {
     const at::Device device = k->device();
     const int64_t N = k->size(0), H = k->size(1), D = k->size(2);
     batch = cu ? cu->dim() == 1 ? cu->size(0) - 1 : -1 : N;
-    return batch >= 0 && rows(k, 3, type, device) && rows(v, 3, type, device) && same_shape(*k, *v) && H > 0 && D >= 2 && D % 2 == 0 && D <= 256 &&
+    return batch >= 0 && countable({N, H, q && q->dim() == 3 ? q->size(1) : 0}) && rows(k, 3, type, device) && rows(v, 3, type, device) && same_shape(*k, *v) && H > 0 && D >= 2 && D % 2 == 0 && D <= 256 &&
            inv && inv->dim() == 1 && vector(inv, inv->size(0), at::kFloat, device) && 2 * inv->size(0) <= D &&
            cache_fits(ck, cv, ks, vs, type, H, D, device) && metadata_fits(lens, idx, table, batch, device) &&
            (!cu || vector(cu, batch + 1, at::kInt, device)) && (!off || vector(off, batch, at::kInt, device)) &&
@@ -244,7 +247,7 @@ struct Paged {
     const at::ScalarType type = q->scalar_type();
     const at::Device device = q->device();
     const int64_t H = q->size(1), D = q->size(2), K = ck->size(1);
-    return rows(q, 3, type, device) && D >= 1 && D <= 256 && K > 0 && H > 0 && H % K == 0 && window >= 0 &&
+    return countable({H, K}) && rows(q, 3, type, device) && D >= 1 && D <= 256 && K > 0 && H > 0 && H % K == 0 && window >= 0 &&
            cache_fits(ck, cv, ks, vs, type, K, D, device) && metadata_fits(lens, idx, table, q->size(0), device) &&
            (!out || (rows(out, 3, type, device) && same_shape(*out, *q) && no_overlap(out, *q, {ck, cv}))) &&
            (!workspace || (workspace->device() == device && workspace->is_contiguous())) && apart(out) && !differentiated({q, ck, cv, ks, vs, out});
@@ -317,7 +320,7 @@ struct Adapters {
     const at::ScalarType type = x->scalar_type();
     const at::Device device = x->device();
     const int64_t N = x->size(0), in = x->size(1), columns = y->size(1), count = a->size(0), rank = a->size(2), B = adapter->size(0);
-    return rows(x, 2, type, device) && rows(y, 2, type, device) && rows(a, 3, type, device) && rows(b, 3, type, device) && y->size(0) == N &&
+    return countable({N, in, columns, count, B}) && rows(x, 2, type, device) && rows(y, 2, type, device) && rows(a, 3, type, device) && rows(b, 3, type, device) && y->size(0) == N &&
            a->size(1) == in && b->size(0) == count && b->size(1) == rank && b->size(2) == columns && rank >= 1 && rank <= 256 && in > 0 &&
            columns > 0 && vector(adapter, B, at::kInt, device) && (!scale || vector(scale, count, at::kFloat, device)) &&
            (cu ? vector(cu, B + 1, at::kInt, device) : B == N) &&

@@ -495,6 +495,13 @@ def _tensor(name, t, dtypes, ndim, inner_contiguous=True):
         raise ValueError(f"{name}: innermost dimension must be contiguous")
 
 
+def _countable(**sizes):
+    """Sizes that the C entries take as 32-bit numbers."""
+    for name, n in sizes.items():
+        if n > 2 ** 31 - 1:
+            raise ValueError(f"{name}: {n} is beyond 2^31 - 1")
+
+
 def _apart(name, t):
     """An output's elements have a place in memory each."""
     reach = 1
@@ -582,6 +589,7 @@ def _metadata(lens, idx, table, B):
     _tensor("req_to_token_indexs", table, (torch.int32,), 2)
     if lens.shape[0] != B or idx.shape[0] != B:
         raise ValueError("batch metadata must have one entry per sequence")
+    _countable(batch=B, **{"rows of req_to_token_indexs": table.shape[0], "columns of req_to_token_indexs": table.shape[1]})
 
 
 def _dense_cache(cache_k, cache_v, k_scale, v_scale, dtype, Hkv, D):
@@ -631,6 +639,7 @@ def _check_append(k, v, lens, idx, table, cache_k, cache_v, inv_freq, cache_k_sc
     _tensor("inv_freq", inv_freq, (torch.float32,), 1)
     if Hkv < 1:
         raise ValueError("k and v must have heads")
+    _countable(**{"rows of k": N, "heads of k": Hkv})
     if D < 2 or D % 2 or D > 256 or 2 * inv_freq.shape[0] > D:
         raise ValueError(f"head_dim must be even and at most 256, with at most head_dim / 2 frequencies: {D}, {inv_freq.shape[0]}")
     _dense_cache(cache_k, cache_v, cache_k_scale, cache_v_scale, dtype, Hkv, D)
@@ -651,6 +660,7 @@ def _check_append(k, v, lens, idx, table, cache_k, cache_v, inv_freq, cache_k_sc
         _tensor("q", q, (dtype,), 3)
         if q.shape[0] != N or q.shape[2] != D:
             raise ValueError(f"q must be [{N}, Hq, {D}], got {tuple(q.shape)}")
+        _countable(**{"heads of q": q.shape[1]})
         if q_out is not None:
             _tensor("q_out", q_out, (dtype,), 3)
             if q_out.shape != q.shape:
@@ -733,6 +743,7 @@ def _check_paged(q, lens, idx, table, cache_k, cache_v, k_scale, v_scale, out, w
     _dense_cache(cache_k, cache_v, k_scale, v_scale, q.dtype, Hkv, D)
     if Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise ValueError(f"q heads ({Hq}) must be a multiple of KV heads ({Hkv})")
+    _countable(**{"heads of q": Hq})
     _metadata(lens, idx, table, B)
     if out is not None:
         _tensor("out", out, (q.dtype,), 3)
@@ -820,6 +831,7 @@ def _check_adapters(y, x, a, b, adapter, scale, cu_new, out, workspace):
     if n_in < 1 or n_out < 1:
         raise ValueError("x and y must have columns")
     B = adapter.shape[0]
+    _countable(**{"rows of x": N, "columns of x": n_in, "columns of y": n_out, "adapters": count, "entries of adapter": B})
     if scale is not None:
         _tensor("scale", scale, (torch.float32,), 1)
         if scale.shape[0] != count:
