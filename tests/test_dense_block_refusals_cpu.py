@@ -1,11 +1,12 @@
 """What the dense attention block's operators refuse beyond tests/test_dense_block_cpu.py: both ways of a call, without a GPU."""
+import ctypes
 import random
 
 import pytest
 import torch
 
 from tests.dense_block import pages, state
-from tests.test_dense_block_cpu import H16, _adapters, _append, _bind_args, _paged
+from tests.test_dense_block_cpu import FAKE, H16, _adapter_params, _adapters, _append, _bind_args, _paged, _paged_params
 from wsvd_b200 import _lib, ops
 
 CALLS = {"append": _append, "paged": _paged, "adapter": _adapters}
@@ -161,3 +162,13 @@ def test_sizes_beyond_32_bits_are_refused_not_cut():
             adapter=two, cu_new=cu)
     refused("adapter", "adapters", a=torch.zeros(1, 16, 4, dtype=H16).expand(many, 16, 4), b=torch.zeros(1, 4, 24, dtype=H16).expand(many, 4, 24))
     accepted("append", q=none)
+
+
+def test_lengths_that_a_last_step_would_carry_past_32_bits_are_refused():
+    """A page table of 2^31 - 1 columns: the step behind the last position would count on from below zero."""
+    lib = _lib.lib()
+    for most, status in ((2 ** 31 - 1, 8), (2 ** 31 - 1024, 8)):
+        assert lib.wsvd_paged_decode(ctypes.byref(_paged_params(max_len=most)), FAKE, 1 << 60, None) == status
+        for kw in (dict(rows=most), dict(batch=most), dict(n_in=most), dict(rows=most, batch=most, cu_new=None)):
+            assert lib.wsvd_adapter_add(ctypes.byref(_adapter_params(**kw)), FAKE, 1 << 60, None) == status
+    assert lib.wsvd_adapter_add(ctypes.byref(_adapter_params(n_out=2 ** 31 - 1)), FAKE, 1 << 60, None) == 8

@@ -942,7 +942,8 @@ int wsvd_adapter_add(const WsvdAdapterAddParams* p, void* workspace, size_t work
   if (p->rank <= 0 || p->rank > 256) return WSVD_ERR_BAD_SHAPE;
   if (p->dtype != WSVD_F16 && p->dtype != WSVD_BF16) return WSVD_ERR_BAD_DTYPE;
   if (!p->cu_new && p->rows != p->batch) return WSVD_ERR_BAD_SHAPE;
-  if ((p->n_out + 255) / 256 > 65535) return WSVD_ERR_TOO_LARGE;
+  if (p->rows > wsvd::kMostCounted || p->batch > wsvd::kMostCounted || p->n_in > wsvd::kMostCounted) return WSVD_ERR_TOO_LARGE;
+  if ((p->n_out - 1) / 256 >= 65535) return WSVD_ERR_TOO_LARGE;
   if (p->rows == 0) return WSVD_OK;
   if (!p->y || !p->x || !p->out || (p->batch > 0 && !p->adapter)) return WSVD_ERR_NULL_POINTER;
   if (p->n_adapters > 0 && (!p->a || !p->b)) return WSVD_ERR_NULL_POINTER;

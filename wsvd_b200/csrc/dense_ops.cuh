@@ -8,6 +8,9 @@
 
 namespace wsvd {
 
+// Positions and rows are counted in steps of up to 2048 as 32-bit numbers: what is beyond this would pass 2^31 in the last step.
+constexpr int32_t kMostCounted = INT32_MAX - 4096;
+
 // Recorded by the three operators, each in its translation unit's own word; wsvd_kernel_status reads them all.
 constexpr unsigned int kOutsideTable = 5;    // a position beyond the page table's width
 constexpr unsigned int kOutsideStorage = 7;  // a slot, request or adapter that does not exist

@@ -949,7 +949,7 @@ int wsvd_paged_decode(const WsvdPagedDecodeParams* p, void* workspace, size_t wo
   if (p->dtype != WSVD_F16 && p->dtype != WSVD_BF16) return WSVD_ERR_BAD_DTYPE;
   const bool i8 = p->cache_dtype == WSVD_I8;
   if (!i8 && p->cache_dtype != p->dtype) return WSVD_ERR_BAD_DTYPE;
-  if (p->batch > 65535 || p->n_q_heads > 65535) return WSVD_ERR_TOO_LARGE;
+  if (p->batch > 65535 || p->n_q_heads > 65535 || p->max_len > wsvd::kMostCounted) return WSVD_ERR_TOO_LARGE;
   if (p->batch == 0) return WSVD_OK;
   if (!p->q || !p->out || !p->b_req_idx || !p->b_seq_len) return WSVD_ERR_NULL_POINTER;
   const bool places = p->n_token_slots > 0 && p->n_req > 0 && p->max_len > 0;  // (else no sequence has positions)
