@@ -164,3 +164,47 @@ def test_an_outlier_in_one_head_of_a_group():
     q[0, 2, 5] = 200.0
     k[..., 5] = 0
     _check_long_bytes(q, st, k, v, ks, vs)
+
+
+# ------------------------------------------------------------------ append: bytes of values between two steps
+
+def _between_steps(dtype, D):
+    """Rows [n, D] of values whose quotient by the row's scale and whose product with 1 / scale round to different steps."""
+    found = []
+    ones = torch.arange(128 if dtype is BF16 else 1024, dtype=torch.float32) / (128 if dtype is BF16 else 1024) + 1
+    for amax in ones.tolist():
+        scale = (torch.tensor(amax) / 127).half().float()
+        x = torch.cat([ones * 2.0 ** -e for e in range(1, 8)])
+        x = x[(x.to(dtype).float() == x) & (x <= amax)]
+        apart = x[(x / scale).round() != (x * (1 / scale)).round()]
+        if len(apart):
+            row = torch.full((D,), amax)
+            row[1:] = apart[torch.arange(D - 1) % len(apart)] * torch.where(torch.arange(D - 1) % 3 == 0, -1.0, 1.0)
+            found.append(row)
+    return torch.stack(found).to(dtype) if found else torch.zeros(0, D, dtype=dtype)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [128, 40])  # the second one on the kernel for any shape
+@pytest.mark.parametrize("many", [False, True])
+def test_bytes_are_those_of_the_quotient(dtype, D, many):
+    """int8 rows are round(x / scale), as latent_quant_append stores them: equal, also between two steps."""
+    rows = _between_steps(dtype, D)
+    assert (len(rows) > 3) == (dtype is F16)  # (8 bits of bf16 meet no such scale)
+    n = 30000 if many and D == 128 else 300
+    rows = torch.cat([rows, randn(torch.Generator().manual_seed(D), 61, D, dtype=dtype)])
+    rows = rows.repeat(n // len(rows) + 1, 1)[:n]
+    kv = torch.stack([rows, rows.flip(0)], 1).cuda()  # [n, 2, D]
+    table = torch.randperm(n, generator=torch.Generator().manual_seed(1)).int()[None].contiguous()
+    st = gpu(state([0], table))
+    caches = [torch.zeros(n, 2, D, dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros(n, 2, dtype=torch.float16, device="cuda") for _ in range(2)]
+    ops.kv_rope_append(kv, kv, st, *caches, torch.zeros(0, device="cuda"), cache_k_scale=scales[0], cache_v_scale=scales[1],
+                       cu_new=torch.tensor([0, n], dtype=torch.int32).cuda())
+    x = kv.cpu().float()
+    scale = (x.abs().amax(-1) / 127).half()
+    want = (x / scale.float()[..., None]).round().clamp(-128, 127).to(torch.int8)
+    at = table[0].long()
+    for cache, held in zip(caches, scales):
+        assert torch.equal(held.cpu()[at], scale)
+        assert torch.equal(cache.cpu()[at], want)

@@ -10,8 +10,8 @@
 // to [-pi, pi] with a two-term 2 pi, and only then handed to sincosf in f32.
 //
 // Memory bound: 14856 rows of prompts, 40 heads of 128, f16: 139 us, 6.57 TB/s read and written (a plain copy has that rate); into
-// bytes, 5665 rows of 8 KV heads and 32 queries: 33 us, 3.9 TB/s (a row's maximum has to be there before its first byte).  A step
-// of up to 64 rows: 3 us, the chain length -> page -> row.
+// bytes, 5665 rows of 8 KV heads and 32 queries: 34.5 us, 3.7 TB/s (two block barriers around the angles, and instructions: ncu has the
+// barrier and not-selected stalls in front, DRAM at a third).  A step of up to 64 rows: 3 to 4 us, the chain length -> page -> row.
 #include "dense_ops.cuh"
 
 namespace wsvd {
@@ -27,11 +27,20 @@ __device__ __forceinline__ void rotation(int64_t place, float freq, float* sn, f
   sincosf((float)r, sn, cs);
 }
 
-// A value in steps of the scale, as a byte.  (Times 1 / scale, a division a row: one for every value took a fifth of the time of
-// a prompt's append into bytes.  A value within an f32 rounding of the middle between two steps may go to either.)
-// The low byte of the answer is the byte: adding 1.5 2^23 rounds to a whole number, to even, and leaves it in the last bits.
-__device__ __forceinline__ uint32_t byte_of(float x, float to_step) {
-  return __float_as_uint(fminf(fmaxf(x * to_step, -128.f), 127.f) + 12582912.f);
+// A value in steps of the scale, rounded to even: the low byte of the answer.
+__device__ __forceinline__ uint32_t byte_of(float x, float scale) { return (uint32_t)(int)fminf(fmaxf(rintf(x / scale), -128.f), 127.f); }
+
+// The same from x times 1 / scale (a division a value took 43 us for 5665 rows, the product without a look at
+// the middle 32, with it 34.5), for scales that are f16's own max|x| / 127, neither among its subnormals nor at its end, so that the product is between -128 and 128; `open` where it may
+// not be the quotient's.  The low byte again: adding 1.5 2^23 rounds to a whole number, to even, and leaves it in the last bits.
+// Up to 2^-15 before the middle of two steps the product rounds as the quotient does: 1 / scale and the product are each off by 2^-24,
+// together by 2^-16 at 128 steps.  (The quotient itself comes to lie on the middle only if x does: the middle times an f16 scale is an
+// f32 value.)  NaN is on no side.
+__device__ __forceinline__ bool whole_scale(float scale) { return scale >= 6.103515625e-5f && scale < 65504.f; }
+__device__ __forceinline__ uint32_t byte_by_product(float x, float to_step, bool* open) {
+  const float t = x * to_step, n = t + 12582912.f;
+  *open |= !(fabsf(t - (n - 12582912.f)) <= 0.5f - 1.f / 32768);
+  return __float_as_uint(n);
 }
 
 // What a row is: its sequence, its position (for the rotation) and its token slot (-1: not stored).
@@ -123,14 +132,14 @@ __global__ void __launch_bounds__(128) kv_append_any_kernel(const __grid_constan
   amax = warp_max(amax);
   // (the stored scale is f16: clamped to its range, as wsvd_latent_quant_append_i8 does)
   const __half scale = __float2half_rn(amax == 0.f ? 1.f : fminf(fmaxf(amax / 127.f, 5.9604644775390625e-8f), 65504.f));
-  const float to_step = 1.f / __half2float(scale);
+  const float step = __half2float(scale);
   int8_t* dst = is_v ? reinterpret_cast<int8_t*>(p.cache_v) + at.slot * p.cv_stride_t + (int64_t)h * p.cv_stride_h
                      : reinterpret_cast<int8_t*>(p.cache_k) + at.slot * p.ck_stride_t + (int64_t)h * p.ck_stride_h;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     if (i0[j] < 0) continue;
-    dst[i0[j]] = (int8_t)(byte_of(a[j], to_step) & 255u);
-    dst[i0[j] + (lane + 32 * j < half ? apart : 1)] = (int8_t)(byte_of(b[j], to_step) & 255u);
+    dst[i0[j]] = (int8_t)byte_of(a[j], step);
+    dst[i0[j] + (lane + 32 * j < half ? apart : 1)] = (int8_t)byte_of(b[j], step);
   }
   if (lane == 0) {
     if (is_v) reinterpret_cast<__half*>(p.v_scale)[at.slot * p.vs_stride_t + (int64_t)h * p.vs_stride_h] = scale;
@@ -194,20 +203,22 @@ template <typename T>
 __device__ __forceinline__ uint4 close8(const float (&f)[8]) {
   return make_uint4(Pair<T>::close(f[0], f[1]), Pair<T>::close(f[2], f[3]), Pair<T>::close(f[4], f[5]), Pair<T>::close(f[6], f[7]));
 }
-__device__ __forceinline__ uint2 bytes8(const float (&f)[8], float to_step) {
+template <typename F>
+__device__ __forceinline__ uint2 bytes8(const float (&f)[8], F byte) {
   uint32_t w[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const uint32_t low = __byte_perm(byte_of(f[4 * i], to_step), byte_of(f[4 * i + 1], to_step), 0x0040);
-    const uint32_t high = __byte_perm(byte_of(f[4 * i + 2], to_step), byte_of(f[4 * i + 3], to_step), 0x0040);
+    const uint32_t low = __byte_perm(byte(f[4 * i]), byte(f[4 * i + 1]), 0x0040);
+    const uint32_t high = __byte_perm(byte(f[4 * i + 2]), byte(f[4 * i + 3]), 0x0040);
     w[i] = __byte_perm(low, high, 0x5410);
   }
   return make_uint2(w[0], w[1]);
 }
 
 // lanes: log2 of the lanes of a head (D / 16 rounded up to a power of two); per_row: units of a row; U: units of a thread
+// (bytes, four units: three blocks an SM, so that bf16 ones have the registers for it; with the four of 64 registers they spill: 35.2 us, 34.5 so; 0: as the compiler chooses)
 template <typename T, bool I8, int U>
-__global__ void __launch_bounds__(kVecThreads)
+__global__ void __launch_bounds__(kVecThreads, I8 && U == 4 ? 3 : 0)
 kv_append_vec_kernel(const __grid_constant__ WsvdKvRopeAppendParams p, const int lanes, const Divisor per_row, const int most_rows) {
   extern __shared__ __align__(16) unsigned char smem[];
   const int half = p.rot_dim / 2, groups = p.rot_dim / 16;  // angles of a row, units that turn
@@ -315,11 +326,19 @@ kv_append_vec_kernel(const __grid_constant__ WsvdKvRopeAppendParams p, const int
       for (int o = 1; o < (1 << lanes); o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       if (hk >= 0 && active && slot >= 0) {
         const __half scale = __float2half_rn(amax == 0.f ? 1.f : fminf(fmaxf(amax / 127.f, 5.9604644775390625e-8f), 65504.f));
-        const float to_step = 1.f / __half2float(scale);
+        const float step = __half2float(scale), to_step = 1.f / step;
+        bool open = !whole_scale(step);
+        auto by_product = [&](float x) { return byte_by_product(x, to_step, &open); };
+        uint2 low = bytes8(a, by_product), high = bytes8(b, by_product);
+        if (open) {  // (16 values: one in a thousand)
+          auto by_quotient = [&](float x) { return byte_of(x, step); };
+          low = bytes8(a, by_quotient);
+          high = bytes8(b, by_quotient);
+        }
         int8_t* dst = hv < 0 ? reinterpret_cast<int8_t*>(p.cache_k) + slot * p.ck_stride_t + (int64_t)hk * p.ck_stride_h
                              : reinterpret_cast<int8_t*>(p.cache_v) + slot * p.cv_stride_t + (int64_t)hv * p.cv_stride_h;
-        *reinterpret_cast<uint2*>(dst + d0) = bytes8(a, to_step);
-        *reinterpret_cast<uint2*>(dst + d1) = bytes8(b, to_step);
+        *reinterpret_cast<uint2*>(dst + d0) = low;
+        *reinterpret_cast<uint2*>(dst + d1) = high;
         if (j == 0) {
           if (hv < 0) reinterpret_cast<__half*>(p.k_scale)[slot * p.ks_stride_t + (int64_t)hk * p.ks_stride_h] = scale;
           else reinterpret_cast<__half*>(p.v_scale)[slot * p.vs_stride_t + (int64_t)hv * p.vs_stride_h] = scale;
