@@ -10,14 +10,16 @@ import os
 import shutil
 import struct
 import subprocess
+import sys
 import threading
+import warnings
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 _ROOT = os.path.dirname(_PKG)
 _CSRC = os.path.join(_PKG, "csrc")
 _INCLUDE = os.path.join(_ROOT, "include")
 LIB_PATH = os.path.join(_PKG, "libwsvd_b200.so")
-BIND_PATH = os.path.join(_PKG, "_bind.so")  # csrc/bind.cpp: calls of the dense block's operators straight from torch tensors
+NO_BIND = (ImportError, OSError, RuntimeError)  # what building or loading csrc/bind.cpp's module fails with
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -48,8 +50,16 @@ def _older(path, deps) -> bool:
     return any(os.path.getmtime(f) > t for f in deps)
 
 
-def _stale() -> bool:
-    return _older(LIB_PATH, _deps()) or _older(BIND_PATH, _bind_deps())
+def bind_path() -> str:
+    """csrc/bind.cpp's module: calls of the dense block's operators straight from torch tensors.  It is made for one Python and one
+    torch, which its name says."""
+    import importlib.metadata
+
+    try:
+        torch = importlib.metadata.version("torch")
+    except importlib.metadata.PackageNotFoundError as e:
+        raise ImportError("csrc/bind.cpp needs torch") from e
+    return os.path.join(_PKG, f"_bind.{sys.implementation.cache_tag}-torch{torch}.so")
 
 
 def _bind_command(out):
@@ -57,7 +67,10 @@ def _bind_command(out):
     import importlib.util
     import sysconfig
 
-    torch = importlib.util.find_spec("torch").submodule_search_locations[0]
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        raise ImportError("csrc/bind.cpp needs torch")
+    torch = spec.submodule_search_locations[0]
     cuda = os.environ.get("CUDA_HOME") or "/usr/local/cuda"
     include = [_INCLUDE, os.path.join(torch, "include"), os.path.join(torch, "include", "torch", "csrc", "api", "include"),
                sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
@@ -67,47 +80,70 @@ def _bind_command(out):
             "-lc10_cuda"]
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile every .cu under csrc/ into one shared object for sm_100a, and csrc/bind.cpp into a Python module.
+def _made(path, deps, force, make) -> str:
+    """`path`, made by make(temporary name) where it is missing, older than one of `deps` or `force`d.
 
     Safe when several processes start at once (one rank per GPU under torchrun): the
     staleness check, the compile and the rename happen under an inter-process file lock, the
     compiler writes to a per-process temporary name, and a process that gets the lock after
-    another one has built finds the library fresh and returns."""
+    another one has built finds the file fresh and returns."""
     import fcntl
 
     with _lock:
-        if not force and not _stale():
-            return LIB_PATH
-        with open(LIB_PATH + ".lock", "w") as lockfile:
+        if not force and not _older(path, deps()):
+            return path
+        with open(path + ".lock", "w") as lockfile:
             fcntl.flock(lockfile, fcntl.LOCK_EX)
+            tmp = f"{path}.{os.getpid()}.tmp"
             try:
-                if not force and not _stale():
-                    return LIB_PATH
-                nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
-                if not os.path.exists(nvcc):
-                    raise RuntimeError("nvcc not found: cannot build libwsvd_b200.so")
-                tmp, tmp_bind = (f"{p}.{os.getpid()}.tmp" for p in (LIB_PATH, BIND_PATH))
-                cmd = [nvcc, *NVCC_FLAGS, "-I", _INCLUDE, "-I", _CSRC, *sources(), "-o", tmp, "-lcuda"]
-                if verbose:
-                    cmd.insert(1, "-Xptxas=-v")
-                bind = subprocess.Popen(_bind_command(tmp_bind), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-                res = subprocess.run(cmd, capture_output=True, text=True)
-                said = bind.communicate()[0]
-                if res.returncode != 0 or bind.returncode != 0:
-                    for f in (tmp, tmp_bind):
-                        if os.path.exists(f):
-                            os.remove(f)
-                    if res.returncode != 0:
-                        raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
-                    raise RuntimeError("the C++ compiler failed on csrc/bind.cpp:\n" + said)
-                if verbose:
-                    print(res.stderr)
-                os.replace(tmp_bind, BIND_PATH)
-                os.replace(tmp, LIB_PATH)
+                if force or _older(path, deps()):
+                    make(tmp)
+                    os.replace(tmp, path)
             finally:
+                if os.path.exists(tmp):
+                    os.remove(tmp)
                 fcntl.flock(lockfile, fcntl.LOCK_UN)
-        return LIB_PATH
+        return path
+
+
+def _compile_lib(verbose):
+    def make(tmp):
+        nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+        if not os.path.exists(nvcc):
+            raise RuntimeError("nvcc not found: cannot build libwsvd_b200.so")
+        cmd = [nvcc, *NVCC_FLAGS, "-I", _INCLUDE, "-I", _CSRC, *sources(), "-o", tmp, "-lcuda"]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError("nvcc failed:\n" + res.stdout + res.stderr)
+        if verbose:
+            print(res.stderr)
+
+    return make
+
+
+def _compile_bind(tmp):
+    res = subprocess.run(_bind_command(tmp), stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("the C++ compiler failed on csrc/bind.cpp:\n" + res.stdout)
+
+
+def _build_bind(force: bool = False) -> str:
+    return _made(bind_path(), _bind_deps, force, _compile_bind)
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    """Compile every .cu under csrc/ into one shared object for sm_100a, and csrc/bind.cpp into a Python module.
+
+    The module needs a C++ compiler and torch's headers; without them the library is all there is, and calls go through
+    ctypes (a warning says so)."""
+    path = _made(LIB_PATH, _deps, force, _compile_lib(verbose))
+    try:
+        _build_bind(force)
+    except NO_BIND as e:
+        warnings.warn(f"csrc/bind.cpp was not built, calls go through ctypes: {e}", RuntimeWarning, stacklevel=2)
+    return path
 
 
 class LatentDecodeParams(ctypes.Structure):
@@ -313,7 +349,7 @@ def lib() -> ctypes.CDLL:
     """The loaded library; builds it first if the shared object is missing or stale."""
     global _lib
     if _lib is None:
-        build()
+        _made(LIB_PATH, _deps, False, _compile_lib(False))
         handle = ctypes.CDLL(LIB_PATH)
         for name, (res, args) in SYMBOLS.items():
             fn = getattr(handle, name)  # AttributeError if the symbol is missing
@@ -327,7 +363,8 @@ _bind = None
 
 
 def bind():
-    """The module of csrc/bind.cpp, connected to the library's entries; builds both first where they are missing or stale."""
+    """The module of csrc/bind.cpp, connected to the library's entries; builds both first where they are missing or stale.
+    Raises one of NO_BIND where there is no such module to be had."""
     global _bind
     if _bind is None:
         import importlib.util
@@ -335,7 +372,7 @@ def bind():
         import torch  # noqa: F401  (the module's libraries)
 
         handle = lib()
-        spec = importlib.util.spec_from_file_location("wsvd_b200._bind", BIND_PATH)
+        spec = importlib.util.spec_from_file_location("wsvd_b200._bind", _build_bind())
         module = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(module)
         module.connect(*(ctypes.cast(getattr(handle, f"wsvd_{n}"), ctypes.c_void_p).value for n in

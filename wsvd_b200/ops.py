@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import warnings
 from typing import Callable, Optional, Tuple
 
 import torch
@@ -465,15 +466,28 @@ _pack_adapter = _lib.packer(_lib.AdapterAddParams)
 
 # An ordinary call (the current stream, torch's allocator, arguments as they should be) goes through csrc/bind.cpp, which
 # answers None to any other: the checks below say what is wrong with it, or it is made the long way.  (A single token's append
-# takes the GPU 3 us; with its arguments looked at in Python the call took 14, so it takes 6.)
+# takes the GPU 3 us; with its arguments looked at in Python the call took 14, so it takes 6.)  Where that module cannot be built or
+# loaded all calls are made the long way, to the same entries of the library.
 
 _fast = None
+
+
+class _LongWay:
+    @staticmethod
+    def append(*args):
+        return None
+
+    paged = adapter = append
 
 
 def _ordinary():
     global _fast
     if _fast is None:
-        _fast = _lib.bind()
+        try:
+            _fast = _lib.bind()
+        except _lib.NO_BIND as e:
+            warnings.warn(f"csrc/bind.cpp is not there, calls go through ctypes and take some 10 us more: {e}", RuntimeWarning, stacklevel=3)
+            _fast = _LongWay
     return _fast
 
 
