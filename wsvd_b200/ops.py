@@ -624,11 +624,15 @@ def _dense_cache(cache_k, cache_v, k_scale, v_scale, dtype, Hkv, D):
 
 
 def _new(alloc_tensor_func, like, shape, dtype, stream):
-    """A buffer of the op's own.  On a stream of the caller's its memory must not go back to the current stream's pool while
-    that one still works on it."""
-    t = alloc_tensor_func(shape, dtype=dtype, device=like.device)
-    if stream is not None:
-        t.record_stream(stream)
+    """A buffer of the op's own.  For a stream of the caller's it comes from that stream's pool (what the current stream's pool hands
+    out may still be in use there, by work that the other stream has not waited for), and goes back once the current stream, where the
+    caller may read it, has done with it too."""
+    if stream is None:
+        return alloc_tensor_func(shape, dtype=dtype, device=like.device)
+    current = torch.cuda.current_stream(like.device)
+    with torch.cuda.stream(stream):
+        t = alloc_tensor_func(shape, dtype=dtype, device=like.device)
+    t.record_stream(current)
     return t
 
 
