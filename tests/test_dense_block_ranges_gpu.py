@@ -208,3 +208,22 @@ def test_bytes_are_those_of_the_quotient(dtype, D, many):
     for cache, held in zip(caches, scales):
         assert torch.equal(held.cpu()[at], scale)
         assert torch.equal(cache.cpu()[at], want)
+
+
+# ------------------------------------------------------------------ attention: values as large as their type's
+
+@pytest.mark.parametrize("D", [128, 40])
+@pytest.mark.parametrize("largest", [3e38, 1.0])
+def test_bf16_values_at_the_end_of_their_range(D, largest):
+    """Scores that grow by e^5.4 inside a share (four tiles of 64 tokens), less than what makes the kernel take a new reference for the
+    weights; one token has a value, so that the result is its weight times it, below f32's end."""
+    n = 128 * 256
+    q, k, v = torch.zeros(1, 1, D, dtype=BF16), torch.zeros(n, 1, D, dtype=BF16), torch.zeros(n, 1, D, dtype=BF16)
+    q[..., 0] = 1
+    k[torch.arange(n) % 256 >= 64, 0, 0] = 5.4
+    v[200] = largest
+    st = state([n], torch.arange(n, dtype=torch.int32)[None].contiguous())
+    want, lse, bound, lse_bound = attend64(q, st, k, v, None, None, 0, 1.0)
+    got, got_lse = ops.paged_decode(q.cuda(), gpu(st), k.cuda(), v.cuda(), sm_scale=1.0, return_lse=True)
+    assert ((got.cpu().double() - want).abs() <= bound).all()
+    assert ((got_lse.cpu().double() - lse).abs() <= lse_bound).all()

@@ -241,8 +241,8 @@ struct Cfg {
   static constexpr uint32_t FULL = TOK == 32 ? 0xffffffffu : 0xffffu;
   // The reference of the weights is a past maximum until one is 2^SLACK above it: sums are rescaled once or twice instead of
   // at every new maximum.  f16 weights are lifted so far that they use all of f16's range above one: 2^7 2^8 = 2^15, and
-  // what is left of them below it is 2^-31 of the reference.
-  static constexpr float SLACK = 8.f, LIFT = std::is_same<M, __half>::value ? 7.f : 0.f;
+  // what is left of them below it is 2^-31 of the reference.  bf16 ones are let down to at most one: values may be as large as f32's.
+  static constexpr float SLACK = 8.f, LIFT = std::is_same<M, __half>::value ? 7.f : -SLACK;
 };
 
 // What the ring holds besides rows: which tokens count, and (read where a run begins or ends) of which item.
