@@ -227,3 +227,19 @@ def test_bf16_values_at_the_end_of_their_range(D, largest):
     got, got_lse = ops.paged_decode(q.cuda(), gpu(st), k.cuda(), v.cuda(), sm_scale=1.0, return_lse=True)
     assert ((got.cpu().double() - want).abs() <= bound).all()
     assert ((got_lse.cpu().double() - lse).abs() <= lse_bound).all()
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("n_in", [512, 509])
+@pytest.mark.parametrize("x_size,scale", [(1e33, 1e-33), (1e-33, 1e33)])
+def test_bf16_sums_whose_products_pass_f32(packed, n_in, x_size, scale):
+    """Sums of some 1e33, whose products with 1e6 are beyond f32 before the adapter's scale brings them back; and small ones."""
+    g = torch.Generator().manual_seed(9)
+    rows, r, n_out = 70, 16, 64
+    x, a = randn(g, rows, n_in, scale=x_size, dtype=BF16), randn(g, 1, n_in, r, scale=n_in ** -0.5, dtype=BF16)
+    b = randn(g, 1, r, n_out, scale=1e6 if scale < 1 else 1e-6, dtype=BF16)
+    y, s = randn(g, rows, n_out, dtype=BF16), torch.tensor([scale])
+    how = _rows([0, 66, rows], rows) if packed else _rows(None, rows)
+    want, bound, _ = adapters64(y, x, a, b, torch.tensor(how["adapter"]), s, how.get("cu"))
+    got = _adapters(y, x, a, b, scale=s, **how)
+    assert ((got.double() - want).abs() <= bound).all(), ((got.double() - want).abs() - bound).max().item()

@@ -47,8 +47,8 @@ __global__ void __launch_bounds__(256) expand_any_kernel(const __grid_constant__
   float s = 0.f;
   if (i >= 0) {
     const T* b = reinterpret_cast<const T*>(p.b) + (int64_t)i * p.b_stride_i + c;
-    for (int r = 0; r < p.rank; ++r) s = fmaf(h[(int64_t)n * p.rank + r], wide(b[(int64_t)r * p.b_stride_r]), s);
-    if (p.scale != nullptr) s *= p.scale[i];
+    const float scale = p.scale != nullptr ? p.scale[i] : 1.f;  // (on h: its products with B alone may pass f32's range)
+    for (int r = 0; r < p.rank; ++r) s = fmaf(scale * h[(int64_t)n * p.rank + r], wide(b[(int64_t)r * p.b_stride_r]), s);
   }
   const float y = wide(reinterpret_cast<const T*>(p.y)[(int64_t)n * p.y_stride + c]);
   reinterpret_cast<T*>(p.out)[(int64_t)n * p.out_stride + c] = narrow<T>(y + s);
@@ -443,15 +443,16 @@ struct Shrink {
   static constexpr int STAGE = kTileRows * X_PITCH + K * A_PITCH;
   static constexpr int LD = RP + 4;  // of the warps' sums (four more words a row: no bank twice)
 };
-// h of packed rows between the two kernels, rounded once to the rows' type.  x A has f32's range, which f16 has not: f16 rows are
-// stored times the power of two that brings their largest to 2^14 .. 2^15 (what is below it keeps all 11 bits down to 2^-28 of it).
+// h of packed rows between the two kernels, rounded once to the rows' type.  x A has f32's range, which f16 has not, and its products with
+// B may pass it where scale brings them back: rows are stored times the power of two that brings their largest to 2^14 .. 2^15
+// (what is below it keeps all 11 bits of f16 down to 2^-28 of it).
 // Why 16 bits: the error against 64 bits is 2.15e-4 in f16 and 1.76e-3 in bf16 (an adapter's share of a third of y, rank 64), where the
 // result's own rounding is 2.08e-4 and 1.66e-3; a second 16-bit term takes that away for twice the products (7095 rows of
 // 4096 to 11008: rank 64 89 us and 106 with it, rank 128 146 and 186).
 template <typename T>
 struct PackedH {
   T* rows;      // [rows][rp], rp: the rank rounded up to 16
-  float* back;  // [rows] the inverse of the row's factor, f16 only
+  float* back;  // [rows] the inverse of the row's factor
 };
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
@@ -613,15 +614,12 @@ shrink_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const Packe
       if (isfinite(v[j].x)) amax = fmaxf(amax, fabsf(v[j].x));
       if (isfinite(v[j].y)) amax = fmaxf(amax, fabsf(v[j].y));
     }
-    float up = 1.f;
-    if constexpr (std::is_same<T, __half>::value) {
 #pragma unroll
-      for (int o = 1; o < G; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      // (a sum of products of f16 values is 0 or a multiple of 2^-48 below 2^63)
-      const int e = amax > 0.f ? (__float_as_int(amax) >> 23) - 127 - 14 : 0;
-      up = power_of_two(-e);
-      if (on && member == 0) h.back[tile.row + row] = power_of_two(e);
-    }
+    for (int o = 1; o < G; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    // (below 2^-112 nothing is left of the row in a product with 16-bit values that counts)
+    const int e = amax > 0.f ? max(-126, (__float_as_int(amax) >> 23) - 127 - 14) : 0;
+    const float up = power_of_two(-e);
+    if (on && member == 0) h.back[tile.row + row] = power_of_two(e);
 #pragma unroll
     for (int j = 0; j < PAIRS; ++j) {
       const int r = 2 * (member + j * G);
@@ -717,13 +715,13 @@ expand_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const Packe
       copy16(hd + row * h_pitch + r * 2, h.rows + (on ? (int64_t)(tile.row + row) * rp + r : 0), on);
     }
     copies_commit();
-    float back[kMt][2];  // of rows g and g + 8 of every 16: the adapter's scale, and of f16 rows what their factor takes back
+    float back[kMt][2];  // of rows g and g + 8 of every 16: the adapter's scale, and what the row's factor takes back
 #pragma unroll
     for (int i = 0; i < kMt; ++i)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = warp * kWarpRows + 16 * i + 8 * e + g;
-        back[i][e] = std::is_same<T, __half>::value && row < tile.rows ? scale * __ldcg(h.back + tile.row + row) : scale;
+        back[i][e] = row < tile.rows ? scale * __ldcg(h.back + tile.row + row) : 0.f;
       }
     const uint32_t ha = hd + (warp * kWarpRows + (lane & 15)) * h_pitch + (lane >> 4) * 16;
     uint32_t hr[HK > 0 ? HK : 1][kMt][4];
