@@ -171,37 +171,18 @@ struct Divisor {  // n / d for n < 2^31
 };
 
 template <typename T>
-struct Pair;
-template <>
-struct Pair<__half> {
-  static __device__ __forceinline__ float2 open(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-  static __device__ __forceinline__ uint32_t close(float x, float y) {
-    const __half2 h = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-};
-template <>
-struct Pair<__nv_bfloat16> {
-  static __device__ __forceinline__ float2 open(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v)); }
-  static __device__ __forceinline__ uint32_t close(float x, float y) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-};
-
-template <typename T>
 __device__ __forceinline__ void open8(const uint4& v, float (&f)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float2 t = Pair<T>::open(w[i]);
+    const float2 t = two<T>(w[i]);
     f[2 * i] = t.x;
     f[2 * i + 1] = t.y;
   }
 }
 template <typename T>
 __device__ __forceinline__ uint4 close8(const float (&f)[8]) {
-  return make_uint4(Pair<T>::close(f[0], f[1]), Pair<T>::close(f[2], f[3]), Pair<T>::close(f[4], f[5]), Pair<T>::close(f[6], f[7]));
+  return make_uint4(both<T>(f[0], f[1]), both<T>(f[2], f[3]), both<T>(f[4], f[5]), both<T>(f[6], f[7]));
 }
 template <typename F>
 __device__ __forceinline__ uint2 bytes8(const float (&f)[8], F byte) {

@@ -136,36 +136,10 @@ constexpr int kWarps = 4, kThreads = kWarps * 32;
 // 24 us with at most 128, 48 with all of the GPU's, whose partials one block has to join)
 constexpr int kMaxSms = 160, kMaxCtas = 4, kMaxParts = 128;
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool on) {  // zeros where it is not on
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() {
-  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
-__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
-}
 __device__ __forceinline__ uint32_t turned(uint32_t v) {  // an 8 x 8 fragment of 16-bit values, transposed
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
   return r;
-}
-template <typename M>
-__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  if constexpr (sizeof(M) == 2 && std::is_same<M, __half>::value)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_s8_s8(int32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -174,28 +148,6 @@ __device__ __forceinline__ void mma_s8_s8(int32_t (&c)[4], const uint32_t (&a)[4
 __device__ __forceinline__ void mma_s8_u8(int32_t (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
       : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <typename M>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <typename M>
-__device__ __forceinline__ float2 unpack2(uint32_t v);
-template <>
-__device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
-  return __half22float2(*reinterpret_cast<const __half2*>(&v));
-}
-template <>
-__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
-  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
 }
 // bytes of u (signed values + 128) at two places -> f16 pair: 0x64 on top of a byte is 1024 + byte
 template <uint32_t kPlaces>
@@ -210,7 +162,6 @@ __device__ __forceinline__ void touch(const void* p) {
   uint32_t ignored;
   asm volatile("ld.global.ca.b32 %0, [%1];\n" : "=r"(ignored) : "l"(p));
 }
-__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
@@ -483,7 +434,7 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
               const int d = C::I8 ? 32 * (k / 2) + 2 * (k & 1) + 16 * e + 4 * c4 : 16 * k + 2 * c4 + 8 * e;
               q[j][k][e] = on ? *reinterpret_cast<const uint32_t*>(qr + d) : 0u;
               if constexpr (C::I8) {
-                const float2 f = unpack2<T>(q[j][k][e]);
+                const float2 f = two<T>(q[j][k][e]);
                 amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
                 finite &= fabsf(f.x) < INFINITY && fabsf(f.y) < INFINITY;
               }
@@ -500,7 +451,7 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
             for (int k = 0; k < D / 16; k += 2)
 #pragma unroll
               for (int t = 0; t < 2; ++t) {
-                const float2 f0 = unpack2<T>(q[j][k][t]), f1 = unpack2<T>(q[j][k + 1][t]);
+                const float2 f0 = two<T>(q[j][k][t]), f1 = two<T>(q[j][k + 1][t]);
                 const int v[4] = {__float2int_rn(f0.x * up), __float2int_rn(f0.y * up), __float2int_rn(f1.x * up), __float2int_rn(f1.y * up)};
                 uint32_t high = 0, mid = 0, low = 0;
 #pragma unroll
@@ -542,7 +493,7 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
             uint32_t a[4];
             ldmatrix4(a, C::skip(k_base + u * 16 * C::PITCH, 2 * k));
 #pragma unroll
-            for (int j = 0; j < NT; ++j) mma<M>(part[u][j][k % SUMS], a[0], a[1], a[2], a[3], q[j][k][0], q[j][k][1]);
+            for (int j = 0; j < NT; ++j) mma<M>(part[u][j][k % SUMS], a, q[j][k][0], q[j][k][1]);
           }
 #pragma unroll
         for (int u = 0; u < C::SUBS; ++u)
@@ -666,10 +617,10 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
               l[j][i] += w[i];
               if (C::I8) w[i] *= sv[u][e];
             }
-            const uint32_t h = pack2<M>(w[0], w[1]);
-            const float2 f = unpack2<M>(h);
+            const uint32_t h = both<M>(w[0], w[1]);
+            const float2 f = two<M>(h);
             hi_b[j][e] = turned(h);
-            lo_b[j][e] = turned(pack2<M>(w[0] - f.x, w[1] - f.y));
+            lo_b[j][e] = turned(both<M>(w[0] - f.x, w[1] - f.y));
           }
         // ---- values: rows dims, columns heads
         if constexpr (!C::I8) {
@@ -680,8 +631,8 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
             ldmatrix4_trans(a, C::skip(base, 2 * t));
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-              mma<M>(acc[t][j], a[0], a[1], a[2], a[3], hi_b[j][0], hi_b[j][1]);
-              mma<M>(acc[t][j], a[0], a[1], a[2], a[3], lo_b[j][0], lo_b[j][1]);
+              mma<M>(acc[t][j], a, hi_b[j][0], hi_b[j][1]);
+              mma<M>(acc[t][j], a, lo_b[j][0], lo_b[j][1]);
             }
           }
         } else {
@@ -694,12 +645,11 @@ paged_decode_kernel(const __grid_constant__ WsvdPagedDecodeParams p, const Parti
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const uint32_t x = r[2 * e] ^ 0x80808080u, y = r[2 * e + 1] ^ 0x80808080u;
-              const uint32_t a0 = bytes_to_f16<0x4240>(x), a1 = bytes_to_f16<0x4341>(x), a2 = bytes_to_f16<0x4240>(y),
-                             a3 = bytes_to_f16<0x4341>(y);
+              const uint32_t a[4] = {bytes_to_f16<0x4240>(x), bytes_to_f16<0x4341>(x), bytes_to_f16<0x4240>(y), bytes_to_f16<0x4341>(y)};
 #pragma unroll
               for (int j = 0; j < NT; ++j) {
-                mma<M>(acc[t + e][j], a0, a1, a2, a3, hi_b[j][0], hi_b[j][1]);
-                mma<M>(acc[t + e][j], a0, a1, a2, a3, lo_b[j][0], lo_b[j][1]);
+                mma<M>(acc[t + e][j], a, hi_b[j][0], hi_b[j][1]);
+                mma<M>(acc[t + e][j], a, lo_b[j][0], lo_b[j][1]);
               }
             }
           }
