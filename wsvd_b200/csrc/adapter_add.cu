@@ -297,10 +297,11 @@ expand_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* 
 // the input's length is cut into slices over the CTAs of a cluster, so that every SM has work, and their sums meet in
 // shared memory in a fixed order (left to the expanding CTAs in f32 they cost those 12 us).  h is rounded once to the 16-bit
 // type (PackedH, below).  Expand: tiles of 128 rows, equal shares of (tile, 64 columns) over the CTAs that the GPU holds at once; a warp has 32 rows and, up to 64 ranks, keeps
-// their h in registers (what is in shared memory twice is what bounds it: 64-row tiles 97 us, 128 rows 92, with h in registers 89;
+// their h in registers (less that is read from shared memory twice: 64-row tiles 97 us, 128 rows 92, with h in registers 89;
 // 256 threads, or a third stage and a CTA less on the SM, 100 and 104).  B's columns come from L2 and y's from memory a unit ahead,
 // y + product in place in shared memory, 16-byte stores.  7095 rows of 4096 to 11008, rank 64: 89 us, 4.2 TB/s of
-// x, y and out (96 where the card is at its power limit).
+// x, y and out (97 to 99 where the card is at its power limit): twelve warps an SM that wait for shared memory and for each other; neither
+// it (60 %) nor HBM (51 %) is at its limit.
 constexpr int kTileRows = 64, kTileCols = 64, kPackThreads = 128, kColPieces = kTileCols / 8;
 
 // The row tiles of the batch, numbered through the requests in order; what is behind the last one and in front of the first
@@ -382,7 +383,7 @@ __device__ __forceinline__ void stmatrix4(uint32_t addr, const uint32_t (&r)[4])
 }
 // RP: the rank rounded up to 16, 32, 64, 128 or 256.  Pitches are an odd number of 16-byte pieces (conflict-free ldmatrix).
 // Up to 64 ranks a warp takes half of the rows and every other 16 inputs, so that A is read from shared memory twice and not
-// four times (shared memory is what bounds the loop: 56 KB a stage with the rows alone dealt out, 40 KB so, 32 KB with the
+// four times (its reads are what the loop waits for: 56 KB a stage with the rows alone dealt out, 40 KB so, 32 KB with the
 // inputs alone, whose 128 accumulators cost a resident CTA); above, a warp takes 16 rows.
 template <int RP>
 struct Shrink {

@@ -119,8 +119,9 @@ __global__ void __launch_bounds__(kAnyWarps * 32) paged_decode_any_kernel(const 
 // as partial sums, which paged_merge_kernel joins in a fixed order.
 //
 // Measured, a call: 16 sequences of 4096, 40 heads of 128, f16: 212 us, 6.3 TB/s of cache (a plain copy: 6.56); 32 of 300 to 8192,
-// 32 heads on 8, bf16: 86 us, 5.7 TB/s; 48 in a window of 4096, heads of 64: 63 us, 5.3 TB/s; bytes, 8 of up to 32768: 69 to 75 us, 5.1
-// to 4.7 TB/s (bound by instructions: six matrix products a 16 tokens and 32 dims, values converted one by one); one of 2048: 14 us,
+// 32 heads on 8, bf16: 86 us, 5.7 TB/s; 48 in a window of 4096, heads of 64: 63 us, 5.3 TB/s; bytes, 8 of up to 32768: 69 to 78 us, 5.1
+// to 4.5 TB/s (twelve warps an SM wait for their own instructions: seven matrix products a 16 tokens and 32 dims, values converted one by
+// one); one of 2048: 14 us,
 // of which the page table, the rows and the merge wait for one another 10 (at other batches 4 us are the ends of the call).
 //
 // Weights go into the product as two 16-bit terms (17 bits of bf16, 22 of f16): the one rounding that is left is the
