@@ -243,3 +243,30 @@ def test_bf16_sums_whose_products_pass_f32(packed, n_in, x_size, scale):
     want, bound, _ = adapters64(y, x, a, b, torch.tensor(how["adapter"]), s, how.get("cu"))
     got = _adapters(y, x, a, b, scale=s, **how)
     assert ((got.double() - want).abs() <= bound).all(), ((got.double() - want).abs() - bound).max().item()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("D", [128, 40])
+def test_bytes_at_the_ends_of_the_scale(dtype, D):
+    """Rows whose scale is among f16's subnormals, below them, at f16's end and beyond it, 0, infinite and NaN: the same formula, the scale
+    kept inside f16, NaN as the lowest byte, as latent_quant_append has it."""
+    g = torch.Generator().manual_seed(D)
+    sizes = [127 * 6.2e-5, 127 * 3e-5, 127 * 1e-6, 6e-6, 1e-7, 0.0, 60000.0] + ([1e4 * 127, 6.6e4 * 127, 1e30, 3e38] if dtype is BF16 else [])
+    rows = torch.stack([(torch.rand(D, generator=g) * 2 - 1) * s for s in sizes for _ in range(5)]).to(dtype)
+    special = randn(g, 6, D, dtype=dtype)
+    special[0, 3], special[1, 3], special[2, 7], special[3] = float("inf"), float("-inf"), float("nan"), float("nan")
+    special[4, 1], special[4, 2] = float("nan"), float("inf")
+    x = torch.cat([rows, special])[:, None]
+    n = len(x)
+    caches = [torch.zeros(n, 1, D, dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros(n, 1, dtype=torch.float16, device="cuda") for _ in range(2)]
+    st = gpu(state([0], torch.arange(n, dtype=torch.int32)[None].contiguous()))
+    ops.kv_rope_append(x.cuda(), x.cuda(), st, *caches, torch.zeros(0, device="cuda"), cache_k_scale=scales[0], cache_v_scale=scales[1],
+                       cu_new=torch.tensor([0, n], dtype=torch.int32).cuda())
+    f = x.float()
+    amax = torch.nan_to_num(f.abs(), nan=0.0, posinf=float("inf")).amax(-1)
+    scale = torch.where(amax == 0, torch.ones(()), (amax / 127).clamp(2.0 ** -24, 65504.0)).half()
+    want = torch.nan_to_num((f / scale.float()[..., None]).round().clamp(-128, 127), nan=-128.0).to(torch.int8)
+    for cache, held in zip(caches, scales):
+        assert torch.equal(held.cpu(), scale)
+        assert torch.equal(cache.cpu(), want)

@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kAnyWarps * 32) paged_decode_any_kernel(const 
 // Weights go into the product as two 16-bit terms (17 bits of bf16, 22 of f16): the one rounding that is left is the
 // result's.  int8 keys meet their queries as bytes: a query row is taken to 24 bits below its largest value (a power of two
 // times it, so that bf16 ones of any size fit) and split into three bytes, whose products with the keys' are exact.  (Two bytes
-// are 4 to 10 % less time where heads are of 256, 1 % where they are of 128, and lose the small values of a row beside one large one: scores
+// are 9 % less time where heads are of 256, 1 % where they are of 128, and lose the small values of a row beside one large one: scores
 // off by up to 0.01 where it is 200 times the others.)  int8
 // values become f16 exactly (a byte under the exponent of 1024); the running maximum is that of score times v scale, so
 // that the weights with the v scale in them stay at or below one.
