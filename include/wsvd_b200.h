@@ -269,7 +269,8 @@ int wsvd_latent_quant_append_i8(const WsvdQuantAppendParams* p, void* stream);
  *   go through.  WSVD_ROPE_HALF pairs (j, j + rot_dim / 2), WSVD_ROPE_INTERLEAVED (2 j, 2 j + 1).
  *   cache_k, cache_v [T, Hkv, D]: the rows' dtype, or int8 with f16 scales [T, Hkv] per (slot, head): the quantiser of
  *   wsvd_latent_quant_append_i8 on the rotated f32 row.
- *   q_out [rows, Hq, D] receives the rotated queries; it may be q itself (same strides), and must not overlap q, k or v otherwise.
+ *   q_out [rows, Hq, D] receives the rotated queries; it may be q itself (same strides), and must not overlap q, k or v
+ *   otherwise, nor the caches, nor they one another.
  *
  * Rows behind cu_new[batch] are padding: nothing of them is stored (q_out: left as it was, or zeroed with clear_tail).  A row
  * whose position is outside [0, max_len) is skipped (status 5), one whose request or slot does not exist too

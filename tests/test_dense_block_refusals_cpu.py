@@ -172,3 +172,20 @@ def test_lengths_that_a_last_step_would_carry_past_32_bits_are_refused():
         for kw in (dict(rows=most), dict(batch=most), dict(n_in=most), dict(rows=most, batch=most, cu_new=None)):
             assert lib.wsvd_adapter_add(ctypes.byref(_adapter_params(**kw)), FAKE, 1 << 60, None) == status
     assert lib.wsvd_adapter_add(ctypes.byref(_adapter_params(n_out=2 ** 31 - 1)), FAKE, 1 << 60, None) == 8
+
+
+def test_outputs_over_one_another_are_refused():
+    """Keys and values of a token would go to one place."""
+    table, T = pages(2, 8, 4, torch.Generator().manual_seed(1))
+    cache = torch.zeros(T + 1, 2, 16, dtype=H16)
+    refused("append", "cache_k and cache_v overlap", cache_k=cache[1:], cache_v=cache[1:])
+    refused("append", "cache_k and cache_v overlap", cache_k=cache[1:], cache_v=cache[:-1])
+    q = torch.zeros(2, 4, 16, dtype=H16)
+    refused("append", "q_out and cache_k overlap", cache_k=cache[1:], q=q, q_out=cache[3:7].view(2, 4, 16))
+    refused("append", "q_out and cache_v overlap", cache_v=cache[1:], q=q, q_out=cache[3:7].view(2, 4, 16))
+    both = torch.zeros(T, 2, 2, 16, dtype=H16)
+    accepted("append", cache_k=both[:, 0], cache_v=both[:, 1])
+    accepted("append", cache_k=both[:, :, 0], cache_v=both[:, :, 1])
+    halves = torch.zeros(2 * T, 2, 16, dtype=H16)
+    accepted("append", cache_k=halves[:T], cache_v=halves[T:])
+    accepted("append", cache_k=halves[::2], cache_v=halves[1::2])

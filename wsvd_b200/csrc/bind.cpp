@@ -169,7 +169,8 @@ struct Append {
            (!cu || vector(cu, batch + 1, at::kInt, device)) && (!off || vector(off, batch, at::kInt, device)) &&
            (q ? rows(q, 3, type, device) && q->size(0) == N && q->size(2) == D : !q_out) &&
            (!q_out || (rows(q_out, 3, type, device) && same_shape(*q, *q_out) && no_overlap(q_out, *q, {k, v}))) &&
-           apart(q_out) && apart(ck) && apart(cv) && apart(ks) && apart(vs) && !differentiated({k, v, q, q_out, ck, cv, ks, vs, inv});
+           apart(q_out) && apart(ck) && apart(cv) && apart(ks) && apart(vs) && !meet(*ck, *cv) &&
+           !(q_out && (meet(*q_out, *ck) || meet(*q_out, *cv))) && !differentiated({k, v, q, q_out, ck, cv, ks, vs, inv});
   }
 };
 

@@ -690,6 +690,9 @@ def _check_append(k, v, lens, idx, table, cache_k, cache_v, inv_freq, cache_k_sc
     for name, t in (("cache_k", cache_k), ("cache_v", cache_v), ("cache_k_scale", cache_k_scale), ("cache_v_scale", cache_v_scale)):
         if t is not None:
             _apart(name, t)
+    for a, b, names in ((cache_k, cache_v, "cache_k and cache_v"), (q_out, cache_k, "q_out and cache_k"), (q_out, cache_v, "q_out and cache_v")):
+        if a is not None and _meet(a, b):
+            raise ValueError(f"{names} overlap")
     _no_gradient("kv_rope_append", k, v, q, q_out, cache_k, cache_v, cache_k_scale, cache_v_scale, inv_freq)
     _on_one_gpu(k=k, v=v, q=q, q_out=q_out, cache_k=cache_k, cache_v=cache_v, cache_k_scale=cache_k_scale,
                 cache_v_scale=cache_v_scale, inv_freq=inv_freq, b_seq_len=lens, b_req_idx=idx, req_to_token_indexs=table,
@@ -708,7 +711,8 @@ def kv_rope_append(k, v, infer_state, cache_k, cache_v, inv_freq, *, cache_k_sca
     adds the new rows afterwards.  The first ``2 * len(inv_freq)`` dims are rotated by ``(position + pos_offset[b]) *
     inv_freq`` (`rope_layout` as in `latent_decode`), the others and v go through.
     cache_k, cache_v [T, Hkv, D] in the rows' dtype, or int8 with f16 scales [T, Hkv] (the quantiser of
-    `latent_quant_append`, on the rotated f32 row).  `q_out` may be q, and shares no memory with q, k or v otherwise.
+    `latent_quant_append`, on the rotated f32 row).  `q_out` may be q, and shares no memory with q, k or v otherwise, nor do
+    the outputs with one another.
 
     Rows behind cu_new[B] are padding: nothing of them is stored, a `q_out` of the caller's keeps its rows, the op's own has
     zeros there.  A row without a place in the table or the cache is skipped and reported by `kernel_status`.  No two rows may
