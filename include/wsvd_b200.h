@@ -310,7 +310,7 @@ int wsvd_kv_rope_append(const WsvdKvRopeAppendParams* p, void* stream);
  * exp(sm_scale q . k_s).  A sequence without positions gives zeros and -inf.
  * What is stored in slots that no position of the call names is never read.  A page-table entry outside [0, T) is left out
  * as if it were masked, a request outside the table leaves its sequence empty (status 7); a length beyond max_len is
- * clamped to it (status 5).  out may be q itself (same strides), and must not overlap q or the caches otherwise.
+ * clamped to it (status 5).  max_len < 2^31 - 4096.  out may be q itself (same strides), and must not overlap q or the caches otherwise.
  * wsvd_dense_decode_f16 is the reference's dense baseline (f16, each query head for itself); this is the serving form.
  */
 typedef struct WsvdPagedDecodeParams {

@@ -296,8 +296,9 @@ expand_step_kernel(const __grid_constant__ WsvdAdapterAddParams p, const float* 
 // Bound by x, y and out.  Shrink: a warp has 16 rows and all ranks, tiles of 64 inputs come by 16-byte asynchronous copies;
 // the input's length is cut into slices over the CTAs of a cluster, so that every SM has work, and their sums meet in
 // shared memory in a fixed order (left to the expanding CTAs in f32 they cost those 12 us).  h is rounded once to the 16-bit
-// type (PackedH, below).  Expand: tiles of 128 rows, equal shares of (tile, 64 columns) over the CTAs that the GPU holds at once; a warp has 32 rows and, up to 64 ranks, keeps
-// their h in registers (less that is read from shared memory twice: 64-row tiles 97 us, 128 rows 92, with h in registers 89;
+// type (PackedH, below).  Expand: tiles of 128 rows, equal shares of (tile, 64 columns) over the CTAs that the GPU holds at once; a
+// warp has 32 rows and, up to 64 ranks, keeps their h in registers (less that is read from shared memory twice: 64-row tiles
+// 97 us, 128 rows 92, with h in registers 89;
 // 256 threads, or a third stage and a CTA less on the SM, 100 and 104).  B's columns come from L2 and y's from memory a unit ahead,
 // y + product in place in shared memory, 16-byte stores.  7095 rows of 4096 to 11008, rank 64: 89 us, 4.2 TB/s of
 // x, y and out (97 to 99 where the card is at its power limit): twelve warps an SM that wait for shared memory and for each other; neither
@@ -566,7 +567,7 @@ shrink_packed_kernel(const __grid_constant__ WsvdAdapterAddParams p, const Packe
     }
 #pragma unroll
     for (int o = 1; o < G; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    // (below 2^-112 nothing is left of the row in a product with 16-bit values that counts)
+    // (rows below 2^-112 are brought up by 2^126, the largest factor whose inverse is no subnormal)
     const int e = amax > 0.f ? max(-126, (__float_as_int(amax) >> 23) - 127 - 14) : 0;
     const float up = power_of_two(-e);
     if (on && member == 0) h.back[tile.row + row] = power_of_two(e);
@@ -879,7 +880,8 @@ extern "C" {
 
 size_t wsvd_adapter_add_workspace_bytes(const WsvdAdapterAddParams* p) {
   if (!p || p->rows <= 0 || p->rank <= 0 || p->n_in <= 0 || p->batch < 0) return 0;
-  // packed rows: h in f32 or, its rows padded, in 16 bits with a factor a row (the padding only to 16: no more); one row per request: a sum per slice of the input
+  // packed rows: h in f32 or, its rows padded to 16s, in 16 bits with a factor a row, which is no more; one row per request: a sum per
+  // slice of the input
   if (p->cu_new) return (size_t)p->rows * (p->rank < 16 ? 16 : p->rank) * sizeof(float);
   return (size_t)wsvd::slices_of(*p) * p->rows * p->rank * sizeof(float);
 }

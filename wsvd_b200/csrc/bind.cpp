@@ -163,7 +163,8 @@ struct Append {
     const at::Device device = k->device();
     const int64_t N = k->size(0), H = k->size(1), D = k->size(2);
     batch = cu ? cu->dim() == 1 ? cu->size(0) - 1 : -1 : N;
-    return batch >= 0 && countable({N, H, q && q->dim() == 3 ? q->size(1) : 0}) && rows(k, 3, type, device) && rows(v, 3, type, device) && same_shape(*k, *v) && H > 0 && D >= 2 && D % 2 == 0 && D <= 256 &&
+    return batch >= 0 && countable({N, H, q && q->dim() == 3 ? q->size(1) : 0}) && rows(k, 3, type, device) && rows(v, 3, type, device) &&
+           same_shape(*k, *v) && H > 0 && D >= 2 && D % 2 == 0 && D <= 256 &&
            inv && inv->dim() == 1 && vector(inv, inv->size(0), at::kFloat, device) && 2 * inv->size(0) <= D &&
            cache_fits(ck, cv, ks, vs, type, H, D, device) && metadata_fits(lens, idx, table, batch, device) &&
            (!cu || vector(cu, batch + 1, at::kInt, device)) && (!off || vector(off, batch, at::kInt, device)) &&
@@ -321,7 +322,8 @@ struct Adapters {
     const at::ScalarType type = x->scalar_type();
     const at::Device device = x->device();
     const int64_t N = x->size(0), in = x->size(1), columns = y->size(1), count = a->size(0), rank = a->size(2), B = adapter->size(0);
-    return countable({N, in, columns, count, B}) && rows(x, 2, type, device) && rows(y, 2, type, device) && rows(a, 3, type, device) && rows(b, 3, type, device) && y->size(0) == N &&
+    return countable({N, in, columns, count, B}) && rows(x, 2, type, device) && rows(y, 2, type, device) && rows(a, 3, type, device) &&
+           rows(b, 3, type, device) && y->size(0) == N &&
            a->size(1) == in && b->size(0) == count && b->size(1) == rank && b->size(2) == columns && rank >= 1 && rank <= 256 && in > 0 &&
            columns > 0 && vector(adapter, B, at::kInt, device) && (!scale || vector(scale, count, at::kFloat, device)) &&
            (cu ? vector(cu, B + 1, at::kInt, device) : B == N) &&

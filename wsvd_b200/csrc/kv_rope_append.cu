@@ -30,9 +30,10 @@ __device__ __forceinline__ void rotation(int64_t place, float freq, float* sn, f
 // A value in steps of the scale, rounded to even: the low byte of the answer.
 __device__ __forceinline__ uint32_t byte_of(float x, float scale) { return (uint32_t)(int)fminf(fmaxf(rintf(x / scale), -128.f), 127.f); }
 
-// The same from x times 1 / scale (a division a value took 43 us for 5665 rows, the product without a look at
-// the middle 32, with it 34.5), for scales that are f16's own max|x| / 127, neither among its subnormals nor at its end, so that the product is between -128 and 128; `open` where it may
-// not be the quotient's.  The low byte again: adding 1.5 2^23 rounds to a whole number, to even, and leaves it in the last bits.
+// The same from x times 1 / scale (a division a value took 43 us for 5665 rows, the product without a look at the middle 32, with it
+// 34.5), for scales that are f16's own max|x| / 127, neither among its subnormals nor at its end, so that the product is between
+// -128 and 128; `open` where it may not be the quotient's.  The low byte again: adding 1.5 2^23 rounds to a whole
+// number, to even, and leaves it in the last bits.
 // Up to 2^-15 before the middle of two steps the product rounds as the quotient does: 1 / scale and the product are each off by 2^-24,
 // together by 2^-16 at 128 steps.  (The quotient itself comes to lie on the middle only if x does: the middle times an f16 scale is an
 // f32 value.)  NaN is on no side.
@@ -197,7 +198,8 @@ __device__ __forceinline__ uint2 bytes8(const float (&f)[8], F byte) {
 }
 
 // lanes: log2 of the lanes of a head (D / 16 rounded up to a power of two); per_row: units of a row; U: units of a thread
-// (bytes, four units: three blocks an SM, so that bf16 ones have the registers for it; with the four of 64 registers they spill: 35.2 us, 34.5 so; 0: as the compiler chooses)
+// (bytes, four units: three blocks an SM, so that bf16 ones have the registers for it; with the four of 64 registers they spill: 35.2 us,
+// 34.5 so; 0: as the compiler chooses)
 template <typename T, bool I8, int U>
 __global__ void __launch_bounds__(kVecThreads, I8 && U == 4 ? 3 : 0)
 kv_append_vec_kernel(const __grid_constant__ WsvdKvRopeAppendParams p, const int lanes, const Divisor per_row, const int most_rows) {

@@ -885,8 +885,9 @@ def adapter_add(y, x, a, b, adapter, *, scale=None, cu_new=None, out=None, works
     x [N, n_in], y [N, n_out] (the projection's result), a [n_adapters, n_in, rank], b [n_adapters, rank, n_out], all f16 or all
     bf16 (rows at any stride: y and out may be column slices); adapter [B] int32; scale [n_adapters] f32, None means
     1.  Rows are packed by request, `cu_new` [B + 1] int32 as in `kv_rope_append` (None: one row per request).  Returns
-    out; `out=y` adds in place (an `out` that has memory of y, x, a or b otherwise is refused).  x a is summed in f32 (and, of packed rows, rounded to their type's number
-    of bits, with the range of f32).  Rows behind cu_new[B] are padding: a caller's `out` keeps its rows, the op's own has y's there.  An adapter that does not exist adds nothing and is reported by `kernel_status`.
+    out; `out=y` adds in place (an `out` that has memory of y, x, a or b otherwise is refused).  x a is summed in f32 (and, of packed
+    rows, rounded to their type's number of bits, with the range of f32).  Rows behind cu_new[B] are padding: a caller's `out` keeps its
+    rows, the op's own has y's there.  An adapter that does not exist adds nothing and is reported by `kernel_status`.
     `workspace`: an optional CUDA buffer of `adapter_add_workspace_bytes` bytes; calls that may run at the same time need one
     each."""
     if stream is None and alloc_tensor_func is torch.empty:
